@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define KF_ABI_VERSION 6
+#define KF_ABI_VERSION 7
 
 enum kf_status {
   KF_OK = 0,
@@ -258,6 +258,81 @@ int kf_attn_append_decode(const void* q, void* k_cache, void* v_cache, const voi
                           const int64_t* new_v_strides, const int64_t* o_strides, float scale,
                           int num_splits, int dtype, void* workspace, size_t workspace_bytes,
                           void* stream);
+
+/*
+ * Paged K/V cache. Keys and values lie in pools [num_pages, Hkv, page_size, D]
+ * (strides int64_t[3] {page, head, row}, unit head_dim stride, multiples of 8
+ * elements), shared by all requests of a batch. A page table is int32 device
+ * memory: tables [B, columns] (row stride table_stride), the pages of each
+ * request in order, -1 where it has none; lengths [B], its tokens; free_pages
+ * [num_pages], a stack of the pages that belong to no request; counters [4]:
+ * the stack's height, the requests that the last reserve refused, and two
+ * that the library uses, 0 between calls. Position j of request b lies in
+ * page tables[b, j / page_size], row j % page_size; its slot is that page
+ * times page_size plus that row. Nothing of it is read on the host, so every
+ * call can be captured and replayed. A table is changed by one call at a time;
+ * several layers' pools may share one. No reference counterpart: its cache is
+ * one contiguous buffer (kotflash/cache.py:91-290).
+ */
+
+/*
+ * Room for counts[b] (device int32 [B]; null: `count` each) more tokens of
+ * every request, in the requests' order. Request b is refused when its count
+ * is outside [0, width], when its table has too few columns, or when it needs
+ * pages and those asked for by the requests up to it (refused ones included)
+ * are more than the free ones. A served request gets its pages, its length
+ * grows, and slots[b, t] (int64 [B, width], contiguous) names the place of its
+ * new token t < counts[b]; all other entries of slots are -1. A refused request
+ * is left as it was.
+ */
+int kf_page_reserve(int32_t* tables, int32_t* lengths, int32_t* free_pages, int32_t* counters,
+                    const int32_t* counts, int64_t count, int64_t* slots, int64_t width, int64_t B,
+                    int64_t columns, int64_t table_stride, int64_t page_size, int64_t num_pages,
+                    void* stream);
+
+/*
+ * Request b keeps its first min(lengths[b], new_lengths[b]) tokens (device
+ * int32 [B]; null: `new_length` each; a negative entry keeps none). Pages
+ * behind them return to the free stack in the order that undoes the reserve
+ * which took them, and their table entries become -1.
+ */
+int kf_page_trim(int32_t* tables, int32_t* lengths, int32_t* free_pages, int32_t* counters,
+                 const int32_t* new_lengths, int64_t new_length, int64_t B, int64_t columns,
+                 int64_t table_stride, int64_t page_size, int64_t num_pages, void* stream);
+
+/*
+ * pool[slot / page_size, h, slot % page_size, :] = new[b, h, t, :] for slot =
+ * slots[b, t] (device int64 [B, Snew], row stride slots_stride), K and V in one
+ * launch, bit-exact; a slot outside [0, num_pages * page_size) is skipped. The
+ * slots of a call that are not skipped must differ: of two rows with the same
+ * slot either may be stored. new_k/new_v may have any strides (int64_t[4]).
+ */
+int kf_paged_append(void* k_pages, void* v_pages, const void* new_k, const void* new_v,
+                    const int64_t* slots, int64_t B, int64_t H, int64_t Snew, int64_t D,
+                    int64_t num_pages, int64_t page_size, int64_t slots_stride,
+                    const int64_t* k_strides, const int64_t* v_strides,
+                    const int64_t* new_k_strides4, const int64_t* new_v_strides4, int dtype,
+                    void* stream);
+
+/* Workspace for kf_paged_decode in bytes (fp32 partial O and LSE). */
+size_t kf_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);
+
+/*
+ * Attention of q [B, Hq, Sq, D] over the pages: rows of request b see its
+ * positions [0, lengths[b]); with causal != 0 its Sq query tokens are the
+ * request's last, and row i sees [0, lengths[b] - Sq + 1 + i). A row that sees
+ * nothing gives O = 0 and LSE = -inf; positions whose page number is outside
+ * [0, num_pages) are not seen, and lengths count as at most columns *
+ * page_size. page_size is a multiple of 16. Two launches; the split of the
+ * work follows the device lengths. lse (nullable) is fp32 [B, Hq, Sq].
+ */
+int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
+                    const int32_t* tables, const int32_t* lengths, int64_t B, int64_t Hq,
+                    int64_t Hkv, int64_t Sq, int64_t D, int64_t num_pages, int64_t page_size,
+                    int64_t columns, int64_t table_stride, const int64_t* q_strides,
+                    const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides,
+                    float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
+                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@ object: module state, ``isinstance`` checks and monkeypatching are shared.
     kotflash.cache           kotflash_amd.cache
     kotflash._planning       kotflash_amd._planning
     kotflash._cuda_append    kotflash_amd._hip_append (append_kv_cuda)
+    kotflash.paged           kotflash_amd.paged (no reference module)
     kotflash.kernels.*       kotflash.kernels (triton_* names -> hip_* modules)
 
 As in the reference, the package attribute ``kotflash.attention`` is the
@@ -28,6 +29,7 @@ _SUBMODULES = {
     "cache": "kotflash_amd.cache",
     "_planning": "kotflash_amd._planning",
     "_cuda_append": "kotflash_amd._hip_append",
+    "paged": "kotflash_amd.paged",
 }
 for _name, _target in _SUBMODULES.items():
     _sys.modules[f"{__name__}.{_name}"] = _importlib.import_module(_target)
@@ -36,7 +38,7 @@ from . import kernels  # noqa: E402  (registers kotflash.kernels.triton_*)
 from kotflash_amd import __version__, attention, hip_available  # noqa: E402
 from kotflash_amd.kernels.hip_forward import triton_available, triton_turing_supported  # noqa: E402
 
-for _name in ("cache", "_planning", "_cuda_append"):
+for _name in ("cache", "_planning", "_cuda_append", "paged"):
     globals()[_name] = _sys.modules[f"{__name__}.{_name}"]
 del _name, _target
 

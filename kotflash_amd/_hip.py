@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libkotflash_amd.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 KF_F16, KF_BF16 = 0, 1
 KF_BWD_DELTA, KF_BWD_DQ, KF_BWD_DKDV, KF_BWD_DKDV_FIXUP = 1, 2, 4, 8
 KF_BWD_ALL = KF_BWD_DELTA | KF_BWD_DQ | KF_BWD_DKDV | KF_BWD_DKDV_FIXUP
@@ -59,6 +59,13 @@ _SIGNATURES = {
     "kf_attn_append_decode": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                    _I64, _I64, _I64, _I64, _I64P, _I64P, _I64P, _I64P, _I64P,
                                    _I64P, _F, _I, _I, _P, _SZ, _P]),
+    "kf_page_reserve": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
+    "kf_page_trim": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
+    "kf_paged_append": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                             _I64P, _I64P, _I64P, _I64P, _I, _P]),
+    "kf_paged_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "kf_paged_decode": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                             _I64, _I64, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _SZ, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -401,3 +408,63 @@ def append_decode(q, k_cache, v_cache, new_k, new_v, out, lse: Optional[torch.Te
             workspace.numel() * workspace.element_size(), _stream(q.device),
         )
     _check(rc, "kf_attn_append_decode")
+
+
+def page_reserve(tables, lengths, free_pages, counters, counts, slots, *, page_size: int) -> None:
+    """kf_page_reserve: ``counts`` an int or a device int32 [B] tensor."""
+    b, columns = tables.shape
+    on_device = isinstance(counts, torch.Tensor)
+    with _DeviceGuard(tables.device):
+        rc = lib().kf_page_reserve(
+            tables.data_ptr(), lengths.data_ptr(), free_pages.data_ptr(), counters.data_ptr(),
+            counts.data_ptr() if on_device else None, 0 if on_device else counts,
+            slots.data_ptr(), slots.shape[1], b, columns, tables.stride(0), page_size,
+            free_pages.numel(), _stream(tables.device),
+        )
+    _check(rc, "kf_page_reserve")
+
+
+def page_trim(tables, lengths, free_pages, counters, new_lengths, *, page_size: int) -> None:
+    """kf_page_trim: ``new_lengths`` an int or a device int32 [B] tensor."""
+    b, columns = tables.shape
+    on_device = isinstance(new_lengths, torch.Tensor)
+    with _DeviceGuard(tables.device):
+        rc = lib().kf_page_trim(
+            tables.data_ptr(), lengths.data_ptr(), free_pages.data_ptr(), counters.data_ptr(),
+            new_lengths.data_ptr() if on_device else None, 0 if on_device else new_lengths,
+            b, columns, tables.stride(0), page_size, free_pages.numel(), _stream(tables.device),
+        )
+    _check(rc, "kf_page_trim")
+
+
+def paged_append(k_pages, v_pages, new_k, new_v, slots) -> None:
+    b, h, n, d = new_k.shape
+    with _DeviceGuard(k_pages.device):
+        rc = lib().kf_paged_append(
+            k_pages.data_ptr(), v_pages.data_ptr(), new_k.data_ptr(), new_v.data_ptr(),
+            slots.data_ptr(), b, h, n, d, k_pages.shape[0], k_pages.shape[2], slots.stride(0),
+            _strides(k_pages), _strides(v_pages), _strides(new_k), _strides(new_v),
+            dtype_code(k_pages.dtype), _stream(k_pages.device),
+        )
+    _check(rc, "kf_paged_append")
+
+
+@lru_cache(maxsize=256)
+def paged_decode_workspace_bytes(b, hq, hkv, sq, d) -> int:
+    return int(lib().kf_paged_decode_workspace_bytes(b, hq, hkv, sq, d))
+
+
+def paged_decode(q, k_pages, v_pages, out, lse: Optional[torch.Tensor], tables, lengths, *,
+                 scale: float, causal: bool, workspace: torch.Tensor) -> None:
+    b, hq, sq, d = q.shape
+    num_pages, hkv, page_size, _ = k_pages.shape
+    with _DeviceGuard(q.device):
+        rc = lib().kf_paged_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
+            lse.data_ptr() if lse is not None else None, tables.data_ptr(), lengths.data_ptr(),
+            b, hq, hkv, sq, d, num_pages, page_size, tables.shape[1], tables.stride(0),
+            _strides(q), _strides(k_pages), _strides(v_pages), _strides(out), float(scale),
+            int(bool(causal)), dtype_code(q.dtype), workspace.data_ptr(), workspace.nbytes,
+            _stream(q.device),
+        )
+    _check(rc, "kf_paged_decode")

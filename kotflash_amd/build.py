@@ -54,6 +54,7 @@ FILE_FLAGS = {
     "bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

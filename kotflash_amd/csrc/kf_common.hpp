@@ -333,6 +333,18 @@ __device__ inline float wave_group16_sum(float x) {
   return wave_xor32_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// Inclusive sum over the wave: shifts within rows of 16 lanes, then
+// lane 15 of a row and lane 31 of a half added to those behind.
+__device__ inline int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
 // Wave index inside the workgroup as a wave-uniform (scalar) value, so that
 // conditions built from it compile to scalar branches.
 __device__ inline int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }

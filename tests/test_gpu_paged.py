@@ -1,0 +1,513 @@
+"""The paged cache's kernels on the GPU, against the definition in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from kotflash_amd import _hip
+from kotflash_amd.paged import PagedKVCache, PageTable, paged_append, paged_attention
+from tests.paged_oracle import Pages, assert_attention, make_case
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _attend(*args, **kw):
+    return paged_attention(*args, backend="hip", return_lse=True, **kw)
+
+
+def _check(case, **kw):
+    o, lse = _attend(*case, **kw)
+    assert_attention(o, *case, lse=lse, **kw)
+    return o, lse
+
+
+# --- attention ---------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [8, 32, 40, 64, 72, 80, 96, 104, 128])
+def test_head_dims(dtype, d):
+    _check(make_case(4, 8, 2, 1, d, 16, [1, 70, 333, 1000], dtype=dtype, seed=d, device="cuda"))
+
+
+@pytest.mark.parametrize("length", [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, 127, 128, 129, 257])
+@pytest.mark.parametrize("page", [16, 48])
+def test_lengths(length, page):
+    """One request alone, and beside others."""
+    _check(make_case(1, 4, 2, 1, 64, page, [length], dtype=F16, seed=length, device="cuda"))
+    _check(make_case(5, 4, 2, 1, 128, page, [length, 0, 40, length, 0], dtype=BF16, seed=length, device="cuda"))
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 80, 256, 1024])
+def test_page_sizes(page):
+    _check(make_case(3, 8, 4, 1, 64, page, [page - 1, page, 3 * page + 5], dtype=F16, seed=page, device="cuda"))
+
+
+@pytest.mark.parametrize("hq,hkv,sq", [(1, 1, 1), (16, 1, 1), (17, 1, 1), (28, 4, 1), (33, 1, 1), (64, 1, 1),
+                                       (65, 1, 1), (8, 8, 3), (8, 2, 5), (16, 2, 4), (32, 2, 16), (4, 1, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows(hq, hkv, sq, causal, d):
+    """1 to 256 packed rows per KV head: one to four row blocks, and several
+    row groups; causal rows of which the first see nothing."""
+    _check(make_case(4, hq, hkv, sq, d, 16, [3, 0, 100, 259], dtype=F16, seed=hq + sq, device="cuda"), causal=causal)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+def test_batches(batch):
+    """Runs of units over many requests, empty ones among them."""
+    rng = random.Random(batch)
+    lengths = [rng.choice([0, 0, 1, rng.randint(1, 400)]) for _ in range(batch)]
+    _check(make_case(batch, 4, 2, 1, 64, 16, lengths, dtype=F16, seed=batch, device="cuda"))
+    _check(make_case(batch, 2, 1, 1, 32, 16, [0] * batch, dtype=BF16, seed=batch, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_long(dtype):
+    """Runs of several steps per worker, requests cut anywhere."""
+    _check(make_case(3, 4, 1, 1, 128, 16, [40000, 7, 29999], dtype=dtype, seed=8, device="cuda"))
+
+
+def test_runs_over_many_segments():
+    """More steps than workers, and many short requests: a run holds whole
+    requests between two parts of others."""
+    rng = random.Random(5)
+    lengths = [rng.randint(0, 90) for _ in range(700)]
+    lengths[300] = 20000
+    _check(make_case(700, 8, 8, 1, 32, 16, lengths, dtype=F16, seed=5, device="cuda"))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0, 1e-3])
+def test_scales(scale):
+    _check(make_case(2, 4, 2, 2, 64, 16, [50, 333], dtype=F16, seed=2, device="cuda"), scale=scale, causal=True)
+
+
+def test_large_scores():
+    """Scores of several hundred, growing along the keys: the running maximum
+    moves at every step."""
+    q, k, v, tables, lengths = make_case(1, 4, 2, 1, 64, 16, [640], dtype=F16, seed=2, device="cuda", values=2.0)
+    for c in range(40):
+        k[tables[0, c]] *= 0.2 * c
+    _check((q, k, v, tables, lengths), scale=0.5)
+
+
+def test_small_probabilities_of_a_long_tail():
+    """One key far above thousands of equal ones, whose P lie below the
+    smallest fp16 number: together they still count."""
+    q, k, v, tables, lengths = make_case(1, 1, 1, 1, 64, 16, [30000], dtype=F16, seed=2, device="cuda")
+    q.fill_(1.0)
+    k.zero_()
+    v.fill_(1.0)
+    first = int(tables[0, 0])
+    k[first, 0, 0] = 18.0 / 64
+    v[first, 0, 0] = 0.0
+    # exp(-18) = 2^-26 each: 30000 of them are 4.6e-4 of the sum.
+    o, lse = _check((q, k, v, tables, lengths), scale=1.0)
+    assert (o > 3e-4).all()
+
+
+def test_what_lies_behind_is_not_read():
+    """NaN, infinities and the type's lowest value behind every request's end
+    and in the pages of nobody change no bit."""
+    for causal in (False, True):
+        got = []
+        for junk in (0.0, math.nan, math.inf, torch.finfo(BF16).min):
+            case = make_case(3, 8, 2, 2, 96, 32, [5, 64, 201], dtype=BF16, seed=6, device="cuda", junk=junk)
+            got.append(_attend(*case, causal=causal))
+        for o, lse in got[1:]:
+            assert torch.equal(o, got[0][0]) and torch.equal(lse, got[0][1])
+
+
+def test_nan_and_infinity_in_sight():
+    """A visible NaN reaches its request's rows and no others; a value that is
+    infinite reaches its column."""
+    q, k, v, tables, lengths = make_case(3, 4, 2, 1, 64, 16, [100, 100, 100], dtype=F16, seed=6, device="cuda")
+    k[tables[1, 2], 0, 3, 5] = math.nan
+    v[tables[2, 0], 1, 0, 7] = math.inf
+    o = _attend(q, k, v, tables, lengths)[0]
+    assert torch.isnan(o[1, :2]).all()
+    assert torch.isinf(o[2, 2:, 0, 7]).all()
+    rest = o.clone()
+    rest[1, :2] = 0
+    rest[2, 2:, 0, 7] = 0
+    assert torch.isfinite(rest).all()
+
+
+def test_pages_outside_the_pool():
+    q, k, v, tables, lengths = make_case(4, 4, 2, 1, 64, 16, [100, 16, 500, 31], dtype=F16, seed=4, device="cuda")
+    tables[0, 1], tables[1, 0], tables[2, 31] = k.shape[0], -1, 2 ** 31 - 1
+    tables[2, 3:9] = -2 ** 31
+    tables[3, 1] = -7
+    o, lse = _check((q, k, v, tables, lengths))
+    assert (o[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
+def test_lengths_outside_the_table():
+    q, k, v, tables, lengths = make_case(3, 4, 2, 1, 64, 16, [96, 20, 33], dtype=F16, seed=5, device="cuda")
+    tables = tables[:, :6]
+    for bad, worth in ((2 ** 31 - 1, 96), (-2 ** 31, 0), (-1, 0), (97, 96)):
+        lengths[0] = bad
+        o, lse = _attend(q, k, v, tables, lengths)
+        fixed = lengths.clone()
+        fixed[0] = worth
+        assert_attention(o, q, k, v, tables, fixed, lse=lse)
+
+
+def test_layouts():
+    """Pools cut from one tensor, head next to row, tables and lengths that
+    are views, queries of any order."""
+    q, k, v, tables, lengths = make_case(3, 8, 2, 2, 64, 32, [40, 0, 150], dtype=F16, seed=7, device="cuda")
+    ref, ref_lse = _attend(q, k, v, tables, lengths, causal=True)
+    pages, hkv, page, d = k.shape
+    both = torch.full((pages, 2, hkv, page, d), math.nan, dtype=F16, device="cuda")
+    both[:, 0], both[:, 1] = k, v
+    rows = torch.full((pages, page, 2, hkv, d + 8), math.nan, dtype=F16, device="cuda")
+    rows[:, :, 0, :, :d], rows[:, :, 1, :, :d] = k.transpose(1, 2), v.transpose(1, 2)
+    wide = torch.full((3, tables.shape[1] + 5), -9, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + tables.shape[1]] = tables
+    spaced = torch.zeros(6, dtype=torch.int32, device="cuda")
+    spaced[::2] = lengths
+    for kp, vp in ((both[:, 0], both[:, 1]),
+                   (rows[:, :, 0, :, :d].transpose(1, 2), rows[:, :, 1, :, :d].transpose(1, 2))):
+        for qq in (q, q.transpose(1, 2).contiguous().transpose(1, 2), q.transpose(2, 3).contiguous().transpose(2, 3),
+                   torch.cat((q, q), 3)[..., 64:]):
+            for tt in (tables, wide[:, 2:2 + tables.shape[1]], tables.t().contiguous().t()):
+                o, lse = _attend(qq, kp, vp, tt, spaced[::2], causal=True)
+                assert torch.equal(o, ref) and torch.equal(lse, ref_lse)
+
+
+def test_shared_pages():
+    """Requests may hold the same pages (a common prompt): reading them is no
+    matter of whose they are."""
+    q, k, v, tables, lengths = make_case(3, 4, 2, 1, 64, 16, [200, 0, 0], dtype=F16, seed=4, device="cuda")
+    tables[1], tables[2] = tables[0], tables[0]
+    lengths[1], lengths[2] = 200, 64
+    _check((q, k, v, tables, lengths))
+
+
+def test_pool_beyond_32_bits():
+    """Element and byte offsets of the last pages pass 2^31 and 2^32."""
+    hkv, page, d = 4, 64, 128
+    pages = 2 ** 32 // (hkv * page * d * 2) + 9 + 2 ** 31 // (hkv * page * d)
+    q, ks, vs, tables, lengths = make_case(2, 8, hkv, 1, d, page, [130, 300], dtype=F16, seed=4)
+    k = torch.empty((pages, hkv, page, d), dtype=F16, device="cuda")
+    v = torch.empty_like(k)
+    k[-len(ks):], v[-len(ks):] = ks.cuda(), vs.cuda()
+    inside = (tables >= 0) & (tables < len(ks))
+    far = torch.where(inside, tables + pages - len(ks), tables)
+    far = torch.where(~inside & (tables >= 0), -1, far)
+    o, lse = _attend(q.cuda(), k, v, far.cuda(), lengths.cuda())
+    tables = torch.where(inside, tables, -1)
+    assert_attention(o, q, ks, vs, tables, lengths, lse=lse)
+    # And the store at the last slots.
+    slots = torch.tensor([[pages * page - 1, pages * page, (pages - 3) * page]], device="cuda")
+    nk, nv = torch.randn(2, 1, hkv, 3, d, device="cuda").to(F16)
+    paged_append(k, v, nk, nv, slots)
+    for pool, new in ((k, nk), (v, nv)):
+        assert torch.equal(pool[-1, :, -1], new[0, :, 0]) and torch.equal(pool[-3, :, 0], new[0, :, 2])
+    del k, v
+    torch.cuda.empty_cache()
+
+
+def test_same_bits_every_time():
+    case = make_case(5, 32, 8, 1, 128, 16, [4000, 17, 900, 2500, 1], dtype=BF16, seed=4, device="cuda")
+    o, lse = _attend(*case)
+    for _ in range(20):
+        again = _attend(*case)
+        assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+    # The rest of the batch does not change what a row sums, only where it is
+    # cut: alone, it agrees within the bound.
+    alone = tuple(t[:1] if i in (0, 3, 4) else t for i, t in enumerate(case))
+    assert_attention(_attend(*alone)[0], *alone)
+
+
+def test_auto_takes_the_kernels(monkeypatch):
+    case = make_case(2, 4, 2, 1, 64, 16, [50, 100], dtype=F16, seed=4, device="cuda")
+    import kotflash_amd.paged as paged
+    expected = _attend(*case)[0]
+    monkeypatch.setattr(paged, "_sdpa_paged", None)
+    assert torch.equal(paged_attention(*case), expected)
+    assert torch.equal(paged_attention(*case, backend="triton"), expected)
+
+
+def test_what_the_kernels_do_not_take():
+    """auto takes sdpa for these, hip refuses them."""
+    for dtype, d, page in ((torch.float32, 64, 16), (F16, 20, 16), (F16, 64, 24), (F16, 136, 16)):
+        case = make_case(2, 4, 2, 1, d, page, [30, 50], dtype=dtype, seed=4, device="cuda")
+        o, lse = paged_attention(*case, return_lse=True)
+        assert_attention(o, *case, lse=lse)
+        with pytest.raises((ValueError, TypeError)):
+            paged_attention(*case, backend="hip")
+    q, k, v, tables, lengths = make_case(2, 4, 2, 1, 64, 16, [30, 50], dtype=F16, seed=4, device="cuda")
+    with pytest.raises(ValueError, match="same device"):
+        paged_attention(q, k, v, tables.cpu(), lengths)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        paged_attention(q.requires_grad_(), k, v, tables, lengths)
+
+
+# --- tables ------------------------------------------------------------------
+
+def _counts(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_table_follows_the_definition(seed):
+    rng = random.Random(seed)
+    batch, page = rng.choice([1, 2, 63, 300, 1023, 1025, 2500]), rng.choice([1, 3, 16, 64, 1000])
+    columns = rng.randint(1, 70)
+    pages = rng.randint(1, batch * columns + 5)
+    table = PageTable(batch, columns * page, num_pages=pages, page_size=page)
+    ref = Pages(batch, columns, pages, page)
+    for _ in range(8):
+        if rng.random() < 0.6:
+            width = rng.choice([1, 1, rng.randint(1, 3 * page), rng.randint(1, min(2000, columns * page))])
+            if rng.random() < 0.3:
+                counts = rng.randint(0, width)
+                assert table.reserve(counts, width=width).tolist() == ref.reserve([counts] * batch, width)
+            else:
+                counts = [rng.choice([-1, width + 1, -2 ** 31, 2 ** 31 - 1]) if rng.random() < 0.02
+                          else rng.randint(0, width) for _ in range(batch)]
+                assert table.reserve(_counts(counts), width=width).tolist() == ref.reserve(counts, width)
+        else:
+            keep = [rng.choice([-2 ** 31, 2 ** 31 - 1, rng.randint(0, columns * page)]) for _ in range(batch)]
+            table.trim(_counts(keep))
+            ref.trim(keep)
+        ref.assert_matches(table)
+    table.trim(0)
+    ref.trim([0] * batch)
+    ref.assert_matches(table)
+    assert sorted(table.free_pages.tolist()) == list(range(pages))
+
+
+def test_torch_and_hip_tables_agree():
+    tables = [PageTable(40, 500, num_pages=300, page_size=16) for _ in range(2)]
+    rng = random.Random(1)
+    for _ in range(10):
+        counts = _counts([rng.randint(0, 90) for _ in range(40)])
+        keep = _counts([rng.randint(0, 400) for _ in range(40)])
+        slots = [t.reserve(counts, width=90, backend=b) for t, b in zip(tables, ("hip", "torch"))]
+        assert torch.equal(*slots)
+        for t, b in zip(tables, ("torch", "hip")):
+            t.trim(keep, backend=b)
+        for name in ("tables", "lengths", "free_pages", "counters"):
+            assert torch.equal(getattr(tables[0], name), getattr(tables[1], name)), name
+
+
+def test_broken_state_stays_inside():
+    """Lengths, tables and counts that no allocator leaves behind: nothing is
+    written outside the table, and slots name places of the pool or -1."""
+    for height, length, entry in ((10 ** 9, 5, 3), (-4, 10 ** 9, -1), (2, -50, 10 ** 9), (8, 2 ** 31 - 1, -2 ** 31)):
+        guard = torch.full((4 + 4, 6 + 2), 77, dtype=torch.int32, device="cuda")
+        table = PageTable(4, 96, num_pages=8, page_size=16)
+        table.tables = guard[2:6, 1:7]
+        table.tables.fill_(entry)
+        table.lengths.fill_(length)
+        table.free_count.fill_(height)
+        for _ in range(2):
+            slots = table.reserve(20)
+            assert slots.shape == (4, 20)
+            table.trim(3)
+        inner = torch.zeros_like(guard, dtype=torch.bool)
+        inner[2:6, 1:7] = True
+        assert (guard[~inner] == 77).all()
+        assert 0 <= table.num_free() <= 8
+
+
+# --- store -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("b,hkv,n,d,page", [(1, 1, 1, 8, 16), (3, 2, 7, 64, 16), (64, 8, 1, 128, 16), (2, 3, 33, 20, 5),
+                                            (5, 4, 130, 96, 48), (2, 16, 9, 128, 1)])
+@pytest.mark.parametrize("layout", ["bhsd", "bshd", "odd"])
+def test_store_is_exact(dtype, b, hkv, n, d, page, layout):
+    g = torch.Generator().manual_seed(n)
+    pages = -(-b * n // page) + 3
+    k = torch.full((pages, hkv, page, d), math.nan, dtype=dtype, device="cuda")
+    v = k.clone()
+    slots = torch.randperm(pages * page, generator=g)[:b * n].reshape(b, n)
+    skip = torch.rand(b, n, generator=g) < 0.2
+    slots[skip] = torch.tensor([-1, pages * page, 2 ** 62, -2 ** 62])[torch.arange(int(skip.sum())) % 4]
+    new = torch.randn(2, b, hkv, n, d, generator=g).to(dtype).cuda()
+    if layout == "bshd":
+        nk, nv = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in new)
+    elif layout == "odd":
+        nk, nv = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in new)
+    else:
+        nk, nv = new
+    paged_append(k, v, nk, nv, slots.cuda(), backend="hip")
+    ek = torch.full((pages, hkv, page, d), math.nan, dtype=dtype, device="cuda")
+    ev = ek.clone()
+    paged_append(ek, ev, *new, slots.cuda(), backend="torch")
+    for got, want in ((k, ek), (v, ev)):
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+def test_store_layouts_of_pool_and_slots():
+    """Pools interleaved in one tensor, offsets that rule out 16-byte rows,
+    slots read from a view."""
+    both = torch.zeros(4, 16, 2, 2, 68, dtype=F16, device="cuda")
+    nk, nv = torch.randn(2, 2, 2, 5, 64, device="cuda").to(F16)
+    wide = torch.randperm(64, device="cuda")[:20].reshape(2, 10)
+    for lo in (0, 2):
+        kp, vp = (both[:, :, i, :, lo:lo + 64].transpose(1, 2) for i in range(2))
+        both.zero_()
+        paged_append(kp, vp, nk, nv, wide[:, ::2], backend="hip")
+        for b in range(2):
+            for t in range(5):
+                s = int(wide[b, 2 * t])
+                assert torch.equal(both[s // 16, s % 16, 0, :, lo:lo + 64], nk[b, :, t])
+                assert torch.equal(both[s // 16, s % 16, 1, :, lo:lo + 64], nv[b, :, t])
+        assert int((both != 0).sum()) <= 2 * 2 * 5 * 2 * 64
+    with pytest.raises(ValueError, match="unit head_dim"):
+        t = torch.zeros(4, 2, 64, 16, dtype=F16, device="cuda").transpose(2, 3)
+        paged_append(t, t.clone(), nk, nv, wide[:, ::2])
+
+
+# --- together ----------------------------------------------------------------
+
+def _serve(table, caches, hq, dtype, steps, seed):
+    """Prompts, steps, drafts of which some are dropped, requests that leave
+    and others that come: checked against each request's own tokens."""
+    g = torch.Generator().manual_seed(seed)
+    rng = random.Random(seed)
+    batch = table.batch
+    d, hkv = caches[0].k_pages.shape[3], caches[0].k_pages.shape[1]
+    own = [[torch.zeros(2, hkv, 0, d, dtype=dtype) for _ in range(batch)] for _ in caches]
+    lens = [0] * batch
+    for step in range(steps):
+        kind = "prompt" if step == 0 else rng.choice(["one", "one", "drafts", "leave"])
+        if kind == "leave":
+            keep = [0 if rng.random() < 0.3 else n for n in lens]
+        elif kind == "one":
+            keep = lens
+        else:
+            keep = [max(0, n - rng.randint(0, 3)) for n in lens]
+        if keep != lens:
+            table.trim(_counts(keep))
+            own = [[x[:, :, :m] for x, m in zip(layer, keep)] for layer in own]
+        n = {"prompt": 70, "leave": 50, "one": 1, "drafts": 4}[kind]
+        counts = [n if kind in ("one", "drafts") else rng.randint(0, n) * (m == 0) for m in keep]
+        slots = table.reserve(_counts(counts), width=n)
+        for cache, layer in zip(caches, own):
+            q = torch.randn(batch, hq, n, d, generator=g).to(dtype)
+            new = torch.randn(2, batch, n, hkv, d, generator=g).to(dtype)
+            nk, nv = (x.cuda().transpose(1, 2) for x in new)
+            if kind in ("one", "drafts"):
+                out = cache.append_and_attend(q.cuda(), nk, nv, slots, causal=kind == "drafts")
+            else:
+                cache.append(nk, nv, slots)
+            for b, c in enumerate(counts):
+                layer[b] = torch.cat((layer[b], new[:, b, :c].transpose(1, 2)), 2)
+            if kind in ("one", "drafts"):
+                most = max(x.shape[2] for x in layer)
+                pools = [torch.zeros(batch, hkv, most, d, dtype=dtype) for _ in range(2)]
+                for b, x in enumerate(layer):
+                    for i in range(2):
+                        pools[i][b, :, :x.shape[2]] = x[i]
+                ids = torch.arange(batch, dtype=torch.int32)[:, None]
+                assert_attention(out, q, *pools, ids, _counts([x.shape[2] for x in layer]).cpu(),
+                                 causal=kind == "drafts")
+        lens = [a + c for a, c in zip(keep, counts)]
+        assert table.lengths.tolist() == lens
+        table.check()
+
+
+@pytest.mark.parametrize("dtype,d,page", [(F16, 64, 16), (BF16, 128, 32), (F16, 80, 48)])
+def test_a_server_s_run(dtype, d, page):
+    table = PageTable(6, 400, num_pages=150, page_size=page)
+    caches = [PagedKVCache(table, 2, d, dtype=dtype) for _ in range(2)]
+    for c in caches:
+        c.k_pages.fill_(math.nan)
+        c.v_pages.fill_(math.nan)
+    _serve(table, caches, 8, dtype, 14, page)
+
+
+def test_captured_steps_grow():
+    """One captured step, replayed as the requests grow over page borders,
+    with eager work between the replays; each replay against eager calls on
+    a copy."""
+    batch, hq, hkv, d, page = 3, 8, 2, 64, 16
+    both = []
+    for _ in range(2):
+        table = PageTable(batch, 256, num_pages=40, page_size=page)
+        cache = PagedKVCache(table, hkv, d, dtype=F16)
+        cache.k_pages.zero_()
+        cache.v_pages.zero_()
+        g = torch.Generator(device="cuda").manual_seed(3)
+        slots = table.reserve(_counts([14, 0, 31]), width=31)
+        cache.append(*torch.randn(2, batch, hkv, 31, d, device="cuda", generator=g).to(F16), slots)
+        both.append((table, cache))
+    (table, cache), (table2, cache2) = both
+    q = torch.zeros(batch, hq, 1, d, device="cuda", dtype=F16)
+    nk, nv = torch.zeros(2, batch, hkv, 1, d, device="cuda", dtype=F16)
+    counts = _counts([1, 1, 1])
+    keep = table.lengths.clone()
+
+    def step(table, cache):
+        table.trim(keep)
+        slots = table.reserve(counts, width=1)
+        return cache.append_and_attend(q, nk, nv, slots)
+
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        step(table, cache)  # warm-up; the trim in the step takes it back
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(table, cache)
+    torch.cuda.synchronize()
+    for r in range(6):
+        q.copy_(torch.randn(q.shape, device="cuda"))
+        nk.copy_(torch.randn(nk.shape, device="cuda"))
+        nv.copy_(torch.randn(nv.shape, device="cuda"))
+        counts.copy_(_counts([1, r % 2, 1]))
+        torch.cuda.synchronize()
+        graph.replay()
+        expected = step(table2, cache2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, expected), r
+        for name in ("tables", "lengths", "free_pages", "counters"):
+            assert torch.equal(getattr(table, name), getattr(table2, name)), (r, name)
+        assert torch.equal(cache.k_pages, cache2.k_pages) and torch.equal(cache.v_pages, cache2.v_pages)
+        keep.copy_(table.lengths)
+        torch.zeros(1 << 20, device="cuda").sum().item()
+
+
+def test_two_streams_and_a_graph():
+    """Calls on two streams, and a graph replayed beside them, share no
+    scratch memory."""
+    cases = [make_case(4, 16, 4, 1, 128, 16, [3000, 10, 700, 1], dtype=F16, seed=s, device="cuda") for s in (1, 2)]
+    want = [_attend(*c) for c in cases]
+    torch.cuda.synchronize()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(sa):
+        _attend(*cases[0])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=sa):
+            captured = _attend(*cases[0])
+    torch.cuda.synchronize()
+    for r in range(4):
+        with torch.cuda.stream(sb):
+            graph.replay()
+        with torch.cuda.stream(sa):
+            eager = [_attend(*cases[1]) for _ in range(3)]
+        torch.cuda.synchronize()
+        for got, w in [(captured, want[0])] + [(e, want[1]) for e in eager]:
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1]), r
+
+
+# --- the C ABI ---------------------------------------------------------------
+
+def test_library_refuses_a_small_workspace():
+    q, k, v, tables, lengths = make_case(2, 4, 2, 1, 64, 16, [50, 100], dtype=F16, seed=4, device="cuda")
+    need = _hip.paged_decode_workspace_bytes(2, 4, 2, 1, 64)
+    out = torch.full_like(q, 5.0)
+    with pytest.raises(RuntimeError, match="workspace"):
+        _hip.paged_decode(q, k, v, out, None, tables, lengths, scale=0.1, causal=False,
+                          workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+    assert (out == 5).all()
+    _hip.paged_decode(q, k, v, out, None, tables, lengths, scale=0.125, causal=False,
+                      workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
+    assert_attention(out, q, k, v, tables, lengths, scale=0.125)
