@@ -472,7 +472,242 @@ PyObject* py_store_lengths(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// Paged cache. A page table's state: tables int32 [B, columns] with a unit
+// column stride, lengths [B], free_pages [pages] and counters [4], contiguous.
+
+bool int32_on(const Tensor* t, const c10::Device& dev) {
+  return t && t->scalar_type() == at::kInt && t->device() == dev && !t->is_inference();
+}
+
+// Pools [pages, Hkv, page, D] that the kernels read and write in place.
+bool pools_ok(const Tensor& k, const Tensor& v) {
+  if (k.dim() != 4 || k.sizes() != v.sizes() || k.numel() == 0) return false;
+  if (!half_type(k) || v.scalar_type() != k.scalar_type() || v.device() != k.device()) return false;
+  return k.size(2) % 16 == 0 && k.size(3) % 8 == 0 && k.size(3) <= 128 && layout_ok(k) && layout_ok(v) &&
+         is_gfx950(k.device().index());
+}
+
+struct PagedArgs {
+  const Tensor *q, *k, *v, *tables, *lengths;
+  double scale;
+  bool causal;
+  // Arguments from `a`: q, k_pages, v_pages, tables, lengths, causal, scale or None.
+  bool read(PyObject* const* a) {
+    q = plain_tensor(a[0]); k = plain_tensor(a[1]); v = plain_tensor(a[2]);
+    tables = plain_tensor(a[3]); lengths = plain_tensor(a[4]);
+    if (!q || !k || !v || !tables || !lengths || !exact_bool(a[5], causal) || !plain_mode() ||
+        !pools_ok(*k, *v))
+      return false;
+    if (q->dim() != 4 || q->numel() == 0 || q->size(3) != k->size(3) || q->size(1) % k->size(1) ||
+        q->scalar_type() != k->scalar_type() || q->device() != k->device() || wants_grad({q, k, v}))
+      return false;
+    const int64_t b = q->size(0);
+    if (tables->scalar_type() != at::kInt || lengths->scalar_type() != at::kInt ||
+        tables->device() != q->device() || lengths->device() != q->device() || tables->dim() != 2 ||
+        lengths->dim() != 1 || tables->size(0) != b || lengths->size(0) != b || tables->size(1) == 0 ||
+        tables->stride(1) != 1 || tables->stride(0) < 0 || !lengths->is_contiguous())
+      return false;
+    if (a[6] == Py_None) scale = 1.0 / std::sqrt((double)q->size(3));
+    else if (PyFloat_CheckExact(a[6])) scale = PyFloat_AS_DOUBLE(a[6]);
+    else return false;
+    return std::isfinite(scale);
+  }
+};
+
+Tensor launch_paged(const PagedArgs& a, Tensor* lse) {
+  const Tensor q = readable(*a.q);
+  const Tensor &k = *a.k, &v = *a.v;
+  const int64_t b = q.size(0), hq = q.size(1), sq = q.size(2), d = q.size(3), hkv = k.size(1);
+  Tensor out = at::empty({b, hq, sq, d}, q.options());
+  if (lse) *lse = at::empty({b, hq, sq}, q.options().dtype(at::kFloat));
+  Tensor ws = bytes_like(q, kf_paged_decode_workspace_bytes(b, hq, hkv, sq, d));
+  check(kf_paged_decode(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(),
+                        lse ? lse->data_ptr<float>() : nullptr, a.tables->const_data_ptr<int32_t>(),
+                        a.lengths->const_data_ptr<int32_t>(), b, hq, hkv, sq, d, k.size(0), k.size(2),
+                        a.tables->size(1), a.tables->stride(0), q.strides().data(), k.strides().data(),
+                        v.strides().data(), out.strides().data(), (float)a.scale, a.causal, dtype_code(q),
+                        ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
+        "kf_paged_decode");
+  return out;
+}
+
+// paged_attention(q, k_pages, v_pages, tables, lengths, causal, scale or None,
+// return_lse).
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  PagedArgs a;
+  bool with_lse;
+  if (n != 8 || !exact_bool(args[7], with_lse) || !a.read(args)) return not_handled();
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.q->device());
+    out = launch_paged(a, with_lse ? &lse : nullptr);
+  }
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) throw python_error();
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+struct StoreArgs {
+  const Tensor *k, *v, *nk, *nv, *slots;
+  // Arguments from `a`: k_pages, v_pages, new_k, new_v, slots.
+  bool read(PyObject* const* a) {
+    k = plain_tensor(a[0]); v = plain_tensor(a[1]); nk = plain_tensor(a[2]); nv = plain_tensor(a[3]);
+    slots = plain_tensor(a[4]);
+    if (!k || !v || !nk || !nv || !slots || !plain_mode() || !pools_ok(*k, *v)) return false;
+    if (nk->dim() != 4 || nk->sizes() != nv->sizes() || nk->numel() == 0 || nk->size(1) != k->size(1) ||
+        nk->size(3) != k->size(3) || nk->scalar_type() != k->scalar_type() ||
+        nv->scalar_type() != k->scalar_type() || nk->device() != k->device() || nv->device() != k->device())
+      return false;
+    for (const Tensor* t : {k, v})
+      for (int i = 0; i < 4; ++i)
+        if (t->stride(i) == 0 && t->size(i) > 1) return false;
+    return slots->scalar_type() == at::kLong && slots->dim() == 2 && slots->size(0) == nk->size(0) &&
+           slots->size(1) == nk->size(2) && slots->stride(1) == 1 && slots->device() == k->device();
+  }
+};
+
+void launch_store(const StoreArgs& a) {
+  check(kf_paged_append(a.k->data_ptr(), a.v->data_ptr(), a.nk->const_data_ptr(), a.nv->const_data_ptr(),
+                        a.slots->const_data_ptr<int64_t>(), a.nk->size(0), a.nk->size(1), a.nk->size(2),
+                        a.nk->size(3), a.k->size(0), a.k->size(2), a.slots->stride(0),
+                        a.k->strides().data(), a.v->strides().data(), a.nk->strides().data(),
+                        a.nv->strides().data(), dtype_code(*a.k), stream_of(*a.k)),
+        "kf_paged_append");
+}
+
+// paged_append(k_pages, v_pages, new_k, new_v, slots).
+PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  StoreArgs a;
+  if (n != 5 || !a.read(args)) return not_handled();
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.k->device());
+    launch_store(a);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_step(q, k_pages, v_pages, tables, lengths, causal, None, new_k, new_v,
+// slots): the store, then the attention.
+PyObject* py_paged_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  PagedArgs a;
+  StoreArgs st;
+  if (n != 10 || !a.read(args)) return not_handled();
+  PyObject* const store[] = {args[1], args[2], args[7], args[8], args[9]};
+  if (!st.read(store)) return not_handled();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.q->device());
+    launch_store(st);
+    out = launch_paged(a, nullptr);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+struct TableArgs {
+  const Tensor *tables, *lengths, *free_pages, *counters;
+  const int32_t* each;  // per-request values, or null
+  int64_t all;          // the value of every request
+  int64_t page;
+  // Arguments from `a`: tables, lengths, free_pages, counters, an int or a
+  // tensor of one value per request, page_size.
+  bool read(PyObject* const* a) {
+    tables = plain_tensor(a[0]); lengths = plain_tensor(a[1]); free_pages = plain_tensor(a[2]);
+    counters = plain_tensor(a[3]);
+    if (!tables || !plain_mode() || !is_gfx950(tables->device().index())) return false;
+    const auto dev = tables->device();
+    if (!int32_on(tables, dev) || !int32_on(lengths, dev) || !int32_on(free_pages, dev) ||
+        !int32_on(counters, dev))
+      return false;
+    if (tables->dim() != 2 || tables->stride(1) != 1 || lengths->dim() != 1 || free_pages->dim() != 1 ||
+        counters->dim() != 1 || lengths->size(0) != tables->size(0) || counters->size(0) != 4 ||
+        !lengths->is_contiguous() || !free_pages->is_contiguous() || !counters->is_contiguous())
+      return false;
+    each = nullptr;
+    all = 0;
+    if (PyLong_CheckExact(a[4])) {
+      int over = 0;
+      all = PyLong_AsLongLongAndOverflow(a[4], &over);
+      if (over || all < 0 || all >= (1 << 30)) return false;
+    } else {
+      const Tensor* t = plain_tensor(a[4]);
+      if (!t || t->scalar_type() != at::kInt || t->device() != dev || t->dim() != 1 ||
+          t->size(0) != tables->size(0) || !t->is_contiguous())
+        return false;
+      each = t->const_data_ptr<int32_t>();
+    }
+    if (!PyLong_CheckExact(a[5])) return false;
+    page = PyLong_AsLongLong(a[5]);
+    return true;
+  }
+  // The version counters of what a call has written, as an in-place torch
+  // operation moves them.
+  void written() const {
+    for (const Tensor* t : {tables, lengths, free_pages, counters}) t->unsafeGetTensorImpl()->bump_version();
+  }
+};
+
+// page_reserve(tables, lengths, free_pages, counters, counts, page_size,
+// width): the slots.
+PyObject* py_page_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TableArgs t;
+  if (n != 7 || !PyLong_CheckExact(args[6]) || !t.read(args)) return not_handled();
+  const int64_t width = PyLong_AsLongLong(args[6]);
+  if (width <= 0 || width >= (1 << 30) || (!t.each && t.all > width)) return not_handled();
+  Tensor slots;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(t.tables->device());
+    slots = at::empty({t.tables->size(0), width}, t.tables->options().dtype(at::kLong));
+    check(kf_page_reserve(t.tables->data_ptr<int32_t>(), t.lengths->data_ptr<int32_t>(),
+                          t.free_pages->data_ptr<int32_t>(), t.counters->data_ptr<int32_t>(), t.each, t.all,
+                          slots.data_ptr<int64_t>(), width, t.tables->size(0), t.tables->size(1),
+                          t.tables->stride(0), t.page, t.free_pages->size(0), stream_of(*t.tables)),
+          "kf_page_reserve");
+  }
+  t.written();
+  return THPVariable_Wrap(std::move(slots));
+  END_HANDLE_TH_ERRORS
+}
+
+// page_trim(tables, lengths, free_pages, counters, lengths, page_size).
+PyObject* py_page_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TableArgs t;
+  if (n != 6 || !t.read(args)) return not_handled();
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(t.tables->device());
+    check(kf_page_trim(t.tables->data_ptr<int32_t>(), t.lengths->data_ptr<int32_t>(),
+                       t.free_pages->data_ptr<int32_t>(), t.counters->data_ptr<int32_t>(), t.each, t.all,
+                       t.tables->size(0), t.tables->size(1), t.tables->stride(0), t.page,
+                       t.free_pages->size(0), stream_of(*t.tables)),
+          "kf_page_trim");
+  }
+  t.written();
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
+    {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
+    {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},
+    {"paged_step", (PyCFunction)(void (*)(void))py_paged_step, METH_FASTCALL, nullptr},
+    {"page_reserve", (PyCFunction)(void (*)(void))py_page_reserve, METH_FASTCALL, nullptr},
+    {"page_trim", (PyCFunction)(void (*)(void))py_page_trim, METH_FASTCALL, nullptr},
     {"store_lengths", (PyCFunction)(void (*)(void))py_store_lengths, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void (*)(void))py_attention, METH_FASTCALL, nullptr},
     {"append_step", (PyCFunction)(void (*)(void))py_append_step, METH_FASTCALL, nullptr},

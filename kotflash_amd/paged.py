@@ -66,6 +66,11 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots, *, backend: str = "auto"
     at ``slots`` (int64 [B, S]: page * page_size + row): K and V bit-exact, in
     one launch. Slots outside the pool (-1 in the padding of ``reserve``) are
     skipped; two tokens of a call must not share a slot."""
+    # The ordinary GPU call is checked and launched natively; anything else (and
+    # every error) takes the checks below. So do the calls further down.
+    if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling() \
+            and _hip.native().paged_append(k_pages, v_pages, new_k, new_v, slots) is None:
+        return
     hip_paged.check_append(k_pages, v_pages, new_k, new_v, slots)
     if _store_on_hip(backend, k_pages, half=True):
         hip_paged.append_paged(k_pages, v_pages, new_k, new_v, slots)
@@ -96,6 +101,11 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
     these hold and ``sdpa`` (one call per request, lengths on the host)
     elsewhere. With ``return_lse``, returns (O, LSE), LSE in fp32 [B, Hq, Sq].
     """
+    if backend in ("auto", "hip", "triton") and not torch.compiler.is_compiling():
+        out = _hip.native().paged_attention(q, k_pages, v_pages, tables, lengths, causal, scale,
+                                            return_lse)
+        if out is not NotImplemented:
+            return out
     scale, on_hip = _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backend)
     if on_hip:
         return hip_paged.attention_paged(q, k_pages, v_pages, tables, lengths, causal=causal,
@@ -230,6 +240,12 @@ class PageTable:
         pages asked for by the requests up to it are more than the free ones:
         its slots are all -1 and ``refused`` counts it.
         """
+        if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling():
+            slots = _hip.native().page_reserve(
+                self.tables, self.lengths, self.free_pages, self.counters, counts, self.page_size,
+                max(counts, 1) if width is None and type(counts) is int else width)
+            if slots is not NotImplemented:
+                return slots
         counts = self._per_request("counts", counts)
         if width is None:
             if isinstance(counts, torch.Tensor):
@@ -248,6 +264,10 @@ class PageTable:
         [batch] on the device; longer than it is: all of them). The pages
         behind go back to the stack, so that the ``reserve`` that took them
         would take the same again."""
+        if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling() \
+                and _hip.native().page_trim(self.tables, self.lengths, self.free_pages, self.counters,
+                                            lengths, self.page_size) is None:
+            return
         lengths = self._per_request("lengths", lengths)
         state = (self.tables, self.lengths, self.free_pages, self.counters)
         if _store_on_hip(backend, self.tables, half=False):
@@ -330,6 +350,12 @@ class PagedKVCache:
                           append_backend: str = "auto", attention_backend: str = "auto"):
         """``append``, then ``attend``: a decoding step of this layer, after
         the table's ``reserve`` of the step."""
+        if append_backend in ("auto", "hip", "cuda") and attention_backend in ("auto", "hip", "triton") \
+                and not torch.compiler.is_compiling():
+            out = _hip.native().paged_step(q, self.k_pages, self.v_pages, self.table.tables,
+                                           self.table.lengths, causal, None, new_k, new_v, slots)
+            if out is not NotImplemented:
+                return out
         # Every check of the attention comes before the store writes anything.
         _attention_route(q, self.k_pages, self.v_pages, self.table.tables, self.table.lengths, causal,
                          None, attention_backend)
