@@ -15,39 +15,46 @@ namespace kf {
 // a column then combine with lane swaps (v_permlane16/32_swap).
 constexpr int kMergeU = 16;
 
-// One output row: orr / lrr address split s's O row at s * ostride floats
-// and its LSE at s * lstride floats; every offset must fit 32 bits (checked
-// by the callers' hosts).
-template <typename T, int QL>
-__device__ inline void merge_row(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsrc_t lrr,
-                                 uint32_t ostride, uint32_t lstride, int nsplit, int D,
-                                 uint16_t* out_row, float* lse_out) {
+// A lane's part of a merge: 4 columns and the denominator, in units of
+// 2^M, M the largest LSE (log2) it has seen.
+struct MergeState {
+  f32x4 acc;
+  float den, M;
+};
+
+// Splits [first, last) of one output row: orr / lrr address split s's O row at
+// s * ostride floats and its LSE at s * lstride floats; every offset must fit
+// 32 bits (checked by the callers' hosts). All SW lanes of a column end with
+// the same state.
+template <int QL>
+__device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsrc_t lrr,
+                                          uint32_t ostride, uint32_t lstride, int first, int last, int D) {
   constexpr int SW = 64 / QL;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   const int q = lane % QL, sl = lane / QL;
   const bool col = 4 * q < D;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f, mrun = kNegInf;  // running reference max of this lane's chunks (log2 units)
-  for (int c0 = 0; c0 < nsplit; c0 += kMergeU * SW) {
+  for (int c0 = first; c0 < last; c0 += kMergeU * SW) {
     u32x4 v[kMergeU];
     float w[kMergeU];
     uint32_t lw[kMergeU];
 #pragma unroll
     for (int u = 0; u < kMergeU; ++u) {
       const int s2 = c0 + sl + SW * u;
-      lw[u] = __builtin_amdgcn_raw_buffer_load_b32(lrr, s2 < nsplit ? (uint32_t)s2 * lstride * 4u : kOOB, 0, 0);
+      lw[u] = __builtin_amdgcn_raw_buffer_load_b32(lrr, s2 < last ? (uint32_t)s2 * lstride * 4u : kOOB, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < kMergeU; ++u) {
       const int s2 = c0 + sl + SW * u;
-      v[u] = buf_load16(orr, s2 < nsplit && col ? ((uint32_t)s2 * ostride + 4u * q) * 4u : kOOB);
+      v[u] = buf_load16(orr, s2 < last && col ? ((uint32_t)s2 * ostride + 4u * q) * 4u : kOOB);
     }
     // Keep every load of the chunk ahead of the first use: left alone, the
     // scheduler recycles early result registers and waits for them mid-batch.
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < kMergeU; ++u)
-      w[u] = c0 + sl + SW * u < nsplit ? __uint_as_float(lw[u]) * kLog2e : kNegInf;
+      w[u] = c0 + sl + SW * u < last ? __uint_as_float(lw[u]) * kLog2e : kNegInf;
     float mx = kNegInf;
 #pragma unroll
     for (int u = 0; u < kMergeU; ++u) mx = fmaxf(mx, w[u]);
@@ -77,14 +84,29 @@ __device__ inline void merge_row(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsr
     const float x = acc[e] * sc;
     acc[e] = QL == 16 ? wave_group16_sum(x) : wave_xor32_sum(x);
   }
-  if (sl == 0 && col) {
-    const float inv = dtot > 0.f ? 1.f / dtot : 0.f;
+  return {acc, dtot, M};
+}
+
+// O and LSE of the row, from the lanes of the first SW.
+template <typename T, int QL>
+__device__ inline void merge_store(const MergeState& m, int D, uint16_t* out_row, float* lse_out) {
+  const int lane = threadIdx.x & 63;
+  const int q = lane % QL;
+  if (lane < QL && 4 * q < D) {
+    const float inv = m.den > 0.f ? 1.f / m.den : 0.f;
     u32x2 wv;
-    wv[0] = pack2<T>(acc[0] * inv, acc[1] * inv);
-    wv[1] = pack2<T>(acc[2] * inv, acc[3] * inv);
+    wv[0] = pack2<T>(m.acc[0] * inv, m.acc[1] * inv);
+    wv[1] = pack2<T>(m.acc[2] * inv, m.acc[3] * inv);
     *reinterpret_cast<u32x2*>(out_row + 4 * q) = wv;
-    if (q == 0 && lse_out) *lse_out = dtot > 0.f ? (M + fast_log2(dtot)) * kLn2 : kNegInf;
+    if (q == 0 && lse_out) *lse_out = m.den > 0.f ? (m.M + fast_log2(m.den)) * kLn2 : kNegInf;
   }
+}
+
+template <typename T, int QL>
+__device__ inline void merge_row(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsrc_t lrr,
+                                 uint32_t ostride, uint32_t lstride, int nsplit, int D,
+                                 uint16_t* out_row, float* lse_out) {
+  merge_store<T, QL>(merge_splits<QL>(orr, lrr, ostride, lstride, 0, nsplit, D), D, out_row, lse_out);
 }
 
 }  // namespace kf

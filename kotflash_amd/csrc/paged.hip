@@ -55,6 +55,7 @@ struct PagedParams {
   float* lse;
   float* part_o;    // [slots][rows][D]
   float* part_lse;  // [slots][rows]
+  int32_t* parts;   // [B * heads][2]: first worker of a row group, its number of partials
   const int32_t* tables;
   const int32_t* lengths;
   int64_t t_sb;
@@ -64,6 +65,7 @@ struct PagedParams {
   int64_t o_sb, o_sh, o_ss;
   int B, Hq, Hkv, Sq, D, G;
   int pages, gpp;  // pages of the pool; 16-row groups per page
+  uint32_t gpp_inv;  // floor(2^32 / gpp)
   int cap;         // tokens that a table has columns for
   int rows, nrb;   // packed rows per row group, row groups per KV head
   int heads;       // Hkv * nrb
@@ -75,18 +77,38 @@ struct PagedParams {
 // Direct-to-LDS load (kf_common.hpp) whose resource may have been written by
 // the vector unit just before (a spilled scalar comes back by v_readlane): a
 // vector-memory instruction may read such a register five wait states later.
+// STREAM: marked as read once (nt).
+template <bool STREAM>
 __device__ inline void dma16_r(__amdgpu_buffer_rsrc_t r, uint32_t lds_m0, uint32_t voff) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 4\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      :
-      : "s"(__builtin_amdgcn_readfirstlane(lds_m0)), "v"(voff), "s"(r)
-      : "memory", "m0");
+  if constexpr (STREAM) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_m0)), "v"(voff), "s"(r)
+        : "memory", "m0");
+  } else {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(__builtin_amdgcn_readfirstlane(lds_m0)), "v"(voff), "s"(r)
+        : "memory", "m0");
+  }
 }
 
 constexpr int kStep = 32;     // keys per unit
 constexpr int kPagedRing = 2; // steps of a worker in flight
+
+// K/V bytes of a call from which its loads are marked as read once. Such loads
+// do not go through the 256 MB memory-side cache, which costs the others a
+// tenth of their rate (measured, three sets of inputs in turn: 1158 MB 209 us
+// plain and 188 marked, 537 MB 103 and 93, 300 MB 64 and 57, 294 MB 62 and
+// 54); but a call of which the cache still holds a part from the last time is
+// faster plain (59 MB 21 and 23).
+constexpr int64_t kStreamBytes = 128 << 20;
 
 __device__ inline int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
@@ -95,10 +117,10 @@ __device__ inline int steps_of(const PagedParams& p, int len) { return (visible(
 __device__ inline int lane_steps(const PagedParams& p, int b) {
   return b < p.B ? steps_of(p, p.lengths[b]) : 0;
 }
-// Steps of the whole batch (one head).
-__device__ inline int total_steps(const PagedParams& p, int lane) {
+// Steps (of one head) of the requests from b0 on.
+__device__ inline int steps_from(const PagedParams& p, int b0, int lane) {
   int n = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) n += lane_steps(p, b0 + lane);
+  for (; b0 < p.B; b0 += 64) n += lane_steps(p, b0 + lane);
   return wave_sum(n);
 }
 // Units per worker.
@@ -125,28 +147,40 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
   const int l16 = lane & 15, g16 = lane >> 4;
   const const_i32 lengths = (const_i32)(uintptr_t)p.lengths;
 
-  // This worker's run of units, and where it begins.
+  // This worker's run of units, and where it begins: request b, whose first
+  // unit is `start`. The first 64 requests' lengths are read once.
   const int worker = blockIdx.x;
-  const int run = run_length(p, total_steps(p, lane));
-  int u = worker * run;
-  int b = 0, start = 0;  // request of unit u, its first unit
-  bool found = false;
-  for (int b0 = 0; b0 < p.B && !found; b0 += 64) {
-    const int mine = lane_steps(p, b0 + lane) * p.heads;
-    const int sum = wave_scan(mine);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(start + sum > u);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      start += __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(mine, at);
-      b = b0 + at;
-      found = true;
-    } else {
+  const int len0 = lane < p.B ? visible(p, p.lengths[lane]) : 0;
+  const int mine0 = (len0 + kStep - 1) / kStep;
+  const int sum0 = wave_scan(mine0);
+  int total = __builtin_amdgcn_readlane(sum0, 63);
+  if (p.B > 64) total += steps_from(p, 64, lane);
+  const int run = run_length(p, total);
+  const int u = worker * run;
+  if (u >= total * p.heads) return;  // more workers than runs
+  int b, start, len;
+  uint64_t past = __builtin_amdgcn_ballot_w64(sum0 * p.heads > u);
+  if (past) {
+    b = __builtin_ctzll(past);
+    len = __builtin_amdgcn_readlane(len0, b);
+    start = (__builtin_amdgcn_readlane(sum0, b) - __builtin_amdgcn_readlane(mine0, b)) * p.heads;
+  } else {
+    start = __builtin_amdgcn_readlane(sum0, 63) * p.heads;
+    for (b = 64;; b += 64) {
+      const int mine = lane_steps(p, b + lane) * p.heads;
+      const int sum = wave_scan(mine);
+      past = __builtin_amdgcn_ballot_w64(start + sum > u);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        start += __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(mine, at);
+        b += at;
+        break;
+      }
       start += __builtin_amdgcn_readlane(sum, 63);
     }
+    len = visible(p, lengths[b]);
   }
-  if (!found) return;  // more workers than runs
-  int len = visible(p, lengths[b]);
-  int n = steps_of(p, len);
+  int n = (len + kStep - 1) / kStep;
   int hh = (u - start) / n;
   int s0 = (u - start) - hh * n;
   int left = run;
@@ -165,6 +199,7 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     voff[k] = ok ? (uint32_t)(r * p.v_ss + c * 8) * 2u : kOOB;
   }
   const uint32_t ring0 = lds_addr(ring);
+  const bool stream = (int64_t)total * p.heads * (kStep * 4 * p.D) > kStreamBytes;
 
   for (;;) {
     // One segment: steps [s0, s1) of row group hh of request b.
@@ -191,33 +226,62 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       }
     }
 
-    // Visible rows of 16-row group gi, 0 where its page is not in the pool,
-    // and its loads.
-    auto issue_group = [&](int gi, uint32_t m0) -> int {
-      int vis = min(max(len - 16 * gi, 0), 16);
-      const int column = gi / p.gpp;
-      const int page = vis > 0 ? __builtin_amdgcn_readfirstlane(table[column]) : 0;
-      if (page < 0 || page >= p.pages) vis = 0;
-      const int row0 = (gi - column * p.gpp) * 16;
-      const int64_t at = vis > 0 ? page : 0;
-      const auto kr = make_rsrc(kh + at * p.k_sp + row0 * p.k_ss, rows_extent(vis, p.k_ss, p.D));
-      const auto vr = make_rsrc(vh + at * p.v_sp + row0 * p.v_ss, rows_extent(vis, p.v_ss, p.D));
+    // The pages of a step's two 16-row groups (column and first row of each,
+    // the last visible group's where the second lies behind it). Read one
+    // step before they are needed, all of a ring's at the segment's start.
+    struct StepPages {
+      int page[2], row0[2];
+    };
+    auto look_up = [&](int s) {
+      StepPages sp;
 #pragma unroll
-      for (int k = 0; k < NGI; ++k) {
-        dma16_r(kr, m0 + k * 1024u, koff[k]);
-        dma16_r(vr, m0 + VT * 2 + k * 1024u, voff[k]);
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t gi = min(2 * s + g, (len - 1) >> 4);
+        uint32_t column = __umulhi(gi, p.gpp_inv);
+        uint32_t rest = gi - column * p.gpp;
+        const bool up = rest >= (uint32_t)p.gpp;  // the quotient may be one short
+        column += up;
+        rest -= up ? p.gpp : 0;
+        sp.page[g] = table[column];
+        sp.row0[g] = (int)rest * 16;
       }
-      return vis;
+      return sp;
     };
+    // Loads of step s into its slot; visible rows per group, 0 where the page
+    // is not in the pool.
     int vis[kPagedRing][2];
-    auto issue = [&](int s, auto slot_c) {
+    auto issue = [&](int s, const StepPages& sp, auto slot_c) {
       constexpr int slot = decltype(slot_c)::value;
-      const uint32_t m0 = ring0 + slot * 2 * VT * 2;
-      vis[slot][0] = issue_group(2 * s, m0);
-      vis[slot][1] = issue_group(2 * s + 1, m0 + 16 * DT * 2);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t m0 = ring0 + slot * 2 * VT * 2 + g * 16 * DT * 2;
+        const int page = __builtin_amdgcn_readfirstlane(sp.page[g]);
+        int seen = min(max(len - 32 * s - 16 * g, 0), 16);
+        if (page < 0 || page >= p.pages) seen = 0;
+        const int64_t at = seen > 0 ? page : 0;
+        const auto kr = make_rsrc(kh + at * p.k_sp + sp.row0[g] * p.k_ss, rows_extent(seen, p.k_ss, p.D));
+        const auto vr = make_rsrc(vh + at * p.v_sp + sp.row0[g] * p.v_ss, rows_extent(seen, p.v_ss, p.D));
+        if (stream) {
+#pragma unroll
+          for (int k = 0; k < NGI; ++k) {
+            dma16_r<true>(kr, m0 + k * 1024u, koff[k]);
+            dma16_r<true>(vr, m0 + VT * 2 + k * 1024u, voff[k]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < NGI; ++k) {
+            dma16_r<false>(kr, m0 + k * 1024u, koff[k]);
+            dma16_r<false>(vr, m0 + VT * 2 + k * 1024u, voff[k]);
+          }
+        }
+        vis[slot][g] = seen;
+      }
     };
+    StepPages first[kPagedRing];
+    static_for<0, kPagedRing>([&](auto sc) { first[decltype(sc)::value] = look_up(s0 + decltype(sc)::value); });
+    StepPages next = look_up(s0 + kPagedRing);
     static_for<0, kPagedRing>([&](auto sc) {
-      if (s0 + decltype(sc)::value < s1) issue(s0 + decltype(sc)::value, sc);
+      if (s0 + decltype(sc)::value < s1) issue(s0 + decltype(sc)::value, first[decltype(sc)::value], sc);
     });
 
     f32x4 oacc[QB][NDB];  // O^T: lane l, register r = head dim 16 db + 4 (l / 16) + r of row l % 16
@@ -321,17 +385,21 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       static_for<0, kPagedRing>([&](auto sc) {
         const int s = j0 + decltype(sc)::value;
         if (s < s1) {
-          if (s + 1 < s1) KF_WAIT_VMCNT(NL);
-          else KF_WAIT_VMCNT(0);
+          // This step's loads are done once only those of later ones are left.
+          const int later = min(kPagedRing - 1, s1 - 1 - s);
+          static_for<0, kPagedRing>([&](auto lc) {
+            if (later == decltype(lc)::value) KF_WAIT_VMCNT(decltype(lc)::value * NL);
+          });
           step(s, sc);
           if (s + kPagedRing < s1) {
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read
-            issue(s + kPagedRing, sc);
+            issue(s + kPagedRing, next, sc);
+            next = look_up(s + kPagedRing + 1);
           }
         }
       });
     }
-    static_assert(kPagedRing == 2, "the waits above assume at most one later step in flight");
+    static_assert((kPagedRing - 1) * NL < 64, "the counter of outstanding loads has six bits");
 
     // O and LSE, or the partial of this worker.
     const bool whole = s0 == 0 && s1 == n;
@@ -365,6 +433,13 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       }
     }
 
+    // The row group's first worker says how many there are: the steps behind
+    // its own fill whole runs.
+    if (s0 == 0 && lane == 0) {
+      p.parts[2 * (b * p.heads + hh)] = worker;
+      p.parts[2 * (b * p.heads + hh) + 1] = 1 + (n - s1 + run - 1) / run;
+    }
+
     left -= s1 - s0;
     if (left <= 0) break;
     // The next segment: next row group, or the next request that holds keys.
@@ -380,40 +455,64 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
   }
 }
 
-// One wave per output row: merges the row's partials, writes zeros where the
-// request holds nothing, and leaves rows that one worker wrote whole.
-template <typename T, int QL>
-__global__ __launch_bounds__(64) void paged_merge_kernel(const PagedParams p) {
-  const int lane = threadIdx.x;
+// One workgroup of W waves per output row: merges the row's partials, writes
+// zeros where the request holds nothing, and leaves rows that one worker wrote
+// whole. Bound by its chain of loads: which partials, then all of them. The
+// first wave alone takes what one round trip brings; more partials the waves
+// share, and combine through LDS in their order.
+template <typename T, int QL, int W>
+__global__ __launch_bounds__(64 * W) void paged_merge_kernel(const PagedParams p) {
+  const int lane = threadIdx.x & 63, wave = wave_index();
   const int r = blockIdx.x % p.rows;
   const int bh = blockIdx.x / p.rows;
   const int hh = bh % p.heads, b = bh / p.heads;
   const int kvh = hh / p.nrb, rho = (hh % p.nrb) * p.rows + r;
+  // What the workers wrote is not there for a request without keys.
+  const int len = ((const_i32)(uintptr_t)p.lengths)[b];
+  const int w0 = ((const_i32)(uintptr_t)p.parts)[2 * bh], parts = ((const_i32)(uintptr_t)p.parts)[2 * bh + 1];
   if (rho >= p.G * p.Sq) return;
-  int all = 0, before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int s = lane_steps(p, b0 + lane);
-    all += s;
-    before += b0 + lane < b ? s : 0;
-  }
-  const int run = run_length(p, wave_sum(all));
-  const int n = steps_of(p, ((const_i32)(uintptr_t)p.lengths)[b]);
-  const int u0 = wave_sum(before) * p.heads + hh * n;
-  const int w0 = u0 / run, w1 = (u0 + n - 1) / run;
+  const bool alone = W == 1 || len <= 0 || parts <= kMergeU * (64 / QL);
+  if (alone && wave > 0) return;
   const int h = kvh * p.G + rho / p.Sq, i = rho % p.Sq;
   uint16_t* out = p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss;
   float* lse = p.lse ? p.lse + ((int64_t)b * p.Hq + h) * p.Sq + i : nullptr;
-  if (n == 0) {
+  if (len <= 0) {
     if (4 * lane < p.D) *reinterpret_cast<u32x2*>(out + 4 * lane) = u32x2{0u, 0u};
     if (lane == 0 && lse) *lse = kNegInf;
     return;
   }
-  if (w0 == w1) return;
+  if (parts == 1) return;
   const int64_t slot = (int64_t)(w0 + bh) * p.rows + r;
-  const int parts = w1 - w0 + 1;
   const auto orr = make_rsrc(p.part_o + slot * p.D, (uint32_t)(((int64_t)(parts - 1) * p.rows * p.D + p.D) * 4));
   const auto lrr = make_rsrc(p.part_lse + slot, (uint32_t)(((int64_t)(parts - 1) * p.rows + 1) * 4));
-  merge_row<T, QL>(orr, lrr, (uint32_t)(p.rows * p.D), (uint32_t)p.rows, parts, p.D, out, lse);
+  const uint32_t ostride = (uint32_t)(p.rows * p.D), lstride = (uint32_t)p.rows;
+  if (alone) {
+    merge_row<T, QL>(orr, lrr, ostride, lstride, parts, p.D, out, lse);
+    return;
+  }
+  if constexpr (W > 1) {
+    __shared__ float sums[W][QL][6];
+    const int share = (parts + W - 1) / W;
+    const MergeState mine = merge_splits<QL>(orr, lrr, ostride, lstride, min(wave * share, parts),
+                                             min((wave + 1) * share, parts), p.D);
+    if (lane < QL) {
+      float* to = sums[wave][lane];
+      to[0] = mine.M; to[1] = mine.den;
+      for (int e = 0; e < 4; ++e) to[2 + e] = mine.acc[e];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    MergeState all = {{0.f, 0.f, 0.f, 0.f}, 0.f, kNegInf};
+    for (int w = 0; w < W; ++w) all.M = fmaxf(all.M, sums[w][lane % QL][0]);
+    const float Ms = all.M == kNegInf ? 0.f : all.M;
+    for (int w = 0; w < W; ++w) {
+      const float* from = sums[w][lane % QL];
+      const float sc = fast_exp2(from[0] - Ms);
+      all.den += sc * from[1];
+      for (int e = 0; e < 4; ++e) all.acc[e] += sc * from[2 + e];
+    }
+    merge_store<T, QL>(all, p.D, out, lse);
+  }
 }
 
 // Packed rows per worker: 16-row MFMA blocks, up to four of them.
@@ -432,6 +531,27 @@ static int64_t paged_slots(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64
   return paged_workers(D) + B * Hkv * ((R + paged_rows(R) - 1) / paged_rows(R));
 }
 
+// Waves per row of the merge, from the most partials a row group can have: a
+// head's share of the workers (all of them on one request), cut at both ends.
+// More waves cost launch time, a few tenths of a us where they are not needed
+// (1158 MB over 64 requests: 4.6 us with one wave, 5.0 with four, 7.2 with
+// eight), and save round trips where one row has many partials (131072 keys of
+// one request, 128 partials: 5.9 us with one wave, 4.6 with four).
+template <typename T, int QL>
+static void launch_merge(const PagedParams& p, hipStream_t stream) {
+  constexpr int kTrip = kMergeU * (64 / QL);  // partials that a wave takes at once
+  const int64_t rows = (int64_t)p.B * p.heads * p.rows;
+  const int share = p.workers / p.heads + 2, steps = p.cap / kStep + 1;
+  const int most = share < steps ? share : steps;
+  const dim3 grid((unsigned)rows);
+  if (most > 16 * kTrip && rows <= 256)
+    hipLaunchKernelGGL((paged_merge_kernel<T, QL, 16>), grid, dim3(1024), 0, stream, p);
+  else if (most > kTrip && (rows <= 256 || most > 8 * kTrip))
+    hipLaunchKernelGGL((paged_merge_kernel<T, QL, 4>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), grid, dim3(64), 0, stream, p);
+}
+
 template <typename T, int DT>
 static int launch_paged(const PagedParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.workers);
@@ -442,9 +562,8 @@ static int launch_paged(const PagedParams& p, hipStream_t stream) {
   }
   const int rc = check_launch("kf_paged_decode(workers)");
   if (rc) return rc;
-  const dim3 rows((unsigned)((int64_t)p.B * p.heads * p.rows));
-  if (p.D <= 64) hipLaunchKernelGGL((paged_merge_kernel<T, 16>), rows, dim3(64), 0, stream, p);
-  else hipLaunchKernelGGL((paged_merge_kernel<T, 32>), rows, dim3(64), 0, stream, p);
+  if (p.D <= 64) launch_merge<T, 16>(p, stream);
+  else launch_merge<T, 32>(p, stream);
   return check_launch("kf_paged_decode(merge)");
 }
 
@@ -464,8 +583,11 @@ using namespace kf;
 
 extern "C" size_t kf_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || D <= 0 || D > 128 || Hq % Hkv) return 0;
-  const size_t rows = (size_t)paged_slots(B, Hq, Hkv, Sq, D) * paged_rows(Hq / Hkv * Sq);
-  return (rows * (size_t)D * sizeof(float) + 255) / 256 * 256 + (rows * sizeof(float) + 255) / 256 * 256;
+  const int64_t R = Hq / Hkv * Sq;
+  const size_t rows = (size_t)paged_slots(B, Hq, Hkv, Sq, D) * paged_rows(R);
+  const size_t groups = (size_t)(B * Hkv * ((R + paged_rows(R) - 1) / paged_rows(R)));
+  return (rows * (size_t)D * sizeof(float) + 255) / 256 * 256 + (rows * sizeof(float) + 255) / 256 * 256 +
+         groups * 2 * sizeof(int32_t);
 }
 
 extern "C" int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
@@ -513,13 +635,16 @@ extern "C" int kf_paged_decode(const void* q, const void* k_pages, const void* v
   const size_t slot_rows = (size_t)paged_slots(B, Hq, Hkv, Sq, D) * rows;
   p.part_o = (float*)workspace;
   p.part_lse = (float*)((char*)workspace + (slot_rows * (size_t)D * sizeof(float) + 255) / 256 * 256);
+  p.parts = (int32_t*)((char*)p.part_lse + (slot_rows * sizeof(float) + 255) / 256 * 256);
   p.t_sb = table_stride;
   p.q_sb = q_strides[0]; p.q_sh = q_strides[1]; p.q_ss = q_strides[2];
   p.k_sp = k_strides[0]; p.k_sh = k_strides[1]; p.k_ss = k_strides[2];
   p.v_sp = v_strides[0]; p.v_sh = v_strides[1]; p.v_ss = v_strides[2];
   p.o_sb = o_strides[0]; p.o_sh = o_strides[1]; p.o_ss = o_strides[2];
   p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.Sq = (int)Sq; p.D = (int)D; p.G = (int)(Hq / Hkv);
-  p.pages = (int)num_pages; p.gpp = (int)(page_size / 16); p.cap = (int)cap;
+  p.pages = (int)num_pages; p.gpp = (int)(page_size / 16);
+  p.gpp_inv = (uint32_t)((1ull << 32) / p.gpp > 0xffffffffull ? 0xffffffffull : (1ull << 32) / p.gpp);
+  p.cap = (int)cap;
   p.rows = rows; p.nrb = (int)nrb; p.heads = (int)heads;
   p.workers = paged_workers(D); p.least = 1;
   p.causal = causal != 0;
