@@ -25,8 +25,8 @@ struct MergeState {
 // Splits [first, last) of one output row: orr / lrr address split s's O row at
 // s * ostride floats and its LSE at s * lstride floats; every offset must fit
 // 32 bits (checked by the callers' hosts). All SW lanes of a column end with
-// the same state.
-template <int QL>
+// the same state; U of a lane's splits are in flight at once.
+template <int QL, int U = kMergeU>
 __device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsrc_t lrr,
                                           uint32_t ostride, uint32_t lstride, int first, int last, int D) {
   constexpr int SW = 64 / QL;
@@ -35,17 +35,17 @@ __device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_b
   const bool col = 4 * q < D;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   float den = 0.f, mrun = kNegInf;  // running reference max of this lane's chunks (log2 units)
-  for (int c0 = first; c0 < last; c0 += kMergeU * SW) {
-    u32x4 v[kMergeU];
-    float w[kMergeU];
-    uint32_t lw[kMergeU];
+  for (int c0 = first; c0 < last; c0 += U * SW) {
+    u32x4 v[U];
+    float w[U];
+    uint32_t lw[U];
 #pragma unroll
-    for (int u = 0; u < kMergeU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int s2 = c0 + sl + SW * u;
       lw[u] = __builtin_amdgcn_raw_buffer_load_b32(lrr, s2 < last ? (uint32_t)s2 * lstride * 4u : kOOB, 0, 0);
     }
 #pragma unroll
-    for (int u = 0; u < kMergeU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int s2 = c0 + sl + SW * u;
       v[u] = buf_load16(orr, s2 < last && col ? ((uint32_t)s2 * ostride + 4u * q) * 4u : kOOB);
     }
@@ -53,11 +53,11 @@ __device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_b
     // scheduler recycles early result registers and waits for them mid-batch.
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < kMergeU; ++u)
+    for (int u = 0; u < U; ++u)
       w[u] = c0 + sl + SW * u < last ? __uint_as_float(lw[u]) * kLog2e : kNegInf;
     float mx = kNegInf;
 #pragma unroll
-    for (int u = 0; u < kMergeU; ++u) mx = fmaxf(mx, w[u]);
+    for (int u = 0; u < U; ++u) mx = fmaxf(mx, w[u]);
     // Lane-local online rescale across chunks (one chunk in the common case).
     const float mnew = fmaxf(mrun, mx);
     const float ms = mnew == kNegInf ? 0.f : mnew;
@@ -65,7 +65,7 @@ __device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_b
     acc *= alpha;
     den *= alpha;
 #pragma unroll
-    for (int u = 0; u < kMergeU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const float wt = fast_exp2(w[u] - ms);
       den += wt;
       acc[0] += wt * __uint_as_float(v[u][0]); acc[1] += wt * __uint_as_float(v[u][1]);
@@ -102,11 +102,11 @@ __device__ inline void merge_store(const MergeState& m, int D, uint16_t* out_row
   }
 }
 
-template <typename T, int QL>
+template <typename T, int QL, int U = kMergeU>
 __device__ inline void merge_row(__amdgpu_buffer_rsrc_t orr, __amdgpu_buffer_rsrc_t lrr,
                                  uint32_t ostride, uint32_t lstride, int nsplit, int D,
                                  uint16_t* out_row, float* lse_out) {
-  merge_store<T, QL>(merge_splits<QL>(orr, lrr, ostride, lstride, 0, nsplit, D), D, out_row, lse_out);
+  merge_store<T, QL>(merge_splits<QL, U>(orr, lrr, ostride, lstride, 0, nsplit, D), D, out_row, lse_out);
 }
 
 }  // namespace kf

@@ -17,9 +17,10 @@
 //  * A worker finds its run from the lengths: a sum over the batch, and the
 //    request in which the run begins.
 //  * Within a run the part in one (request, head) is a segment: the packed
-//    query rows of the group against its steps, with a wave-private LDS ring
-//    that direct-to-LDS loads fill two steps ahead (S^T = K Q^T, online
-//    softmax, O^T += V^T P^T on 16x16x32 MFMAs, as in the contiguous decode).
+//    query rows of the group against its steps (S^T = K Q^T, online softmax,
+//    O^T += V^T P^T on 16x16x32 MFMAs, as in the contiguous decode). Two units
+//    are in flight in a wave-private LDS ring that direct-to-LDS loads fill,
+//    across the ends of segments: short requests stream like long ones.
 //  * A segment that is a whole request writes O; others write an fp32 partial
 //    (O, LSE) to slot worker + row group. Both numbers grow along the units
 //    and one of them at every segment, so the slots are distinct, and those of
@@ -60,47 +61,55 @@ struct PagedParams {
   const int32_t* lengths;
   int64_t t_sb;
   int64_t q_sb, q_sh, q_ss;
-  int64_t k_sp, k_sh, k_ss;  // page, head, row
-  int64_t v_sp, v_sh, v_ss;
+  int64_t k_sh, v_sh;            // per KV head
+  uint32_t k_page, v_page;       // bytes of a page
+  uint32_t k_row, v_row;         // bytes of a row
   int64_t o_sb, o_sh, o_ss;
   int B, Hq, Hkv, Sq, D, G;
   int pages, gpp;  // pages of the pool; 16-row groups per page
-  uint32_t gpp_inv;  // floor(2^32 / gpp)
   int cap;         // tokens that a table has columns for
   int rows, nrb;   // packed rows per row group, row groups per KV head
   int heads;       // Hkv * nrb
   int workers, least;
+  uint32_t q_bytes, o_bytes;  // extents of a KV head's queries and outputs
   int causal;
   float scale_log2;
 };
 
-// Direct-to-LDS load (kf_common.hpp) whose resource may have been written by
-// the vector unit just before (a spilled scalar comes back by v_readlane): a
-// vector-memory instruction may read such a register five wait states later.
+// Direct-to-LDS loads (kf_common.hpp) of whole tiles: N loads of 1 KB, one
+// per lane offset, to consecutive places from LDS address `to` on. A resource
+// may have been written by the vector unit just before (a spilled scalar comes
+// back by v_readlane), and a vector-memory instruction may read such a register
+// five wait states later: hence the first, longer s_nop. The others separate
+// the write of M0 from its use.
 // STREAM: marked as read once (nt).
-template <bool STREAM>
-__device__ inline void dma16_r(__amdgpu_buffer_rsrc_t r, uint32_t lds_m0, uint32_t voff) {
-  if constexpr (STREAM) {
-    asm volatile(
-        "s_mov_b32 m0, %0\n\t"
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
-        :
-        : "s"(__builtin_amdgcn_readfirstlane(lds_m0)), "v"(voff), "s"(r)
-        : "memory", "m0");
-  } else {
-    asm volatile(
-        "s_mov_b32 m0, %0\n\t"
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %2, 0 offen lds"
-        :
-        : "s"(__builtin_amdgcn_readfirstlane(lds_m0)), "v"(voff), "s"(r)
-        : "memory", "m0");
+#define KF_FIRST(off, rsrc, nt) "s_nop 4\n\tbuffer_load_dwordx4 " off ", " rsrc ", 0 offen" nt " lds\n\t"
+#define KF_NEXT(off, rsrc, nt) \
+  "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 " off ", " rsrc ", 0 offen" nt " lds\n\t"
+#define KF_TILE1(nt) "s_mov_b32 m0, %0\n\t" KF_FIRST("%2", "%1", nt)
+#define KF_TILE2(nt) KF_TILE1(nt) KF_NEXT("%3", "%1", nt)
+#define KF_TILE3(nt) KF_TILE2(nt) KF_NEXT("%4", "%1", nt)
+#define KF_TILE4(nt) KF_TILE3(nt) KF_NEXT("%5", "%1", nt)
+template <int N, bool STREAM>
+__device__ inline void dma_tile(__amdgpu_buffer_rsrc_t r, uint32_t to, const uint32_t* off) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(to);
+#define KF_EMIT(text, ...)                                                                        \
+  do {                                                                                            \
+    if constexpr (STREAM) asm volatile(text(" nt") : : "s"(m0), "s"(r), __VA_ARGS__ : "memory", "m0", "scc"); \
+    else asm volatile(text("") : : "s"(m0), "s"(r), __VA_ARGS__ : "memory", "m0", "scc");         \
+  } while (0)
+  if constexpr (N == 1) KF_EMIT(KF_TILE1, "v"(off[0]));
+  else if constexpr (N == 2) KF_EMIT(KF_TILE2, "v"(off[0]), "v"(off[1]));
+  else if constexpr (N == 3) KF_EMIT(KF_TILE3, "v"(off[0]), "v"(off[1]), "v"(off[2]));
+  else if constexpr (N == 4) KF_EMIT(KF_TILE4, "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]));
+  else {
+    dma_tile<4, STREAM>(r, to, off);
+    dma_tile<N - 4, STREAM>(r, to + 4096u, off + 4);
   }
+#undef KF_EMIT
 }
 
 constexpr int kStep = 32;     // keys per unit
-constexpr int kPagedRing = 2; // steps of a worker in flight
 
 // K/V bytes of a call from which its loads are marked as read once. Such loads
 // do not go through the 256 MB memory-side cache, which costs the others a
@@ -128,9 +137,21 @@ __device__ inline int run_length(const PagedParams& p, int total) {
   return max(p.least, (total * p.heads + p.workers - 1) / p.workers);
 }
 
+// A unit: a step of row group hh of request b, with `rem` keys of the request
+// from its first on. begin: 1 if a segment begins with it, 2 if that is the
+// row group's first step.
+struct Unit {
+  int b, hh, rem, begin;
+};
+
 template <typename T> struct PBias;  // P = 2^(s - m + bias), see paged_kernel
 template <> struct PBias<_Float16> { static constexpr float v = 7.f; };
 template <> struct PBias<__bf16> { static constexpr float v = 0.f; };
+
+// 1 KB loads of a row group's Q tile.
+constexpr int q_loads(int DT, int QB) { return 16 * QB * (DT / 8) / 64; }
+// LDS of a worker: two steps of K and V, and the Q tiles of two segments.
+constexpr int worker_lds(int DT, int QB) { return 2 * (2 * kStep * DT * 2 + q_loads(DT, QB) * 1024); }
 
 template <typename T, int DT, int QB>
 __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
@@ -140,50 +161,21 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
   constexpr int VT = kStep * DT;      // elements of one K (or V) step tile
   constexpr int NGI = 16 * CPR / 64;  // 1 KB loads per 16-row group of K (or V)
   constexpr int NL = 4 * NGI;         // loads per step: two groups of K and of V
+  constexpr int NQ = q_loads(DT, QB);
   using Tile = SwizzledTile<CPR>;
-  __shared__ __attribute__((aligned(16))) uint16_t ring[kPagedRing * 2 * VT];
+  static_assert(NL + NQ < 64, "the counter of outstanding loads has six bits");
+  // Per ring slot: a step's K and V tiles, and the Q tile of the segment that
+  // begins with it.
+  __shared__ __attribute__((aligned(16))) uint16_t smem[worker_lds(DT, QB) / 2];
 
   const int lane = threadIdx.x;
   const int l16 = lane & 15, g16 = lane >> 4;
   const const_i32 lengths = (const_i32)(uintptr_t)p.lengths;
 
-  // This worker's run of units, and where it begins: request b, whose first
-  // unit is `start`. The first 64 requests' lengths are read once.
-  const int worker = blockIdx.x;
-  const int len0 = lane < p.B ? visible(p, p.lengths[lane]) : 0;
-  const int mine0 = (len0 + kStep - 1) / kStep;
-  const int sum0 = wave_scan(mine0);
-  int total = __builtin_amdgcn_readlane(sum0, 63);
-  if (p.B > 64) total += steps_from(p, 64, lane);
-  const int run = run_length(p, total);
-  const int u = worker * run;
-  if (u >= total * p.heads) return;  // more workers than runs
-  int b, start, len;
-  uint64_t past = __builtin_amdgcn_ballot_w64(sum0 * p.heads > u);
-  if (past) {
-    b = __builtin_ctzll(past);
-    len = __builtin_amdgcn_readlane(len0, b);
-    start = (__builtin_amdgcn_readlane(sum0, b) - __builtin_amdgcn_readlane(mine0, b)) * p.heads;
-  } else {
-    start = __builtin_amdgcn_readlane(sum0, 63) * p.heads;
-    for (b = 64;; b += 64) {
-      const int mine = lane_steps(p, b + lane) * p.heads;
-      const int sum = wave_scan(mine);
-      past = __builtin_amdgcn_ballot_w64(start + sum > u);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        start += __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(mine, at);
-        b += at;
-        break;
-      }
-      start += __builtin_amdgcn_readlane(sum, 63);
-    }
-    len = visible(p, lengths[b]);
-  }
-  int n = (len + kStep - 1) / kStep;
-  int hh = (u - start) / n;
-  int s0 = (u - start) - hh * n;
-  int left = run;
+  // The first 64 requests' lengths. What does not depend on them is computed
+  // while they are on their way: a short call is one chain of loads (lengths,
+  // pages, keys), 5 us of it in this kernel.
+  const int raw0 = p.lengths[min(lane, p.B - 1)];
 
   // Per-lane plan of a group's loads: this lane's 16-byte chunk within the 16
   // rows (kOOB for head-dim padding). The swizzle key has a period of 16 rows,
@@ -195,263 +187,397 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     const int r = pc / CPR;
     const int c = (pc % CPR) ^ Tile::key(r);
     const bool ok = c * 8 < p.D;
-    koff[k] = ok ? (uint32_t)(r * p.k_ss + c * 8) * 2u : kOOB;
-    voff[k] = ok ? (uint32_t)(r * p.v_ss + c * 8) * 2u : kOOB;
+    koff[k] = ok ? (uint32_t)r * p.k_row + c * 16u : kOOB;
+    voff[k] = ok ? (uint32_t)r * p.v_row + c * 16u : kOOB;
   }
-  const uint32_t ring0 = lds_addr(ring);
+  // The parameters that only the ends of segments need are read again there:
+  // the scalar registers do not hold them all, and spilled ones cost vector
+  // instructions in every step. (The empty asm keeps the compiler from reading
+  // them once.)
+  auto cold = [&]() -> const PagedParams KF_CONST& {
+    auto ptr = (const PagedParams KF_CONST*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(ptr));
+    return *ptr;
+  };
+  // And of the Q tile's loads and the outputs, for the first row group of a
+  // KV head (of most, the only one).
+  auto query_offset = [&](const auto& c, int k, int rb) -> uint32_t {
+    const int pc = k * 64 + lane;
+    const int r = pc / CPR;
+    const int ch = (pc % CPR) ^ Tile::key(r);
+    const int rho = rb * c.rows + r;
+    const int g = rho / c.Sq, i = rho - g * c.Sq;
+    const bool ok = r < c.rows && rho < c.G * c.Sq && ch * 8 < c.D;
+    return ok ? (uint32_t)(g * c.q_sh + i * c.q_ss + ch * 8) * 2u : kOOB;
+  };
+  struct Row {
+    uint32_t out;  // byte offset of the row within its KV head's outputs, kOOB if there is none
+    int lag;       // keys that it sees fewer than the last query token does
+  };
+  auto output_row = [&](const auto& c, int qb, int rb) -> Row {
+    const int r = qb * 16 + l16, rho = rb * c.rows + r;
+    const int g = rho / c.Sq, i = rho - g * c.Sq;
+    return {r < c.rows && rho < c.G * c.Sq ? (uint32_t)(g * c.o_sh + i * c.o_ss) * 2u : kOOB,
+            c.causal ? c.Sq - 1 - i : 0};
+  };
+  // (One row block only: more have no registers to spare, and more to do per
+  // segment anyway.)
+  constexpr bool KEEP = QB == 1;
+  uint32_t qoff[KEEP ? NQ : 1];
+  Row row0[KEEP ? QB : 1];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) qoff[k] = query_offset(p, k, 0);
+    row0[0] = output_row(p, 0, 0);
+  }
+
+  // This worker's run of units, and where it begins: request b, whose first
+  // unit is `start`.
+  const int worker = blockIdx.x;
+  const int len0 = lane < p.B ? visible(p, raw0) : 0;
+  const int mine0 = (len0 + kStep - 1) / kStep;
+  const int sum0 = wave_scan(mine0);
+  int total = __builtin_amdgcn_readlane(sum0, 63);
+  if (p.B > 64) total += steps_from(p, 64, lane);
+  const int run = run_length(p, total);
+  const int u = worker * run;
+  if (u >= total * p.heads) return;  // more workers than runs
+  const int count = min(run, total * p.heads - u);
+  Unit at;  // the next one to load
+  int len, start;
+  uint64_t past = __builtin_amdgcn_ballot_w64(sum0 * p.heads > u);
+  if (past) {
+    at.b = __builtin_ctzll(past);
+    len = __builtin_amdgcn_readlane(len0, at.b);
+    start = (__builtin_amdgcn_readlane(sum0, at.b) - __builtin_amdgcn_readlane(mine0, at.b)) * p.heads;
+  } else {
+    start = __builtin_amdgcn_readlane(sum0, 63) * p.heads;
+    for (at.b = 64;; at.b += 64) {
+      const int mine = lane_steps(p, at.b + lane) * p.heads;
+      const int sum = wave_scan(mine);
+      past = __builtin_amdgcn_ballot_w64(start + sum > u);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        start += __builtin_amdgcn_readlane(sum, i) - __builtin_amdgcn_readlane(mine, i);
+        at.b += i;
+        break;
+      }
+      start += __builtin_amdgcn_readlane(sum, 63);
+    }
+    len = visible(p, lengths[at.b]);
+  }
+  const int n0 = (len + kStep - 1) / kStep;
+  at.hh = (u - start) / n0;
+  const int s0 = (u - start) - at.hh * n0;
+  at.rem = len - kStep * s0;
+  at.begin = s0 == 0 ? 2 : 1;
+  // Its first 16-row group: column of the table, group of that page.
+  int column = 2 * s0 / p.gpp, part = 2 * s0 - column * p.gpp;
+
+  const uint32_t lds0 = lds_addr(smem);
   const bool stream = (int64_t)total * p.heads * (kStep * 4 * p.D) > kStreamBytes;
 
-  for (;;) {
-    // One segment: steps [s0, s1) of row group hh of request b.
-    const int s1 = min(n, s0 + left);
-    const int kvh = hh / p.nrb, rb = hh % p.nrb;
-    const int R = p.G * p.Sq;
-    const uint16_t* kh = p.k + kvh * p.k_sh;
-    const uint16_t* vh = p.v + kvh * p.v_sh;
-    const const_i32 table = (const_i32)(uintptr_t)(p.tables + b * p.t_sb);
+  // Of the request and head under way at `at`.
+  const_i32 table;
+  uint64_t kh, vh;
+  auto head_base = [&](const auto& c) {
+    const int kvh = at.hh / c.nrb;
+    kh = (uint64_t)(uintptr_t)(c.k + kvh * c.k_sh);
+    vh = (uint64_t)(uintptr_t)(c.v + kvh * c.v_sh);
+  };
+  auto table_base = [&](const auto& c) {
+    table = (const_i32)(uintptr_t)(c.tables + at.b * c.t_sb);
+  };
+  table_base(p);
+  head_base(p);
+  // Pages of the two groups of unit `at`, the first's where the second is not
+  // visible. They are read by the scalar unit one unit before they are needed.
+  int page[2], row1;
+  auto look_up = [&] {
+    const bool same = part + 1 < p.gpp;
+    row1 = same ? (part + 1) * 16 : 0;
+    page[0] = table[(uint32_t)column];
+    page[1] = table[(uint32_t)(same || at.rem <= 16 ? column : column + 1)];
+  };
+  look_up();
+  // `at` to the unit behind: next step, row group, or request that holds keys.
+  auto advance = [&] {
+    at.rem -= kStep;
+    if (at.rem > 0) {
+      at.begin = 0;
+      part += 2;
+      if (part >= p.gpp) part -= p.gpp, ++column;
+      if (part >= p.gpp) part -= p.gpp, ++column;
+      return;
+    }
+    at.begin = 2;
+    column = part = 0;
+    const auto& c = cold();
+    if (++at.hh == c.heads) {
+      at.hh = 0;
+      do {
+        if (++at.b == c.B) return;  // behind the last unit
+        len = min(max(((const_i32)(uintptr_t)c.lengths)[at.b], 0), c.cap);
+      } while (len == 0);
+      table_base(c);
+    }
+    at.rem = len;
+    head_base(c);
+  };
 
-    // Q rows as MFMA B operands: lane l = packed row qb * 16 + l % 16, k slots
-    // = head dims 32 dc + 8 (l / 16) .. + 7.
-    u32x4 qf[QB][NDC];
+  // What is in the ring slots: the unit, and the visible rows of its two
+  // groups (0 for a page outside the pool).
+  Unit held[2] = {at, at};
+  int seen[2][2] = {{0, 0}, {0, 0}};
+  // Loads of unit `at` into a slot: the Q tile if a segment begins, then K and
+  // V. All of the kernel's loads from here on are direct-to-LDS, so that the
+  // explicit waits below are the only ones.
+  auto issue = [&](bool more, auto slot_c) {
+    constexpr int slot = decltype(slot_c)::value;
+    const uint32_t kv0 = lds0 + slot * 2 * VT * 2;
+    if (at.begin) {
+      const auto& c = cold();
+      const int kvh = at.hh / c.nrb;
+      const int rb = at.hh - kvh * c.nrb;
+      const auto qr = make_rsrc(c.q + at.b * c.q_sb + (int64_t)kvh * c.G * c.q_sh, c.q_bytes);
+      const uint32_t q0 = lds0 + 4 * VT * 2 + slot * NQ * 1024u;
+      if (KEEP && rb == 0) {
+        if constexpr (KEEP) dma_tile<NQ, false>(qr, q0, qoff);
+      } else {
+        uint32_t off[NQ];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      const int rho = rb * p.rows + qb * 16 + l16;
-      const bool row = qb * 16 + l16 < p.rows && rho < R;
-      const int g = row ? rho / p.Sq : 0, i = row ? rho % p.Sq : 0;
-      const uint16_t* qrow = p.q + b * p.q_sb + (kvh * p.G + g) * p.q_sh + i * p.q_ss;
-#pragma unroll
-      for (int dc = 0; dc < NDC; ++dc) {
-        const int d = 32 * dc + 8 * g16;
-        qf[qb][dc] = row && d < p.D ? ldg16(qrow + d) : zero_u4();
+        for (int k = 0; k < NQ; ++k) off[k] = query_offset(c, k, rb);
+        dma_tile<NQ, false>(qr, q0, off);
       }
     }
-
-    // The pages of a step's two 16-row groups (column and first row of each,
-    // the last visible group's where the second lies behind it). Read one
-    // step before they are needed, all of a ring's at the segment's start.
-    struct StepPages {
-      int page[2], row0[2];
-    };
-    auto look_up = [&](int s) {
-      StepPages sp;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const uint32_t gi = min(2 * s + g, (len - 1) >> 4);
-        uint32_t column = __umulhi(gi, p.gpp_inv);
-        uint32_t rest = gi - column * p.gpp;
-        const bool up = rest >= (uint32_t)p.gpp;  // the quotient may be one short
-        column += up;
-        rest -= up ? p.gpp : 0;
-        sp.page[g] = table[column];
-        sp.row0[g] = (int)rest * 16;
+    for (int g = 0; g < 2; ++g) {
+      const uint32_t m0 = kv0 + g * 16 * DT * 2;
+      const uint32_t id = __builtin_amdgcn_readfirstlane(page[g]);
+      const int row = g == 0 ? part * 16 : row1;
+      int rows = at.rem - 16 * g;
+      rows = rows < 0 || id >= (uint32_t)p.pages ? 0 : rows < 16 ? rows : 16;
+      const uint64_t ka = kh + (rows ? (uint64_t)id * p.k_page + (uint32_t)row * (uint64_t)p.k_row : 0);
+      const uint64_t va = vh + (rows ? (uint64_t)id * p.v_page + (uint32_t)row * (uint64_t)p.v_row : 0);
+      // The extent ends with the last visible row.
+      const auto kr = make_rsrc((const void*)(uintptr_t)ka, rows ? (rows - 1) * p.k_row + 2 * p.D : 0);
+      const auto vr = make_rsrc((const void*)(uintptr_t)va, rows ? (rows - 1) * p.v_row + 2 * p.D : 0);
+      if (stream) {
+        dma_tile<NGI, true>(kr, m0, koff);
+        dma_tile<NGI, true>(vr, m0 + VT * 2, voff);
+      } else {
+        dma_tile<NGI, false>(kr, m0, koff);
+        dma_tile<NGI, false>(vr, m0 + VT * 2, voff);
       }
-      return sp;
-    };
-    // Loads of step s into its slot; visible rows per group, 0 where the page
-    // is not in the pool.
-    int vis[kPagedRing][2];
-    auto issue = [&](int s, const StepPages& sp, auto slot_c) {
-      constexpr int slot = decltype(slot_c)::value;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const uint32_t m0 = ring0 + slot * 2 * VT * 2 + g * 16 * DT * 2;
-        const int page = __builtin_amdgcn_readfirstlane(sp.page[g]);
-        int seen = min(max(len - 32 * s - 16 * g, 0), 16);
-        if (page < 0 || page >= p.pages) seen = 0;
-        const int64_t at = seen > 0 ? page : 0;
-        const auto kr = make_rsrc(kh + at * p.k_sp + sp.row0[g] * p.k_ss, rows_extent(seen, p.k_ss, p.D));
-        const auto vr = make_rsrc(vh + at * p.v_sp + sp.row0[g] * p.v_ss, rows_extent(seen, p.v_ss, p.D));
-        if (stream) {
-#pragma unroll
-          for (int k = 0; k < NGI; ++k) {
-            dma16_r<true>(kr, m0 + k * 1024u, koff[k]);
-            dma16_r<true>(vr, m0 + VT * 2 + k * 1024u, voff[k]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < NGI; ++k) {
-            dma16_r<false>(kr, m0 + k * 1024u, koff[k]);
-            dma16_r<false>(vr, m0 + VT * 2 + k * 1024u, voff[k]);
-          }
-        }
-        vis[slot][g] = seen;
-      }
-    };
-    StepPages first[kPagedRing];
-    static_for<0, kPagedRing>([&](auto sc) { first[decltype(sc)::value] = look_up(s0 + decltype(sc)::value); });
-    StepPages next = look_up(s0 + kPagedRing);
-    static_for<0, kPagedRing>([&](auto sc) {
-      if (s0 + decltype(sc)::value < s1) issue(s0 + decltype(sc)::value, first[decltype(sc)::value], sc);
-    });
+      seen[slot][g] = rows;
+    }
+    held[slot] = at;
+    if (more) {
+      advance();
+      look_up();
+    }
+  };
 
-    f32x4 oacc[QB][NDB];  // O^T: lane l, register r = head dim 16 db + 4 (l / 16) + r of row l % 16
-    float m_i[QB], l_i[QB];
-    int lim[QB];  // keys before lim are visible to this lane's row
+  // The segment under way.
+  u32x4 qf[QB][NDC];    // Q rows as MFMA B operands: lane l = packed row qb * 16 + l % 16
+  f32x4 oacc[QB][NDB];  // O^T: lane l, register r = head dim 16 db + 4 (l / 16) + r of row l % 16
+  float m_i[QB], l_i[QB];
+  Row row[QB];          // this lane's rows
+  const int most_lag = p.causal ? p.Sq - 1 : 0;
+  bool from_start = false;  // whether it began with the row group's first step
+
+  auto begin_segment = [&](const Unit& w, auto slot_c) {
+    constexpr int slot = decltype(slot_c)::value;
+    const uint16_t* qs = smem + 4 * VT + slot * NQ * 512;
+    const int rb = w.hh % cold().nrb;
+    from_start = w.begin == 2;
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+      for (int dc = 0; dc < NDC; ++dc) qf[qb][dc] = lds_read16(qs + Tile::chunk(qb * 16 + l16, 4 * dc + g16) * 8);
       m_i[qb] = kNegInf;
       l_i[qb] = 0.f;
-      lim[qb] = p.causal ? len - (p.Sq - 1 - (rb * p.rows + qb * 16 + l16) % p.Sq) : len;
+      row[qb] = KEEP && rb == 0 ? row0[0] : output_row(cold(), qb, rb);
 #pragma unroll
       for (int db = 0; db < NDB; ++db) oacc[qb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int least_lim = p.causal ? len - (p.Sq - 1) : len;
+  };
 
-    auto step = [&](int s, auto slot_c) {
-      constexpr int slot = decltype(slot_c)::value;
-      const uint16_t* Ks = ring + slot * 2 * VT;
-      const uint16_t* Vs = Ks + VT;
-      // K rows as MFMA A operands: lane = key kb * 16 + l % 16, slots = head dims.
-      u32x4 ka[2][NDC];
+  auto step = [&](const Unit& w, auto slot_c) {
+    constexpr int slot = decltype(slot_c)::value;
+    const uint16_t* Ks = smem + slot * 2 * VT;
+    const uint16_t* Vs = Ks + VT;
+    // K rows as MFMA A operands: lane = key kb * 16 + l % 16, slots = head dims.
+    u32x4 ka[2][NDC];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int dc = 0; dc < NDC; ++dc) ka[kb][dc] = lds_read16(Ks + Tile::chunk(kb * 16 + l16, 4 * dc + g16) * 8);
+    const bool masked = seen[slot][0] + seen[slot][1] < kStep || w.rem - most_lag < kStep;
+    u32x4 pk[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      // S^T: lane l, register r = key kb * 16 + 4 (l / 16) + r of row l % 16.
+      f32x4 sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) sc[kb] = Elem<T>::mfma16(ka[kb][dc], qf[qb][dc], sc[kb]);
+        sc[kb] *= p.scale_log2;
+      }
+      // Masked after the scale, so that a scale of zero leaves -inf.
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int c = 4 * g16 + r;
+            const bool in = c < seen[slot][kb] && 16 * kb + c < w.rem - row[qb].lag;
+            sc[kb][r] = in ? sc[kb][r] : kNegInf;
+          }
+      }
+      float mx = kNegInf;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int dc = 0; dc < NDC; ++dc) ka[kb][dc] = lds_read16(Ks + Tile::chunk(kb * 16 + l16, 4 * dc + g16) * 8);
-      const bool masked = vis[slot][0] + vis[slot][1] < kStep || (s + 1) * kStep > least_lim;
-      u32x4 pk[QB];
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[kb][r]);
+      mx = wave_group16_max(mx);
+      if (m_i[qb] == kNegInf) {
+        m_i[qb] = mx;
+      } else {
+        const bool grow = mx > m_i[qb] + kRescaleThreshold;
+        if (wave_any(grow)) {
+          const float alpha = grow ? fast_exp2(m_i[qb] - mx) : 1.f;
+          l_i[qb] *= alpha;
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        // S^T: lane l, register r = key kb * 16 + 4 (l / 16) + r of row l % 16.
-        f32x4 sc[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int dc = 0; dc < NDC; ++dc) sc[kb] = Elem<T>::mfma16(ka[kb][dc], qf[qb][dc], sc[kb]);
-          sc[kb] *= p.scale_log2;
+          for (int db = 0; db < NDB; ++db) oacc[qb][db] *= alpha;
+          m_i[qb] = grow ? mx : m_i[qb];
         }
-        // Masked after the scale, so that a scale of zero leaves -inf.
-        if (masked) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int c = 4 * g16 + r;
-              const bool seen = c < vis[slot][kb] && s * kStep + 16 * kb + c < lim[qb];
-              sc[kb][r] = seen ? sc[kb][r] : kNegInf;
-            }
-        }
-        float mx = kNegInf;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[kb][r]);
-        mx = wave_group16_max(mx);
-        if (m_i[qb] == kNegInf) {
-          m_i[qb] = mx;
-        } else {
-          const bool grow = mx > m_i[qb] + kRescaleThreshold;
-          if (wave_any(grow)) {
-            const float alpha = grow ? fast_exp2(m_i[qb] - mx) : 1.f;
-            l_i[qb] *= alpha;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) oacc[qb][db] *= alpha;
-            m_i[qb] = grow ? mx : m_i[qb];
-          }
-        }
-        // P in 16 bits for the second product. With m up to 8 below the
-        // maximum and the bias, P stays below 2^8 in bf16 and 2^15 in fp16,
-        // whose smallest value 2^-24 is then 2^-31 of the maximum: a long tail
-        // of small P is not lost.
-        const float msub = (m_i[qb] == kNegInf) ? 0.f : m_i[qb] - PBias<T>::v;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[kb][r] = fast_exp2(sc[kb][r] - msub);
-        // P^T as the B operand of O^T += V^T P^T: slot t of lane group g holds
-        // key 4 g + t (t < 4) or 16 + 4 g + t - 4 (t >= 4).
-        pk[qb][0] = pack2<T>(sc[0][0], sc[0][1]);
-        pk[qb][1] = pack2<T>(sc[0][2], sc[0][3]);
-        pk[qb][2] = pack2<T>(sc[1][0], sc[1][1]);
-        pk[qb][3] = pack2<T>(sc[1][2], sc[1][3]);
-        // The denominator sums the rounded P that the second product uses.
-        l_i[qb] += sum2_acc<T>(pk[qb][0], sum2_acc<T>(pk[qb][1], 0.f)) +
-                   sum2_acc<T>(pk[qb][2], sum2_acc<T>(pk[qb][3], 0.f));
       }
-      // V^T A operands by transposed reads: lane (g, i) receives V[key][16 db + i]
-      // for the keys of slot t above.
+      // P in 16 bits for the second product. With m up to 8 below the maximum
+      // and the bias, P stays below 2^8 in bf16 and 2^15 in fp16, whose
+      // smallest value 2^-24 is then 2^-31 of the maximum: a long tail of
+      // small P is not lost.
+      const float msub = (m_i[qb] == kNegInf) ? 0.f : m_i[qb] - PBias<T>::v;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int col = 16 * db + 4 * (l16 & 3);
-        const u32x2 lo = lds_read_tr16(Vs + Tile::elem(4 * g16 + (l16 >> 2), col));
-        const u32x2 hi = lds_read_tr16(Vs + Tile::elem(16 + 4 * g16 + (l16 >> 2), col));
-        const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
-      }
-    };
-
-    for (int j0 = s0; j0 < s1; j0 += kPagedRing) {
-      static_for<0, kPagedRing>([&](auto sc) {
-        const int s = j0 + decltype(sc)::value;
-        if (s < s1) {
-          // This step's loads are done once only those of later ones are left.
-          const int later = min(kPagedRing - 1, s1 - 1 - s);
-          static_for<0, kPagedRing>([&](auto lc) {
-            if (later == decltype(lc)::value) KF_WAIT_VMCNT(decltype(lc)::value * NL);
-          });
-          step(s, sc);
-          if (s + kPagedRing < s1) {
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read
-            issue(s + kPagedRing, next, sc);
-            next = look_up(s + kPagedRing + 1);
-          }
-        }
-      });
+        for (int r = 0; r < 4; ++r) sc[kb][r] = fast_exp2(sc[kb][r] - msub);
+      // P^T as the B operand of O^T += V^T P^T: slot t of lane group g holds
+      // key 4 g + t (t < 4) or 16 + 4 g + t - 4 (t >= 4).
+      pk[qb][0] = pack2<T>(sc[0][0], sc[0][1]);
+      pk[qb][1] = pack2<T>(sc[0][2], sc[0][3]);
+      pk[qb][2] = pack2<T>(sc[1][0], sc[1][1]);
+      pk[qb][3] = pack2<T>(sc[1][2], sc[1][3]);
+      // The denominator sums the rounded P that the second product uses.
+      l_i[qb] += sum2_acc<T>(pk[qb][0], sum2_acc<T>(pk[qb][1], 0.f)) +
+                 sum2_acc<T>(pk[qb][2], sum2_acc<T>(pk[qb][3], 0.f));
     }
-    static_assert((kPagedRing - 1) * NL < 64, "the counter of outstanding loads has six bits");
+    // V^T A operands by transposed reads: lane (g, i) receives V[key][16 db + i]
+    // for the keys of slot t above.
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const int col = 16 * db + 4 * (l16 & 3);
+      const u32x2 lo = lds_read_tr16(Vs + Tile::elem(4 * g16 + (l16 >> 2), col));
+      const u32x2 hi = lds_read_tr16(Vs + Tile::elem(16 + 4 * g16 + (l16 >> 2), col));
+      const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
+    }
+  };
 
-    // O and LSE, or the partial of this worker.
-    const bool whole = s0 == 0 && s1 == n;
-    const int64_t slot = (int64_t)(worker + b * p.heads + hh) * p.rows;
+  // O and LSE of the row group, or this worker's partial of it: NS stores in
+  // every case (lanes without an output, and whole stores where there is
+  // nothing to say, lie outside their resource), so that the waits can count
+  // them instead of waiting for them.
+  constexpr int NS = QB * (NDB + 1) + 1;
+  auto end_segment = [&](const Unit& w) {
+    const bool whole = from_start && w.rem <= kStep;
+    const auto& c = cold();
+    const int kvh = w.hh / c.nrb, rb = w.hh - kvh * c.nrb;
+    const int group = w.b * c.heads + w.hh;
+    const int64_t slot = (int64_t)(worker + group) * c.rows;
+    // kOOB is the top bit, which no offset inside a resource has.
+    const uint32_t one_lane = g16 == 0 ? 0u : kOOB;
+    auto beyond = [&](int d) -> uint32_t { return (uint32_t)(c.D - 1 - d) & kOOB; };
+    float inv[QB], lse[QB];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      const int r = qb * 16 + l16;
-      const int rho = rb * p.rows + r;
       const float lt = wave_group16_sum(l_i[qb]);
-      if (r >= p.rows || rho >= R) continue;
-      const float inv = lt > 0.f ? 1.f / lt : 0.f;
-      const float lse = lt > 0.f ? (m_i[qb] - PBias<T>::v + fast_log2(lt)) * kLn2 : kNegInf;
-      const int h = kvh * p.G + rho / p.Sq, i = rho % p.Sq;
+      inv[qb] = lt > 0.f ? 1.f / lt : 0.f;
+      lse[qb] = lt > 0.f ? (m_i[qb] - PBias<T>::v + fast_log2(lt)) * kLn2 : kNegInf;
+    }
+    if (whole) {
+      const auto orr = make_rsrc(c.o + w.b * c.o_sb + (int64_t)kvh * c.G * c.o_sh, c.o_bytes);
+      const auto lrr = make_rsrc(c.lse + ((int64_t)w.b * c.Hq + kvh * c.G) * c.Sq, c.lse ? c.G * c.Sq * 4u : 0u);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int d = 16 * db + 4 * g16;
-        if (d >= p.D) continue;
-        const f32x4 ov = oacc[qb][db] * inv;
-        if (whole) {
-          u32x2 w;
-          w[0] = pack2<T>(ov[0], ov[1]);
-          w[1] = pack2<T>(ov[2], ov[3]);
-          *reinterpret_cast<u32x2*>(p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss + d) = w;
-        } else {
-          *reinterpret_cast<f32x4*>(p.part_o + (slot + r) * p.D + d) = ov;
+      for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const int d = 16 * db + 4 * g16;
+          const f32x4 ov = oacc[qb][db] * inv[qb];
+          const u32x2 o2 = {pack2<T>(ov[0], ov[1]), pack2<T>(ov[2], ov[3])};
+          __builtin_amdgcn_raw_buffer_store_b64(o2, orr, row[qb].out + d * 2u | beyond(d), 0, 0);
         }
+        const int rho = rb * c.rows + qb * 16 + l16;
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse[qb]), lrr, rho * 4u | (row[qb].out & kOOB) | one_lane, 0, 0);
       }
-      if (g16 == 0) {
-        if (!whole) p.part_lse[slot + r] = lse;
-        else if (p.lse) p.lse[((int64_t)b * p.Hq + h) * p.Sq + i] = lse;
+    } else {
+      const auto orr = make_rsrc(c.part_o + slot * c.D, (uint32_t)(c.rows * c.D * 4));
+      const auto lrr = make_rsrc(c.part_lse + slot, c.rows * 4u);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const int r = qb * 16 + l16;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const int d = 16 * db + 4 * g16;
+          const f32x4 ov = oacc[qb][db] * inv[qb];
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, ov), orr,
+                                                 (uint32_t)(r * c.D + d) * 4u | (row[qb].out & kOOB) | beyond(d), 0, 0);
+        }
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse[qb]), lrr, r * 4u | (row[qb].out & kOOB) | one_lane, 0, 0);
       }
     }
-
     // The row group's first worker says how many there are: the steps behind
     // its own fill whole runs.
-    if (s0 == 0 && lane == 0) {
-      p.parts[2 * (b * p.heads + hh)] = worker;
-      p.parts[2 * (b * p.heads + hh) + 1] = 1 + (n - s1 + run - 1) / run;
-    }
+    const u32x2 parts = {(uint32_t)worker, (uint32_t)(1 + ((w.rem - 1) / kStep + run - 1) / run)};
+    __builtin_amdgcn_raw_buffer_store_b64(parts, make_rsrc(c.parts + 2 * (int64_t)group, 8u),
+                                          from_start && lane == 0 ? 0u : kOOB, 0, 0);
+  };
 
-    left -= s1 - s0;
-    if (left <= 0) break;
-    // The next segment: next row group, or the next request that holds keys.
-    s0 = 0;
-    if (++hh == p.heads) {
-      hh = 0;
-      do {
-        if (++b == p.B) return;
-        len = visible(p, lengths[b]);
-      } while (len == 0);
-      n = steps_of(p, len);
+  // Two units are in flight, whatever segments they belong to: a segment's
+  // first steps load while the one before it is computed and written.
+  // Waits until only what was issued behind a unit's loads is left: the
+  // stores of the segment that ended before it, and the next unit's loads.
+  auto wait = [&](bool stores, int later) {
+    if (!stores && later == 1) {
+      KF_WAIT_VMCNT(NL);
+    } else {
+      static_for<0, 6>([&](auto cc) {
+        constexpr int c = decltype(cc)::value;
+        constexpr int n = (c & 1 ? NS : 0) + (c >= 2 ? NL : 0) + (c >= 4 ? NQ : 0);
+        if (c != 2 && 2 * later + stores == c) KF_WAIT_VMCNT(n < 63 ? n : 63);
+      });
     }
+  };
+  bool ended = false;
+  for (int j0 = -2; j0 < count; j0 += 2) {
+    static_for<0, 2>([&](auto sc) {
+      constexpr int slot = decltype(sc)::value;
+      const int j = j0 + slot;
+      if (j >= 0 && j < count) {
+        const bool next = j + 1 < count;
+        wait(ended, next ? held[1 - slot].begin ? 2 : 1 : 0);
+        const Unit w = held[slot];
+        if (w.begin) begin_segment(w, sc);
+        step(w, sc);
+        ended = !next || w.rem <= kStep;
+        if (ended) end_segment(w);
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read
+      }
+      if (j + 2 < count) issue(j + 3 < count, sc);
+    });
   }
 }
 
@@ -460,19 +586,26 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
 // whole. Bound by its chain of loads: which partials, then all of them. The
 // first wave alone takes what one round trip brings; more partials the waves
 // share, and combine through LDS in their order.
+// Half the partials in flight of the contiguous decode's merge (half the
+// registers, twice the rows at once: 8192 rows of two or three partials 7.3 us
+// with 16, 5.7 with 8, 5.3 with 4; 768 rows of 40 partials 5.3, 4.2 and 4.5).
+constexpr int kPartsU = 8;
+// With W = 1, four rows share a workgroup.
 template <typename T, int QL, int W>
-__global__ __launch_bounds__(64 * W) void paged_merge_kernel(const PagedParams p) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(const PagedParams p) {
   const int lane = threadIdx.x & 63, wave = wave_index();
-  const int r = blockIdx.x % p.rows;
-  const int bh = blockIdx.x / p.rows;
+  const int row = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int r = row % p.rows;
+  const int bh = row / p.rows;
+  if (W == 1 && bh >= p.B * p.heads) return;
   const int hh = bh % p.heads, b = bh / p.heads;
   const int kvh = hh / p.nrb, rho = (hh % p.nrb) * p.rows + r;
   // What the workers wrote is not there for a request without keys.
   const int len = ((const_i32)(uintptr_t)p.lengths)[b];
   const int w0 = ((const_i32)(uintptr_t)p.parts)[2 * bh], parts = ((const_i32)(uintptr_t)p.parts)[2 * bh + 1];
   if (rho >= p.G * p.Sq) return;
-  const bool alone = W == 1 || len <= 0 || parts <= kMergeU * (64 / QL);
-  if (alone && wave > 0) return;
+  const bool alone = W == 1 || len <= 0 || parts <= kPartsU * (64 / QL);
+  if (W > 1 && alone && wave > 0) return;
   const int h = kvh * p.G + rho / p.Sq, i = rho % p.Sq;
   uint16_t* out = p.o + b * p.o_sb + h * p.o_sh + i * p.o_ss;
   float* lse = p.lse ? p.lse + ((int64_t)b * p.Hq + h) * p.Sq + i : nullptr;
@@ -487,13 +620,13 @@ __global__ __launch_bounds__(64 * W) void paged_merge_kernel(const PagedParams p
   const auto lrr = make_rsrc(p.part_lse + slot, (uint32_t)(((int64_t)(parts - 1) * p.rows + 1) * 4));
   const uint32_t ostride = (uint32_t)(p.rows * p.D), lstride = (uint32_t)p.rows;
   if (alone) {
-    merge_row<T, QL>(orr, lrr, ostride, lstride, parts, p.D, out, lse);
+    merge_row<T, QL, kPartsU>(orr, lrr, ostride, lstride, parts, p.D, out, lse);
     return;
   }
   if constexpr (W > 1) {
     __shared__ float sums[W][QL][6];
     const int share = (parts + W - 1) / W;
-    const MergeState mine = merge_splits<QL>(orr, lrr, ostride, lstride, min(wave * share, parts),
+    const MergeState mine = merge_splits<QL, kPartsU>(orr, lrr, ostride, lstride, min(wave * share, parts),
                                              min((wave + 1) * share, parts), p.D);
     if (lane < QL) {
       float* to = sums[wave][lane];
@@ -519,27 +652,28 @@ __global__ __launch_bounds__(64 * W) void paged_merge_kernel(const PagedParams p
 static int paged_row_blocks(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 static int paged_rows(int64_t R) { return (int)(R < 64 ? R : 64); }
 
-// Workers: what the LDS of 256 CUs holds of their rings, 4 KB short of 160.
-static int paged_workers(int64_t D) {
-  const int ring = kPagedRing * 2 * kStep * head_tile(D) * 2;
-  const int per_cu = 156 * 1024 / ring;
+// Workers: what the LDS of 256 CUs holds of them (160 KB each, given out in
+// pieces of 1280 bytes), at most 8 per CU.
+static int paged_workers(int64_t D, int64_t R) {
+  const int lds = (worker_lds(head_tile(D), paged_row_blocks(R)) + 1279) / 1280 * 1280;
+  const int per_cu = 160 * 1024 / lds;
   return 256 * (per_cu < 8 ? per_cu : 8);
 }
 
 static int64_t paged_slots(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
   const int64_t R = Hq / Hkv * Sq;
-  return paged_workers(D) + B * Hkv * ((R + paged_rows(R) - 1) / paged_rows(R));
+  return paged_workers(D, R) + B * Hkv * ((R + paged_rows(R) - 1) / paged_rows(R));
 }
 
 // Waves per row of the merge, from the most partials a row group can have: a
 // head's share of the workers (all of them on one request), cut at both ends.
-// More waves cost launch time, a few tenths of a us where they are not needed
-// (1158 MB over 64 requests: 4.6 us with one wave, 5.0 with four, 7.2 with
-// eight), and save round trips where one row has many partials (131072 keys of
-// one request, 128 partials: 5.9 us with one wave, 4.6 with four).
+// More waves cost launch time where they are not needed (1158 MB over 64
+// requests: 4.6 us with one wave, 5.0 with four, 7.2 with eight) and save round
+// trips where one row has many partials (131072 keys of one request, 128
+// partials: 5.9 us with one wave, 4.6 with four).
 template <typename T, int QL>
 static void launch_merge(const PagedParams& p, hipStream_t stream) {
-  constexpr int kTrip = kMergeU * (64 / QL);  // partials that a wave takes at once
+  constexpr int kTrip = kPartsU * (64 / QL);  // partials that a wave takes at once
   const int64_t rows = (int64_t)p.B * p.heads * p.rows;
   const int share = p.workers / p.heads + 2, steps = p.cap / kStep + 1;
   const int most = share < steps ? share : steps;
@@ -549,7 +683,7 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
   else if (most > kTrip && (rows <= 256 || most > 8 * kTrip))
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 4>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), grid, dim3(64), 0, stream, p);
+    hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
 }
 
 template <typename T, int DT>
@@ -618,12 +752,17 @@ extern "C" int kf_paged_decode(const void* q, const void* k_pages, const void* v
   const int rows = paged_rows(R);
   const int64_t nrb = (R + rows - 1) / rows, heads = Hkv * nrb;
   const int64_t cap = columns * page_size;
-  if (heads * ((cap + kStep - 1) / kStep) > 0x7fffffff / B)
+  if (heads * ((cap + kStep - 1) / kStep) > 0x7f000000 / B)
     return set_error(KF_EUNSUPPORTED, "%s: %lld tables of %lld tokens are beyond 32-bit step numbers", what,
                      (long long)B, (long long)cap);
   if (B * heads * rows > 0x7fffffff) return set_error(KF_EUNSUPPORTED, "%s: grid too large", what);
-  if ((15 * k_strides[2] + D) * 2 > 0x7fffffffLL || (15 * v_strides[2] + D) * 2 > 0x7fffffffLL)
-    return set_error(KF_EUNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB", what);
+  const int64_t q_bytes = ((Hq / Hkv - 1) * q_strides[1] + (Sq - 1) * q_strides[2] + D) * 2;
+  const int64_t o_bytes = ((Hq / Hkv - 1) * o_strides[1] + (Sq - 1) * o_strides[2] + D) * 2;
+  if (q_bytes > 0x7fffffff || o_bytes > 0x7fffffff)
+    return set_error(KF_EUNSUPPORTED, "%s: one KV group of q or o spans more than 2 GiB", what);
+  for (const int64_t* st : {k_strides, v_strides})
+    if ((15 * st[2] + D) * 2 > 0x7fffffffLL || st[0] > 0x7fffffffLL)
+      return set_error(KF_EUNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB, or a page more than 4", what);
   const size_t need = kf_paged_decode_workspace_bytes(B, Hq, Hkv, Sq, D);
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(KF_EINVAL, "%s: workspace of %zu bytes required, got %zu", what, need,
@@ -638,15 +777,18 @@ extern "C" int kf_paged_decode(const void* q, const void* k_pages, const void* v
   p.parts = (int32_t*)((char*)p.part_lse + (slot_rows * sizeof(float) + 255) / 256 * 256);
   p.t_sb = table_stride;
   p.q_sb = q_strides[0]; p.q_sh = q_strides[1]; p.q_ss = q_strides[2];
-  p.k_sp = k_strides[0]; p.k_sh = k_strides[1]; p.k_ss = k_strides[2];
-  p.v_sp = v_strides[0]; p.v_sh = v_strides[1]; p.v_ss = v_strides[2];
+  p.k_sh = k_strides[1]; p.v_sh = v_strides[1];
+  p.k_page = (uint32_t)(2 * k_strides[0]); p.v_page = (uint32_t)(2 * v_strides[0]);
+  p.k_row = (uint32_t)(2 * k_strides[2]); p.v_row = (uint32_t)(2 * v_strides[2]);
   p.o_sb = o_strides[0]; p.o_sh = o_strides[1]; p.o_ss = o_strides[2];
   p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.Sq = (int)Sq; p.D = (int)D; p.G = (int)(Hq / Hkv);
   p.pages = (int)num_pages; p.gpp = (int)(page_size / 16);
-  p.gpp_inv = (uint32_t)((1ull << 32) / p.gpp > 0xffffffffull ? 0xffffffffull : (1ull << 32) / p.gpp);
   p.cap = (int)cap;
   p.rows = rows; p.nrb = (int)nrb; p.heads = (int)heads;
-  p.workers = paged_workers(D); p.least = 1;
+  p.workers = paged_workers(D, R);
+  p.least = 1;
+  p.q_bytes = (uint32_t)q_bytes;
+  p.o_bytes = (uint32_t)o_bytes;
   p.causal = causal != 0;
   p.scale_log2 = scale * kLog2e;
   hipStream_t s = (hipStream_t)stream;
