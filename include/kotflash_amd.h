@@ -266,8 +266,8 @@ int kf_attn_append_decode(const void* q, void* k_cache, void* v_cache, const voi
  * memory: tables [B, columns] (row stride table_stride), the pages of each
  * request in order, -1 where it has none; lengths [B], its tokens; free_pages
  * [num_pages], a stack of the pages that belong to no request; counters [4]:
- * the stack's height, the requests that the last reserve refused, and two
- * that the library uses, 0 between calls. Position j of request b lies in
+ * the stack's height, the requests that the last reserve refused, and two that
+ * are left alone. Position j of request b lies in
  * page tables[b, j / page_size], row j % page_size; its slot is that page
  * times page_size plus that row. Nothing of it is read on the host, so every
  * call can be captured and replayed. A table is changed by one call at a time;
@@ -304,8 +304,8 @@ int kf_page_trim(int32_t* tables, int32_t* lengths, int32_t* free_pages, int32_t
  * pool[slot / page_size, h, slot % page_size, :] = new[b, h, t, :] for slot =
  * slots[b, t] (device int64 [B, Snew], row stride slots_stride), K and V in one
  * launch, bit-exact; a slot outside [0, num_pages * page_size) is skipped. The
- * slots of a call that are not skipped must differ: of two rows with the same
- * slot either may be stored. new_k/new_v may have any strides (int64_t[4]).
+ * slots of a call that are not skipped must differ: a slot that two rows name
+ * holds either's, or a mixture. new_k/new_v may have any strides (int64_t[4]).
  */
 int kf_paged_append(void* k_pages, void* v_pages, const void* new_k, const void* new_v,
                     const int64_t* slots, int64_t B, int64_t H, int64_t Snew, int64_t D,

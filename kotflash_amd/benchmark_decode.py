@@ -14,7 +14,10 @@ The same arguments and report fields as the reference's decode benchmark
 - ``preallocated_hip_separate_append`` (torch-copy append, then the HIP
   decode reading the strided prefix view), ``preallocated_auto`` (the
   ``--append-backend`` choice) and ``preallocated_fused_append`` (one split
-  kernel that also writes the new token, then the merge).
+  kernel that also writes the new token, then the merge);
+- with ``--page-size N``, ``paged_auto``: ``PagedKVCache``, every sequence's
+  pages in no order, its step the table's reserve, the store and the attention
+  (and the trim that takes the token back).
 
 Every candidate's output, attention alone and append + attention, is
 checked against the expanded-SDPA output first (rtol = atol = 8e-3, the
@@ -41,6 +44,7 @@ import torch.nn.functional as F
 from .attention import attention
 from .benchmark import _environment, _sync
 from .cache import PreallocatedKVCache, append_kv_cache
+from .paged import PagedKVCache, PageTable
 
 APPEND_BACKENDS = ("auto", "torch", "hip", "cuda", "fused")
 
@@ -131,6 +135,27 @@ def run(args: argparse.Namespace) -> dict:
                                                   attention_backend=attend_backend)
         return attend, decode
 
+    def paged(page):
+        """Two caches behind tables of their own: one that holds all tokens,
+        one that takes the last at every step."""
+        pages = -(-sk // page)
+        caches = []
+        for held, k, v in ((sk, visible_k, visible_v), (sk - 1, past_k, past_v)):
+            table = PageTable(b, sk, num_pages=b * pages, page_size=page, device=device)
+            table.free_pages.copy_(torch.randperm(b * pages, generator=gen))
+            cache = PagedKVCache(table, hkv, d, dtype=dtype)
+            cache.append(k, v, table.reserve(held))
+            caches.append(cache)
+        whole, growing = caches
+
+        def attend():
+            return whole.attend(q)
+
+        def decode():
+            growing.table.trim(sk - 1)
+            return growing.append_and_attend(q, new_k, new_v, growing.table.reserve(1))
+        return attend, decode
+
     candidates = {
         "hip": legacy("hip"),
         "auto": legacy("auto"),
@@ -140,6 +165,8 @@ def run(args: argparse.Namespace) -> dict:
         "preallocated_auto": preallocated("auto", args.append_backend),
         "preallocated_fused_append": preallocated("hip", "fused"),
     }
+    if args.page_size:
+        candidates["paged_auto"] = paged(args.page_size)
     failures = {}
     correctness = {}
     with torch.inference_mode():
@@ -220,6 +247,8 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
     ap.add_argument("--repeats", type=int, default=5)
     ap.add_argument("--append-backend", choices=APPEND_BACKENDS, default="auto",
                     help="append implementation of the preallocated_auto candidate")
+    ap.add_argument("--page-size", type=int, default=0,
+                    help="also time a paged cache with pages of this many tokens (0: no)")
     ap.add_argument("--seed", type=int, default=1337)
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--output", type=Path, default=None)
@@ -230,6 +259,8 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
         ap.error("--q-heads must be divisible by --kv-heads")
     if args.head_dim % 8 or not 8 <= args.head_dim <= 128:
         ap.error("the split-KV decode needs --head-dim a multiple of 8 in [8, 128]")
+    if args.page_size < 0:
+        ap.error("--page-size must not be negative")
     if args.kv_seq < 1024:
         ap.error("the split-KV decode benchmark needs --kv-seq >= 1024")
     if args.warmup < 1 or args.iterations < 1 or args.repeats < 3:

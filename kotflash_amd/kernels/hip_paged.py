@@ -127,9 +127,35 @@ def append_paged(k_pages, v_pages, new_k, new_v, slots) -> None:
     _hip.paged_append(k_pages, v_pages, new_k, new_v, slots)
 
 
+def check_table(tables, lengths, free_pages, counters) -> None:
+    """The state of a page table as the kernels address it."""
+    if not isinstance(tables, torch.Tensor) or tables.ndim != 2 or min(tables.shape) == 0:
+        raise ValueError("tables must be an int32 tensor of shape [B, columns]")
+    device = tables.device
+    _check_int32("tables", tables, tables.shape, device)
+    _check_int32("lengths", lengths, (tables.shape[0],), device)
+    if not isinstance(free_pages, torch.Tensor) or free_pages.ndim != 1 or free_pages.numel() == 0:
+        raise ValueError("free_pages must be an int32 tensor of shape [pages]")
+    _check_int32("free_pages", free_pages, free_pages.shape, device)
+    _check_int32("counters", counters, (4,), device)
+    if tables.stride(1) != 1 or not all(t.is_contiguous() for t in (lengths, free_pages, counters)):
+        raise ValueError("a page table's state must be dense")
+    if not _hip.is_gfx950(device):
+        raise RuntimeError("page tables on the GPU require an AMD gfx950 (MI355X) device")
+
+
+def _per_request(name: str, value, tables):
+    if isinstance(value, torch.Tensor):
+        _check_int32(name, value, (tables.shape[0],), tables.device)
+        return value.contiguous()
+    return value
+
+
 def reserve_pages(tables, lengths, free_pages, counters, counts: Union[int, torch.Tensor],
                   width: int, page_size: int) -> torch.Tensor:
     """Slots of the new tokens (``kf_page_reserve``)."""
+    check_table(tables, lengths, free_pages, counters)
+    counts = _per_request("counts", counts, tables)
     slots = torch.empty((tables.shape[0], width), device=tables.device, dtype=torch.int64)
     _hip.page_reserve(tables, lengths, free_pages, counters, counts, slots, page_size=page_size)
     return slots
@@ -138,4 +164,6 @@ def reserve_pages(tables, lengths, free_pages, counters, counts: Union[int, torc
 def trim_pages(tables, lengths, free_pages, counters, new_lengths: Union[int, torch.Tensor],
                page_size: int) -> None:
     """Gives back the pages behind the new lengths (``kf_page_trim``)."""
+    check_table(tables, lengths, free_pages, counters)
+    new_lengths = _per_request("new_lengths", new_lengths, tables)
     _hip.page_trim(tables, lengths, free_pages, counters, new_lengths, page_size=page_size)

@@ -14,6 +14,14 @@ implementation and, for attention, a registered backward:
 - ``kotflash_amd::append_decode_(q, k_cache, v_cache, new_k, new_v,
   past_length, scale) -> out`` (fused one-token append + split-KV decode,
   reference kotflash/kernels/triton_decode.py:302-386; mutates both caches)
+- ``kotflash_amd::paged_decode(q, k_pages, v_pages, tables, lengths, causal,
+  scale) -> (out, lse)``, ``kotflash_amd::paged_append_(k_pages, v_pages,
+  new_k, new_v, slots) -> ()``, ``kotflash_amd::page_reserve_(tables, lengths,
+  free_pages, counters, counts, page_size, width) -> slots`` and
+  ``kotflash_amd::page_trim_(tables, lengths, free_pages, counters,
+  new_lengths, page_size) -> ()`` (the paged cache of ``kotflash_amd.paged``,
+  no reference counterpart; ``paged_append_`` mutates both pools, the last two
+  the page table's state)
 
 ``torch.compile`` traces through them without graph breaks: the fake
 implementations give it output shapes, dtypes and strides, and autograd
@@ -29,8 +37,13 @@ import torch
 from .kernels.hip_backward import attention_backward
 from .kernels.hip_decode import attention_forward_strided_append, attention_forward_strided_decode
 from .kernels.hip_forward import attention_forward
+from .kernels.hip_paged import (
+    append_paged, attention_paged, check_append, check_attention, require_readable, reserve_pages,
+    trim_pages,
+)
 
-__all__ = ["attn_fwd", "attn_bwd", "decode", "kv_append_", "append_decode_"]
+__all__ = ["attn_fwd", "attn_bwd", "decode", "kv_append_", "append_decode_", "paged_decode",
+           "paged_append_", "page_reserve_", "page_trim_"]
 
 
 def _contig(t: torch.Tensor) -> torch.Tensor:
@@ -136,3 +149,61 @@ def append_decode_(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 @append_decode_.register_fake
 def _append_decode_fake(q, k_cache, v_cache, new_k, new_v, past_length, scale):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("kotflash_amd::paged_decode", mutates_args=())
+def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 tables: torch.Tensor, lengths: torch.Tensor, causal: bool,
+                 scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention over the pages (``kotflash_amd.paged.paged_attention`` on the
+    HIP kernels): O and LSE; inference only."""
+    check_attention(q, k_pages, v_pages, tables, lengths)
+    require_readable(q, k_pages, v_pages)
+    return attention_paged(q, k_pages, v_pages, tables, lengths, causal=causal, scale=scale,
+                           with_lse=True)
+
+
+@paged_decode.register_fake
+def _paged_decode_fake(q, k_pages, v_pages, tables, lengths, causal, scale):
+    b, hq, sq, d = q.shape
+    return q.new_empty((b, hq, sq, d)), q.new_empty((b, hq, sq), dtype=torch.float32)
+
+
+@torch.library.custom_op("kotflash_amd::paged_append_", mutates_args=("k_pages", "v_pages"))
+def paged_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, new_k: torch.Tensor,
+                  new_v: torch.Tensor, slots: torch.Tensor) -> None:
+    """new_k/new_v [B, Hkv, S, D] to their slots of the pools."""
+    check_append(k_pages, v_pages, new_k, new_v, slots)
+    append_paged(k_pages, v_pages, new_k, new_v, slots)
+
+
+@paged_append_.register_fake
+def _paged_append_fake(k_pages, v_pages, new_k, new_v, slots):
+    return None
+
+
+@torch.library.custom_op("kotflash_amd::page_reserve_", mutates_args=("tables", "lengths", "counters"))
+def page_reserve_(tables: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Tensor,
+                  counters: torch.Tensor, counts: torch.Tensor, page_size: int,
+                  width: int) -> torch.Tensor:
+    """Pages and slots for counts[b] more tokens of every request
+    (``PageTable.reserve``)."""
+    return reserve_pages(tables, lengths, free_pages, counters, counts, width, page_size)
+
+
+@page_reserve_.register_fake
+def _page_reserve_fake(tables, lengths, free_pages, counters, counts, page_size, width):
+    return tables.new_empty((tables.shape[0], width), dtype=torch.int64)
+
+
+@torch.library.custom_op("kotflash_amd::page_trim_",
+                         mutates_args=("tables", "lengths", "free_pages", "counters"))
+def page_trim_(tables: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Tensor,
+               counters: torch.Tensor, new_lengths: torch.Tensor, page_size: int) -> None:
+    """Back to new_lengths[b] tokens of every request (``PageTable.trim``)."""
+    trim_pages(tables, lengths, free_pages, counters, new_lengths, page_size)
+
+
+@page_trim_.register_fake
+def _page_trim_fake(tables, lengths, free_pages, counters, new_lengths, page_size):
+    return None

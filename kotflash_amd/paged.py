@@ -65,7 +65,8 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots, *, backend: str = "auto"
     """Store new_k/new_v [B, Hkv, S, D] in the pools [pages, Hkv, page_size, D]
     at ``slots`` (int64 [B, S]: page * page_size + row): K and V bit-exact, in
     one launch. Slots outside the pool (-1 in the padding of ``reserve``) are
-    skipped; two tokens of a call must not share a slot."""
+    skipped. Two tokens of a call must not share a slot: what it holds then is
+    either's, or a mixture."""
     # The ordinary GPU call is checked and launched natively; anything else (and
     # every error) takes the checks below. So do the calls further down.
     if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling() \
@@ -73,6 +74,11 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots, *, backend: str = "auto"
         return
     hip_paged.check_append(k_pages, v_pages, new_k, new_v, slots)
     if _store_on_hip(backend, k_pages, half=True):
+        if torch.compiler.is_compiling():
+            from .ops import paged_append_
+
+            paged_append_(k_pages, v_pages, new_k, new_v, slots)
+            return
         hip_paged.append_paged(k_pages, v_pages, new_k, new_v, slots)
         return
     page = k_pages.shape[2]
@@ -107,6 +113,11 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
         if out is not NotImplemented:
             return out
     scale, on_hip = _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backend)
+    if on_hip and torch.compiler.is_compiling():
+        from .ops import paged_decode
+
+        both = paged_decode(q, k_pages, v_pages, tables, lengths, causal, scale)
+        return both if return_lse else both[0]
     if on_hip:
         return hip_paged.attention_paged(q, k_pages, v_pages, tables, lengths, causal=causal,
                                          scale=scale, with_lse=return_lse)
@@ -205,8 +216,19 @@ class PageTable:
         # The lowest page is on top.
         self.free_pages = torch.arange(num_pages - 1, -1, -1, device=device, dtype=torch.int32)
         self.counters = torch.tensor([num_pages, 0, 0, 0], device=device, dtype=torch.int32)
+        self._views()
+
+    def _views(self) -> None:
         self.free_count = self.counters[0:1]
         self.refused = self.counters[1:2]
+
+    # A copy's or a pickle's views are of its own counters.
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k not in ("free_count", "refused")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._views()
 
     def num_free(self) -> int:
         """Free pages (waits for the device)."""
@@ -226,7 +248,7 @@ class PageTable:
         if isinstance(value, bool) or not isinstance(value, int):
             raise TypeError(f"{name} must be an int or a device int32 tensor")
         if not 0 <= value < 2 ** 30:
-            raise ValueError(f"{name} must not be negative")
+            raise ValueError(f"{name} must be in [0, 2**30)")
         return value
 
     def reserve(self, counts: Union[int, torch.Tensor], *, width: Optional[int] = None,

@@ -511,3 +511,122 @@ def test_library_refuses_a_small_workspace():
     _hip.paged_decode(q, k, v, out, None, tables, lengths, scale=0.125, causal=False,
                       workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
     assert_attention(out, q, k, v, tables, lengths, scale=0.125)
+
+
+# --- launch paths ------------------------------------------------------------
+
+def test_python_and_native_paths_agree(monkeypatch):
+    """Without the native module every call runs the same kernels through the
+    Python path; a native call that it does not take changes nothing first."""
+    case = make_case(3, 8, 2, 4, 64, 16, [50, 0, 333], dtype=F16, seed=4, device="cuda")
+    new = torch.randn(2, 3, 2, 4, 64, device="cuda").to(F16)
+    spare = torch.arange(64, 76, device="cuda").reshape(3, 4)
+
+    def run():
+        table = PageTable(3, 400, num_pages=40)
+        slots = [table.reserve(9), table.reserve(_counts([3, 0, 30]), width=30)]
+        table.trim(_counts([4, 10, 25]))
+        table.trim(24)
+        pools = [t.clone() for t in case[1:3]]
+        paged_append(*pools, *new, spare % (case[1].shape[0] * 16))
+        cache = PagedKVCache(table, 2, 64, dtype=F16)
+        cache.k_pages.zero_()
+        cache.v_pages.zero_()
+        step = cache.append_and_attend(case[0], *new, table.reserve(4), causal=True)
+        return [*slots, table.tables, table.lengths, table.free_pages, table.counters, *pools, step,
+                paged_attention(*case, causal=True), *paged_attention(*case, causal=True, return_lse=True),
+                paged_attention(*case, scale=0.3)]
+
+    native = run()
+    monkeypatch.setattr(_hip, "_NATIVE", _hip._NoNative())
+    for i, (a, b) in enumerate(zip(native, run())):
+        assert a.dtype == b.dtype and a.shape == b.shape
+        assert torch.equal(a.nan_to_num(-7.0) if a.is_floating_point() else a,
+                           b.nan_to_num(-7.0) if b.is_floating_point() else b), i
+
+
+def test_inference_tensors():
+    with torch.inference_mode():
+        table = PageTable(2, 64, num_pages=8)
+        cache = PagedKVCache(table, 2, 64, dtype=F16)
+        new = torch.ones(2, 2, 1, 64, device="cuda", dtype=F16)
+        q = torch.ones(2, 4, 1, 64, device="cuda", dtype=F16)
+        out = cache.append_and_attend(q, new, new, table.reserve(1))
+        table.trim(0)
+    assert (out == 1).all() and table.num_free() == 8
+
+
+def test_tables_change_their_version():
+    table = PageTable(2, 64, num_pages=8)
+    before = [t._version for t in (table.tables, table.lengths, table.counters)]
+    table.reserve(1)
+    assert all(t._version > v for t, v in zip((table.tables, table.lengths, table.counters), before))
+
+
+def test_ops_compile_without_graph_breaks():
+    import kotflash_amd.ops  # noqa: F401
+
+    ns = torch.ops.kotflash_amd
+    q, k, v, tables, lengths = make_case(2, 4, 2, 1, 64, 16, [50, 100], dtype=F16, seed=4, device="cuda", junk=0.0)
+    state = [PageTable(2, 256, num_pages=20) for _ in range(2)]
+    new = torch.randn(2, 2, 2, 1, 64, device="cuda").to(F16)
+    counts = _counts([1, 1])
+
+    def step(q, k, v, nk, nv, tables, lengths, free, counters, counts, keep):
+        ns.page_trim_(tables, lengths, free, counters, keep, 16)
+        slots = ns.page_reserve_(tables, lengths, free, counters, counts, 16, 1)
+        ns.paged_append_(k, v, nk, nv, slots)
+        return ns.paged_decode(q, k, v, tables, lengths, False, 0.125)[0] * 2
+
+    results = []
+    for fn, t in zip((step, torch.compile(step, backend="aot_eager", fullgraph=True)), state):
+        pools = [torch.zeros(20, 2, 16, 64, device="cuda", dtype=F16) for _ in range(2)]
+        for r in range(18):
+            out = fn(q, *pools, new[0] + r, new[1] - r, t.tables, t.lengths, t.free_pages, t.counters, counts,
+                     _counts([100, 100]))
+        results.append([out, *pools, t.tables, t.lengths, t.free_pages, t.counters])
+    assert results[0][4].tolist() == [18, 18]
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def test_cache_under_torch_compile():
+    table = PageTable(2, 64, num_pages=8)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=F16)
+    q = torch.randn(2, 4, 1, 64, device="cuda").to(F16)
+    fn = torch.compile(lambda q, n, s: cache.append_and_attend(q, n, n, s), backend="aot_eager")
+    for _ in range(3):
+        out = fn(q, new, table.reserve(1))
+    assert (out == 1).all() and table.lengths.tolist() == [3, 3]
+
+
+def test_calls_on_a_side_stream():
+    """Inputs made on one stream, used on another with an event between."""
+    side = torch.cuda.Stream()
+    table = PageTable(2, 512, num_pages=64)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    big = torch.randn(2, 2, 300, 64, device="cuda").to(F16)
+    q = torch.randn(2, 4, 1, 64, device="cuda").to(F16)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        slots = table.reserve(_counts([300, 200]), width=300)
+        out = cache.append_and_attend(q, big, big, slots)
+    torch.cuda.current_stream().wait_stream(side)
+    ids = torch.arange(2, dtype=torch.int32)[:, None]
+    assert_attention(out, q, big, big, ids, torch.tensor([300, 200], dtype=torch.int32))
+
+
+def test_every_request_its_own_worker_and_none():
+    """Sizes around the number of workers: units one short of it, equal, one
+    more, twice, and with a last worker that has one unit."""
+    for d, per_request in ((64, 1), (128, 1), (128, 4)):
+        for steps in (1023, 1024, 1025, 2047, 2048, 2049, 4100):
+            batch = -(-steps // per_request)
+            lengths = [32 * per_request] * (batch - 1) + [32 * (steps - per_request * (batch - 1))]
+            case = make_case(batch, 2, 1, 1, d, 32, lengths, dtype=F16, seed=steps, device="cuda")
+            o = _attend(*case)[0]
+            pick = torch.tensor([0, 1, batch // 2, batch - 2, batch - 1])
+            few = tuple(t[pick.to(t.device)] if i in (0, 3, 4) else t for i, t in enumerate(case))
+            assert_attention(o[pick.cuda()], *few)
+            assert torch.isfinite(o).all()
