@@ -334,6 +334,28 @@ int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, voi
                     float scale, int causal, int dtype, void* workspace, size_t workspace_bytes,
                     void* stream);
 
+/*
+ * kf_paged_append and kf_paged_decode of one decoding step in the launches of
+ * the latter: the Snew <= KF_PAGED_STEP_TOKENS new rows of each request are
+ * stored at their slots by the workers that read them. The lengths include
+ * the new tokens, and a request's named slots (those inside the pool) are, in
+ * order, those of its last positions, as kf_page_reserve returned them; rows
+ * of a request with fewer positions than named slots may not be stored. The
+ * new rows need a unit head_dim stride, 16-byte aligned bases and strides that
+ * are multiples of 8 elements (int64_t[3]), and the pool fewer than 2^31 slots.
+ */
+#define KF_PAGED_STEP_TOKENS 16
+int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const void* new_k,
+                           const void* new_v, const int64_t* slots, void* o, float* lse,
+                           const int32_t* tables, const int32_t* lengths, int64_t B, int64_t Hq,
+                           int64_t Hkv, int64_t Sq, int64_t Snew, int64_t D, int64_t num_pages,
+                           int64_t page_size, int64_t columns, int64_t table_stride,
+                           int64_t slots_stride, const int64_t* q_strides,
+                           const int64_t* k_strides, const int64_t* v_strides,
+                           const int64_t* new_k_strides, const int64_t* new_v_strides,
+                           const int64_t* o_strides, float scale, int causal, int dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

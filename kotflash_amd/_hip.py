@@ -22,6 +22,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libkotflash_amd.so"
 ABI_VERSION = 7
 KF_F16, KF_BF16 = 0, 1
+KF_PAGED_STEP_TOKENS = 16
 KF_BWD_DELTA, KF_BWD_DQ, KF_BWD_DKDV, KF_BWD_DKDV_FIXUP = 1, 2, 4, 8
 KF_BWD_ALL = KF_BWD_DELTA | KF_BWD_DQ | KF_BWD_DKDV | KF_BWD_DKDV_FIXUP
 
@@ -66,6 +67,8 @@ _SIGNATURES = {
     "kf_paged_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
     "kf_paged_decode": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                              _I64, _I64, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _SZ, _P]),
+    "kf_paged_append_decode": (_I, [_P] * 10 + [_I64] * 11 + [_I64P] * 6
+                               + [_F, _I, _I, _P, _SZ, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -468,3 +471,20 @@ def paged_decode(q, k_pages, v_pages, out, lse: Optional[torch.Tensor], tables, 
             _stream(q.device),
         )
     _check(rc, "kf_paged_decode")
+
+
+def paged_append_decode(q, k_pages, v_pages, new_k, new_v, slots, out, lse: Optional[torch.Tensor],
+                        tables, lengths, *, scale: float, causal: bool, workspace: torch.Tensor) -> None:
+    b, hq, sq, d = q.shape
+    num_pages, hkv, page_size, _ = k_pages.shape
+    with _DeviceGuard(q.device):
+        rc = lib().kf_paged_append_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), new_k.data_ptr(), new_v.data_ptr(),
+            slots.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+            tables.data_ptr(), lengths.data_ptr(), b, hq, hkv, sq, new_k.shape[2], d, num_pages,
+            page_size, tables.shape[1], tables.stride(0), slots.stride(0), _strides(q),
+            _strides(k_pages), _strides(v_pages), _strides(new_k), _strides(new_v), _strides(out),
+            float(scale), int(bool(causal)), dtype_code(q.dtype), workspace.data_ptr(),
+            workspace.nbytes, _stream(q.device),
+        )
+    _check(rc, "kf_paged_append_decode")

@@ -515,45 +515,6 @@ struct PagedArgs {
   }
 };
 
-Tensor launch_paged(const PagedArgs& a, Tensor* lse) {
-  const Tensor q = readable(*a.q);
-  const Tensor &k = *a.k, &v = *a.v;
-  const int64_t b = q.size(0), hq = q.size(1), sq = q.size(2), d = q.size(3), hkv = k.size(1);
-  Tensor out = at::empty({b, hq, sq, d}, q.options());
-  if (lse) *lse = at::empty({b, hq, sq}, q.options().dtype(at::kFloat));
-  Tensor ws = bytes_like(q, kf_paged_decode_workspace_bytes(b, hq, hkv, sq, d));
-  check(kf_paged_decode(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(),
-                        lse ? lse->data_ptr<float>() : nullptr, a.tables->const_data_ptr<int32_t>(),
-                        a.lengths->const_data_ptr<int32_t>(), b, hq, hkv, sq, d, k.size(0), k.size(2),
-                        a.tables->size(1), a.tables->stride(0), q.strides().data(), k.strides().data(),
-                        v.strides().data(), out.strides().data(), (float)a.scale, a.causal, dtype_code(q),
-                        ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
-        "kf_paged_decode");
-  return out;
-}
-
-// paged_attention(q, k_pages, v_pages, tables, lengths, causal, scale or None,
-// return_lse).
-PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  PagedArgs a;
-  bool with_lse;
-  if (n != 8 || !exact_bool(args[7], with_lse) || !a.read(args)) return not_handled();
-  Tensor out, lse;
-  {
-    pybind11::gil_scoped_release nogil;
-    const c10::OptionalDeviceGuard guard(a.q->device());
-    out = launch_paged(a, with_lse ? &lse : nullptr);
-  }
-  if (!with_lse) return THPVariable_Wrap(std::move(out));
-  PyObject* pair = PyTuple_New(2);
-  if (pair == nullptr) throw python_error();
-  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
-  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
-  return pair;
-  END_HANDLE_TH_ERRORS
-}
-
 struct StoreArgs {
   const Tensor *k, *v, *nk, *nv, *slots;
   // Arguments from `a`: k_pages, v_pages, new_k, new_v, slots.
@@ -582,6 +543,59 @@ void launch_store(const StoreArgs& a) {
         "kf_paged_append");
 }
 
+// The attention, with the store of `fresh` in its launches if there is one.
+Tensor launch_paged(const PagedArgs& a, Tensor* lse, const StoreArgs* fresh) {
+  const Tensor q = readable(*a.q);
+  const Tensor &k = *a.k, &v = *a.v;
+  const int64_t b = q.size(0), hq = q.size(1), sq = q.size(2), d = q.size(3), hkv = k.size(1);
+  Tensor out = at::empty({b, hq, sq, d}, q.options());
+  if (lse) *lse = at::empty({b, hq, sq}, q.options().dtype(at::kFloat));
+  Tensor ws = bytes_like(q, kf_paged_decode_workspace_bytes(b, hq, hkv, sq, d));
+  if (fresh) {
+    const Tensor nk = readable(*fresh->nk), nv = readable(*fresh->nv);
+    check(kf_paged_append_decode(
+              q.const_data_ptr(), k.data_ptr(), v.data_ptr(), nk.const_data_ptr(), nv.const_data_ptr(),
+              fresh->slots->const_data_ptr<int64_t>(), out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
+              a.tables->const_data_ptr<int32_t>(), a.lengths->const_data_ptr<int32_t>(), b, hq, hkv, sq,
+              nk.size(2), d, k.size(0), k.size(2), a.tables->size(1), a.tables->stride(0),
+              fresh->slots->stride(0), q.strides().data(), k.strides().data(), v.strides().data(),
+              nk.strides().data(), nv.strides().data(), out.strides().data(), (float)a.scale, a.causal,
+              dtype_code(q), ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
+          "kf_paged_append_decode");
+    return out;
+  }
+  check(kf_paged_decode(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), out.data_ptr(),
+                        lse ? lse->data_ptr<float>() : nullptr, a.tables->const_data_ptr<int32_t>(),
+                        a.lengths->const_data_ptr<int32_t>(), b, hq, hkv, sq, d, k.size(0), k.size(2),
+                        a.tables->size(1), a.tables->stride(0), q.strides().data(), k.strides().data(),
+                        v.strides().data(), out.strides().data(), (float)a.scale, a.causal, dtype_code(q),
+                        ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
+        "kf_paged_decode");
+  return out;
+}
+
+// paged_attention(q, k_pages, v_pages, tables, lengths, causal, scale or None,
+// return_lse).
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  PagedArgs a;
+  bool with_lse;
+  if (n != 8 || !exact_bool(args[7], with_lse) || !a.read(args)) return not_handled();
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.q->device());
+    out = launch_paged(a, with_lse ? &lse : nullptr, nullptr);
+  }
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) throw python_error();
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
 // paged_append(k_pages, v_pages, new_k, new_v, slots).
 PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -597,20 +611,25 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // paged_step(q, k_pages, v_pages, tables, lengths, causal, None, new_k, new_v,
-// slots): the store, then the attention.
+// slots, fuse): the store, then the attention; in the attention's launches
+// with `fuse`, for rows that these take.
 PyObject* py_paged_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   PagedArgs a;
   StoreArgs st;
-  if (n != 10 || !a.read(args)) return not_handled();
+  bool fuse;
+  if (n != 11 || !exact_bool(args[10], fuse) || !a.read(args)) return not_handled();
   PyObject* const store[] = {args[1], args[2], args[7], args[8], args[9]};
   if (!st.read(store)) return not_handled();
+  if (fuse && (st.nk->size(0) != a.q->size(0) || st.nk->size(2) > KF_PAGED_STEP_TOKENS ||
+               st.k->size(0) * st.k->size(2) >= (1ll << 31)))
+    return not_handled();
   Tensor out;
   {
     pybind11::gil_scoped_release nogil;
     const c10::OptionalDeviceGuard guard(a.q->device());
-    launch_store(st);
-    out = launch_paged(a, nullptr);
+    if (!fuse) launch_store(st);
+    out = launch_paged(a, nullptr, fuse ? &st : nullptr);
   }
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

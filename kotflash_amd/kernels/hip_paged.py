@@ -101,12 +101,7 @@ def attention_paged(q, k_pages, v_pages, tables, lengths, *, causal: bool, scale
                     with_lse: bool = False):
     """O (and LSE) of q over the pages (``kf_paged_decode``); the arguments
     have passed ``check_attention`` and ``require_readable``."""
-    if not _hip.layout_ok(q):
-        q = q.contiguous()
-    if tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < 0):
-        tables = tables.contiguous()
-    if not lengths.is_contiguous():
-        lengths = lengths.contiguous()
+    q, tables, lengths = _dense(q, tables, lengths)
     b, hq, sq, d = q.shape
     out = torch.empty((b, hq, sq, d), device=q.device, dtype=q.dtype)
     lse = torch.empty((b, hq, sq), device=q.device, dtype=torch.float32) if with_lse else None
@@ -114,6 +109,38 @@ def attention_paged(q, k_pages, v_pages, tables, lengths, *, causal: bool, scale
     _hip.paged_decode(q, k_pages, v_pages, out, lse, tables, lengths, scale=scale, causal=causal,
                       workspace=ws)
     return (out, lse) if with_lse else out
+
+
+def _dense(q, tables, lengths):
+    if not _hip.layout_ok(q):
+        q = q.contiguous()
+    if tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < 0):
+        tables = tables.contiguous()
+    return q, tables, lengths if lengths.is_contiguous() else lengths.contiguous()
+
+
+def step_fuses(k_pages, new_k) -> bool:
+    """Whether the attention's launches also store these new rows."""
+    return (new_k.shape[2] <= _hip.KF_PAGED_STEP_TOKENS
+            and k_pages.shape[0] * k_pages.shape[2] < 2 ** 31)
+
+
+def append_attention_paged(q, k_pages, v_pages, new_k, new_v, slots, tables, lengths, *,
+                           causal: bool, scale: float):
+    """O of q over the pages after the store of new_k/new_v at ``slots``, in
+    the attention's launches (``kf_paged_append_decode``); the arguments have
+    passed ``check_attention``, ``require_readable``, ``check_append`` and
+    ``step_fuses``."""
+    q, tables, lengths = _dense(q, tables, lengths)
+    new_k, new_v = (t if _hip.layout_ok(t) else t.contiguous() for t in (new_k, new_v))
+    if slots.stride(1) != 1:
+        slots = slots.contiguous()
+    b, hq, sq, d = q.shape
+    out = torch.empty((b, hq, sq, d), device=q.device, dtype=q.dtype)
+    ws = _hip.workspace(q.device, _hip.paged_decode_workspace_bytes(b, hq, k_pages.shape[1], sq, d))
+    _hip.paged_append_decode(q, k_pages, v_pages, new_k, new_v, slots, out, None, tables, lengths,
+                             scale=scale, causal=causal, workspace=ws)
+    return out
 
 
 def append_paged(k_pages, v_pages, new_k, new_v, slots) -> None:

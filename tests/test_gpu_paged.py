@@ -630,3 +630,97 @@ def test_every_request_its_own_worker_and_none():
             few = tuple(t[pick.to(t.device)] if i in (0, 3, 4) else t for i, t in enumerate(case))
             assert_attention(o[pick.cuda()], *few)
             assert torch.isfinite(o).all()
+
+
+# --- the step that stores and attends in one launch --------------------------
+
+@pytest.mark.parametrize("n", [1, 2, 4, 5, 16])
+@pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 64, 16), (4, 4, 128, 32), (16, 2, 72, 48), (32, 1, 96, 16), (80, 1, 40, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_fused_step_matches_two_launches(n, hq, hkv, d, page, dtype):
+    """Requests whose new tokens end or begin a page or a step, cross them, or
+    are their first; with fewer new tokens than slots, and none."""
+    before = [0, 0, 1, 15, 16, 31, 32, 33, page - 1, page, 2 * page - 2, 200, 1000, 64 - n, 7]
+    counts = [n, 0, n, n, 1, n, n, n, n, n, n, max(1, n - 1), n, n, n // 2]
+    g = torch.Generator(device="cuda").manual_seed(n + d)
+    results = []
+    b = len(before)
+    q = torch.randn(b, hq, n, d, device="cuda", generator=g).to(dtype)
+    new = torch.randn(2, b, n, hkv, d, device="cuda", generator=g).to(dtype).transpose(2, 3)
+    old = torch.randn(2, b, hkv, max(before), d, device="cuda", generator=g).to(dtype)
+    for how in ("fused", "hip", "auto"):
+        table = PageTable(b, 1100, num_pages=400, page_size=page)
+        cache = PagedKVCache(table, hkv, d, dtype=dtype)
+        cache.k_pages.fill_(math.nan)
+        cache.v_pages.fill_(math.nan)
+        cache.append(*old, table.reserve(_counts(before), width=max(before)))
+        slots = table.reserve(_counts(counts), width=n)
+        out = cache.append_and_attend(q, *new, slots, causal=True, append_backend=how)
+        results.append((out, cache.k_pages, cache.v_pages))
+    for other in results[1:]:
+        for a, b_ in zip(results[0], other):
+            assert torch.equal(a.view(torch.int16), b_.view(torch.int16))
+    lens = [x + c for x, c in zip(before, counts)]
+    whole = [torch.cat((old[i], torch.zeros_like(new[i])), 2) for i in range(2)]
+    for i in range(2):
+        for r, (x, c) in enumerate(zip(before, counts)):
+            whole[i][r, :, x:x + c] = new[i][r, :, :c]
+    ids = torch.arange(b, dtype=torch.int32)[:, None]
+    pick = [0, 1, 2, 5, 8, 11, 13, 14]
+    assert_attention(results[0][0][pick], q[pick], *whole, ids[pick], torch.tensor(lens, dtype=torch.int32)[pick],
+                     causal=True)
+
+
+def test_fused_step_leaves_other_slots():
+    """Slots outside the pool, and holes between named ones, store nothing."""
+    table = PageTable(2, 64, num_pages=8)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.zero_()
+    cache.v_pages.zero_()
+    slots = table.reserve(_counts([3, 0]), width=5)
+    holes = torch.full_like(slots, -1)
+    holes[0, 0], holes[0, 2], holes[0, 4] = slots[0, 0], slots[0, 1], slots[0, 2]
+    holes[0, 1], holes[0, 3], holes[1, 0] = 8 * 16, 2 ** 40, -2 ** 62
+    new = torch.randn(2, 2, 2, 5, 64, device="cuda").to(F16)
+    q = torch.randn(2, 4, 1, 64, device="cuda").to(F16)
+    out = cache.append_and_attend(q, *new, holes, append_backend="fused")
+    page = int(table.tables[0, 0])
+    for pool, x in ((cache.k_pages, new[0]), (cache.v_pages, new[1])):
+        assert torch.equal(pool[page, :, :3], x[0][:, [0, 2, 4]])
+        assert int((pool != 0).sum()) <= 2 * 3 * 64
+    assert (out[1] == 0).all()
+    assert_attention(out[:1], q[:1], new[0][:1][:, :, [0, 2, 4]].contiguous(), new[1][:1][:, :, [0, 2, 4]].contiguous(),
+                     torch.zeros(1, 1, dtype=torch.int32), torch.tensor([3], dtype=torch.int32))
+
+
+def test_fused_step_refusals():
+    table = PageTable(2, 64, num_pages=8)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.zero_()
+    slots = table.reserve(17)
+    new = torch.ones(2, 2, 17, 64, device="cuda", dtype=F16)
+    q = torch.ones(2, 4, 1, 64, device="cuda", dtype=F16)
+    with pytest.raises(ValueError, match="up to 16 new tokens"):
+        cache.append_and_attend(q, new, new, slots, append_backend="fused")
+    with pytest.raises(ValueError, match="HIP attention"):
+        cache.append_and_attend(q, new[:, :, :1], new[:, :, :1], slots[:, :1], append_backend="fused",
+                                attention_backend="sdpa")
+    with pytest.raises(ValueError, match="slots"):
+        cache.append_and_attend(q, new[:1, :, :1], new[:1, :, :1], slots[:, :1])
+    assert (cache.k_pages == 0).all()
+    assert (cache.append_and_attend(q, new, new, slots) == 1).all()
+
+
+def test_fused_step_python_path(monkeypatch):
+    monkeypatch.setattr(_hip, "_NATIVE", _hip._NoNative())
+    table = PageTable(2, 64, num_pages=8)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    new = torch.randn(2, 2, 2, 3, 64, device="cuda").to(F16)
+    q = torch.randn(2, 4, 3, 64, device="cuda").to(F16)
+    calls = []
+    real = _hip.paged_append_decode
+    monkeypatch.setattr(_hip, "paged_append_decode", lambda *a, **k: (calls.append(1), real(*a, **k)))
+    out = cache.append_and_attend(q, *new.transpose(3, 4).contiguous().transpose(3, 4), table.reserve(3), causal=True)
+    assert calls == [1]
+    ids = torch.arange(2, dtype=torch.int32)[:, None]
+    assert_attention(out, q, *new, ids, torch.tensor([3, 3], dtype=torch.int32), causal=True)

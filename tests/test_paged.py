@@ -266,3 +266,13 @@ def test_oracle_bound_is_not_loose():
     o, _, tol, _ = attention64(*args)
     short = attention64(*args[:4], torch.tensor([99], dtype=torch.int32))[0]
     assert bool(((short - o).abs() > tol).any())
+
+
+def test_fused_needs_the_kernels():
+    table = _table()
+    cache = PagedKVCache(table, 2, 8, dtype=F32)
+    cache.k_pages.zero_()
+    new = torch.ones(3, 2, 1, 8)
+    with pytest.raises(ValueError, match="fused"):
+        cache.append_and_attend(torch.ones(3, 4, 1, 8), new, new, table.reserve(1), append_backend="fused")
+    assert (cache.k_pages == 0).all()

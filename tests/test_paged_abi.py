@@ -90,3 +90,17 @@ def test_workspace_size():
     for b, hq, hkv, sq, d in ((1, 1, 1, 1, 8), (64, 32, 8, 1, 128), (8, 64, 1, 3, 64)):
         rows = min(64, hq // hkv * sq)
         assert size(b, hq, hkv, sq, d) >= (256 + b * hkv) * rows * (d + 1) * 4
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(nk=None), "new_k is null"), (dict(nk=P + 2), "new_k must be 16-byte"), (dict(ns=_arr(64, 64, 3)), "strides"),
+    (dict(slots=None), "slots"), (dict(n=0), "1 to 16"), (dict(n=17), "1 to 16"), (dict(pages=2 ** 27), "2^31 slots"),
+    (dict(page=8), "multiple of 16"), (dict(B=0), "positive"),
+])
+def test_append_decode(kw, match):
+    a = dict(nk=P, ns=_arr(128, 64, 64), slots=P, n=1, B=2, pages=8, page=16)
+    a.update(kw)
+    s = _arr(2048, 1024, 64)
+    _expect(_hip.lib().kf_paged_append_decode(P, P, P, a["nk"], P, a["slots"], P, None, P, P, a["B"], 4, 2, 1, a["n"],
+                                              64, a["pages"], a["page"], 4, 4, 1, s, s, s, a["ns"], a["ns"], s, 0.1,
+                                              0, 0, P, 1 << 40, None), match)
