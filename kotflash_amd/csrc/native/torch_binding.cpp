@@ -524,7 +524,8 @@ struct StoreArgs {
     if (!k || !v || !nk || !nv || !slots || !plain_mode() || !pools_ok(*k, *v)) return false;
     if (nk->dim() != 4 || nk->sizes() != nv->sizes() || nk->numel() == 0 || nk->size(1) != k->size(1) ||
         nk->size(3) != k->size(3) || nk->scalar_type() != k->scalar_type() ||
-        nv->scalar_type() != k->scalar_type() || nk->device() != k->device() || nv->device() != k->device())
+        nv->scalar_type() != k->scalar_type() || nk->device() != k->device() || nv->device() != k->device() ||
+        wants_grad({k, v, nk, nv}))
       return false;
     for (const Tensor* t : {k, v})
       for (int i = 0; i < 4; ++i)

@@ -154,6 +154,16 @@ struct Unit {
   int b, hh, rem, begin;
 };
 
+// Whether any of eight elements is infinite or NaN (all exponent bits set).
+template <typename T>
+__device__ inline bool any_nonfinite(u32x4 x) {
+  constexpr uint32_t kExp = std::is_same_v<T, _Float16> ? 0x7c00u : 0x7f80u;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bad |= (x[j] & kExp) == kExp || (x[j] >> 16 & kExp) == kExp;
+  return bad;
+}
+
 template <typename T> struct PBias;  // P = 2^(s - m + bias), see paged_kernel
 template <> struct PBias<_Float16> { static constexpr float v = 7.f; };
 template <> struct PBias<__bf16> { static constexpr float v = 0.f; };
@@ -522,14 +532,56 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     }
     // V^T A operands by transposed reads: lane (g, i) receives V[key][16 db + i]
     // for the keys of slot t above.
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) {
+    auto v_operand = [&](int db) -> u32x4 {
       const int col = 16 * db + 4 * (l16 & 3);
       const u32x2 lo = lds_read_tr16(Vs + Tile::elem(4 * g16 + (l16 >> 2), col));
       const u32x2 hi = lds_read_tr16(Vs + Tile::elem(16 + 4 * g16 + (l16 >> 2), col));
-      const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+      return {lo[0], lo[1], hi[0], hi[1]};
+    };
+    // Where the rows' limits differ within the step, a key that one row sees and
+    // another does not may hold a V that is not finite: 0 V would reach both.
+    bool apart = false;
+    if (most_lag > 0 && w.rem - most_lag < kStep) {
+      bool bad = false;
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
+      for (int db = 0; db < NDB; ++db) bad |= any_nonfinite<T>(v_operand(db));
+      apart = wave_any(bad);
+    }
+    if (!apart) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const u32x4 a = v_operand(db);
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
+      }
+      return;
+    }
+    // Then the rows of each limit on their own, V behind it as zeros.
+#pragma unroll 1
+    for (int limit = 1; limit <= kStep; ++limit) {
+      bool mine[QB], any = false;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        mine[qb] = min(w.rem - row[qb].lag, kStep) == limit;
+        any |= mine[qb];
+      }
+      if (!wave_any(any)) continue;
+      u32x4 keep;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = (j < 2 ? 0 : 16) + 4 * g16 + 2 * (j & 1);
+        keep[j] = (key < limit ? 0xffffu : 0u) | (key + 1 < limit ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const u32x4 a = v_operand(db) & keep;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const f32x4 sum = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) oacc[qb][db][r] = mine[qb] ? sum[r] : oacc[qb][db][r];
+        }
+      }
     }
   };
 

@@ -46,6 +46,11 @@ def _on_gfx950(t: torch.Tensor) -> bool:
     return t.is_cuda and _hip.is_gfx950(t.device)
 
 
+def _no_gradients(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference-only; disable gradients")
+
+
 def _store_on_hip(backend: str, t: torch.Tensor, half: bool) -> bool:
     if backend not in STORE_BACKENDS:
         raise ValueError("append backend must be one of: auto, hip, cuda or torch")
@@ -65,14 +70,15 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots, *, backend: str = "auto"
     """Store new_k/new_v [B, Hkv, S, D] in the pools [pages, Hkv, page_size, D]
     at ``slots`` (int64 [B, S]: page * page_size + row): K and V bit-exact, in
     one launch. Slots outside the pool (-1 in the padding of ``reserve``) are
-    skipped. Two tokens of a call must not share a slot: what it holds then is
-    either's, or a mixture."""
+    skipped. Two tokens of a call must not share a slot (what it holds then is
+    either's, or a mixture), and new_k/new_v must not lie in the pools."""
     # The ordinary GPU call is checked and launched natively; anything else (and
     # every error) takes the checks below. So do the calls further down.
     if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling() \
             and _hip.native().paged_append(k_pages, v_pages, new_k, new_v, slots) is None:
         return
     hip_paged.check_append(k_pages, v_pages, new_k, new_v, slots)
+    _no_gradients("paged append", k_pages, v_pages, new_k, new_v)
     if _store_on_hip(backend, k_pages, half=True):
         if torch.compiler.is_compiling():
             from .ops import paged_append_
@@ -141,8 +147,7 @@ def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backen
             raise ValueError("scale must be finite")
     if backend not in PAGED_BACKENDS:
         raise ValueError("backend must be one of: auto, hip, triton, sdpa")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_pages, v_pages)):
-        raise RuntimeError("paged attention is inference-only; disable gradients")
+    _no_gradients("paged attention", q, k_pages, v_pages)
     if backend == "sdpa":
         return scale, False
     if backend == "auto":
@@ -393,6 +398,7 @@ class PagedKVCache:
                                          self.table.lengths, causal, None, attention_backend)
         if fuse and on_hip and not torch.compiler.is_compiling():
             hip_paged.check_append(self.k_pages, self.v_pages, new_k, new_v, slots)
+            _no_gradients("paged append", new_k, new_v)
             if slots.shape[0] == q.shape[0] and hip_paged.step_fuses(self.k_pages, new_k):
                 return hip_paged.append_attention_paged(
                     q, self.k_pages, self.v_pages, new_k, new_v, slots, self.table.tables,

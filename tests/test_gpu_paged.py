@@ -724,3 +724,48 @@ def test_fused_step_python_path(monkeypatch):
     assert calls == [1]
     ids = torch.arange(2, dtype=torch.int32)[:, None]
     assert_attention(out, q, *new, ids, torch.tensor([3, 3], dtype=torch.int32), causal=True)
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv", [(F16, 64, 8, 2), (BF16, 128, 4, 1), (BF16, 96, 24, 1), (F16, 32, 48, 1),
+                                            (F16, 128, 16, 1)])
+@pytest.mark.parametrize("length", [4, 33, 37, 66, 259])
+def test_what_a_row_does_not_see_yet(dtype, d, hq, hkv, length):
+    """K and V of later draft tokens that are NaN or infinite do not reach the
+    rows in front of them; they do reach those that see them."""
+    sq = 4
+    for seed, value in enumerate((math.nan, math.inf, -math.inf)):
+        q, k, v, tables, lengths = make_case(3, hq, hkv, sq, d, 16, [length, 500, length], dtype=dtype, seed=seed,
+                                             device="cuda")
+        clean = _attend(q, k, v, tables, lengths, causal=True)
+        at = length - 2  # seen by the last two rows only
+        page, row = int(tables[0, at // 16]), at % 16
+        bad_k, bad_v = k.clone(), v.clone()
+        bad_v[page, :, row, 3] = value
+        o, lse = _attend(q, k, bad_v, tables, lengths, causal=True)
+        assert torch.equal(lse, clean[1])
+        tol = 2 * torch.finfo(dtype).eps * clean[0].abs() + 2.0 ** -20  # rows summed apart: the order differs
+        assert bool(((o - clean[0]).abs() <= tol)[:, :, :2].all()) and torch.equal(o[1:], clean[0][1:])
+        assert not torch.isfinite(o[0, :, 2:, 3]).any()
+        rest = [i for i in range(d) if i != 3]
+        assert bool(((o - clean[0]).abs() <= tol)[0][..., rest].all())
+        bad_k[page, :, row, 3] = value
+        o, lse = _attend(q, bad_k, v, tables, lengths, causal=True)
+        assert torch.equal(o[:, :, :2], clean[0][:, :, :2]) and torch.equal(lse[:, :, :2], clean[1][:, :, :2])
+        if math.isnan(value):
+            assert torch.isnan(o[0, :, 2:]).all()
+
+
+def test_gradients_are_refused():
+    q, k, v, tables, lengths = make_case(2, 4, 2, 1, 64, 16, [30, 50], dtype=F16, seed=4, device="cuda", junk=0.0)
+    table = PageTable(2, 64, num_pages=k.shape[0])
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.zero_()
+    slots = table.reserve(1)
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=F16, requires_grad=True)
+    for call in (lambda: cache.append(new, new, slots), lambda: cache.append_and_attend(q, new, new, slots)):
+        with pytest.raises(RuntimeError, match="inference-only"):
+            call()
+        assert (cache.k_pages == 0).all()
+    with torch.no_grad():
+        cache.append_and_attend(q, new, new, slots)
+    assert (cache.k_pages != 0).any()
