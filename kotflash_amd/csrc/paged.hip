@@ -168,27 +168,44 @@ template <typename T> struct PBias;  // P = 2^(s - m + bias), see paged_kernel
 template <> struct PBias<_Float16> { static constexpr float v = 7.f; };
 template <> struct PBias<__bf16> { static constexpr float v = 0.f; };
 
-// 1 KB loads of a row group's Q tile.
-constexpr int q_loads(int DT, int QB) { return 16 * QB * (DT / 8) / 64; }
-// LDS of a worker: two steps of K and V, and the Q tiles of two segments.
-constexpr int worker_lds(int DT, int QB) { return 2 * (2 * kStep * DT * 2 + q_loads(DT, QB) * 1024); }
+// 1 KB loads of the Q tile of 16 rows.
+constexpr int q_loads(int DT) { return 16 * (DT / 8) / 64; }
+// LDS of a worker: two steps of K and V, and every wave's Q tiles of two
+// segments.
+constexpr int worker_lds(int DT, int NW) { return 2 * (2 * kStep * DT * 2 + NW * q_loads(DT) * 1024); }
+// Workers that a CU holds: by its 160 KB of LDS, given out in pieces of 1280
+// bytes, and by the registers of two (NW = 1) or three waves per SIMD.
+constexpr int workers_per_cu(int DT, int NW) {
+  const int by_lds = 160 * 1024 / ((worker_lds(DT, NW) + 1279) / 1280 * 1280);
+  const int by_waves = NW == 1 ? 8 : 12 / NW;
+  return by_lds < by_waves ? by_lds : by_waves;
+}
 
-template <typename T, int DT, int QB>
-__global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
+// All waves of a worker are here, and what they have written or read in LDS is
+// behind them. (Each waits for its own loads and reads before.)
+template <int NW>
+__device__ inline void worker_barrier() {
+  if constexpr (NW > 1) asm volatile("s_barrier" ::: "memory");
+}
+
+// NW waves per worker, 16 packed rows each: they share the ring, every wave
+// loading a part of each step, and read all of it.
+template <typename T, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) void paged_kernel(const PagedParams p) {
   constexpr int CPR = DT / 8;         // 16-byte chunks per row
   constexpr int NDC = DT / 32;        // 32-wide head-dim chunks (S contraction)
   constexpr int NDB = DT / 16;        // 16-wide head-dim blocks of O^T
   constexpr int VT = kStep * DT;      // elements of one K (or V) step tile
   constexpr int NGI = 16 * CPR / 64;  // 1 KB loads per 16-row group of K (or V)
-  constexpr int NL = 4 * NGI;         // loads per step: two groups of K and of V
-  constexpr int NQ = q_loads(DT, QB);
+  constexpr int NL = 4 * NGI / NW;    // a wave's loads per step: of two groups of K and of V
+  constexpr int NQ = q_loads(DT);
   using Tile = SwizzledTile<CPR>;
-  static_assert(NL + NQ < 64, "the counter of outstanding loads has six bits");
-  // Per ring slot: a step's K and V tiles, and the Q tile of the segment that
-  // begins with it.
-  __shared__ __attribute__((aligned(16))) uint16_t smem[worker_lds(DT, QB) / 2];
+  static_assert(NW == 1 || NW == 2 || NW == 4);
+  // Two ring slots of a step's K and V tiles; per slot and wave, the Q tile of
+  // the segment that begins with it.
+  __shared__ __attribute__((aligned(16))) uint16_t smem[worker_lds(DT, NW) / 2];
 
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = NW > 1 ? wave_index() : 0;
   const int l16 = lane & 15, g16 = lane >> 4;
   const const_i32 lengths = (const_i32)(uintptr_t)p.lengths;
 
@@ -219,12 +236,12 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     asm volatile("" : "+s"(ptr));
     return *ptr;
   };
-  // And of the Q tile's loads and the outputs, for the first row group of a
+  // And of the wave's Q loads and its lane's row, for the first row group of a
   // KV head (of most, the only one).
   auto query_offset = [&](const auto& c, int k, int rb) -> uint32_t {
     const int pc = k * 64 + lane;
-    const int r = pc / CPR;
-    const int ch = (pc % CPR) ^ Tile::key(r);
+    const int r = wave * 16 + pc / CPR;
+    const int ch = (pc % CPR) ^ Tile::key(pc / CPR);
     const int rho = rb * c.rows + r;
     const int g = rho / c.Sq, i = rho - g * c.Sq;
     const bool ok = r < c.rows && rho < c.G * c.Sq && ch * 8 < c.D;
@@ -234,22 +251,16 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     uint32_t out;  // byte offset of the row within its KV head's outputs, kOOB if there is none
     int lag;       // keys that it sees fewer than the last query token does
   };
-  auto output_row = [&](const auto& c, int qb, int rb) -> Row {
-    const int r = qb * 16 + l16, rho = rb * c.rows + r;
+  auto output_row = [&](const auto& c, int rb) -> Row {
+    const int r = wave * 16 + l16, rho = rb * c.rows + r;
     const int g = rho / c.Sq, i = rho - g * c.Sq;
     return {r < c.rows && rho < c.G * c.Sq ? (uint32_t)(g * c.o_sh + i * c.o_ss) * 2u : kOOB,
             c.causal ? c.Sq - 1 - i : 0};
   };
-  // (One row block only: more have no registers to spare, and more to do per
-  // segment anyway.)
-  constexpr bool KEEP = QB == 1;
-  uint32_t qoff[KEEP ? NQ : 1];
-  Row row0[KEEP ? QB : 1];
-  if constexpr (KEEP) {
+  uint32_t qoff[NQ];
 #pragma unroll
-    for (int k = 0; k < NQ; ++k) qoff[k] = query_offset(p, k, 0);
-    row0[0] = output_row(p, 0, 0);
-  }
+  for (int k = 0; k < NQ; ++k) qoff[k] = query_offset(p, k, 0);
+  const Row row0 = output_row(p, 0);
 
   // This worker's run of units, and where it begins: request b, whose first
   // unit is `start`.
@@ -396,9 +407,9 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       const int kvh = at.hh / c.nrb;
       const int rb = at.hh - kvh * c.nrb;
       const auto qr = make_rsrc(c.q + at.b * c.q_sb + (int64_t)kvh * c.G * c.q_sh, c.q_bytes);
-      const uint32_t q0 = lds0 + 4 * VT * 2 + slot * NQ * 1024u;
-      if (KEEP && rb == 0) {
-        if constexpr (KEEP) dma_tile<NQ, false>(qr, q0, qoff);
+      const uint32_t q0 = lds0 + 4 * VT * 2 + (slot * NW + wave) * NQ * 1024u;
+      if (rb == 0) {
+        dma_tile<NQ, false>(qr, q0, qoff);
       } else {
         uint32_t off[NQ];
 #pragma unroll
@@ -413,19 +424,22 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       const int row = g == 0 ? part * 16 : row1;
       int rows = at.rem - 16 * g;
       rows = rows < 0 || id >= (uint32_t)p.pages ? 0 : rows < 16 ? rows : 16;
-      const uint64_t ka = kh + (rows ? (uint64_t)id * p.k_page + (uint32_t)row * (uint64_t)p.k_row : 0);
-      const uint64_t va = vh + (rows ? (uint64_t)id * p.v_page + (uint32_t)row * (uint64_t)p.v_row : 0);
-      // The extent ends with the last visible row.
-      const auto kr = make_rsrc((const void*)(uintptr_t)ka, rows ? (rows - 1) * p.k_row + 2 * p.D : 0);
-      const auto vr = make_rsrc((const void*)(uintptr_t)va, rows ? (rows - 1) * p.v_row + 2 * p.D : 0);
-      if (stream) {
-        dma_tile<NGI, true>(kr, m0, koff);
-        dma_tile<NGI, true>(vr, m0 + VT * 2, voff);
-      } else {
-        dma_tile<NGI, false>(kr, m0, koff);
-        dma_tile<NGI, false>(vr, m0 + VT * 2, voff);
-      }
       seen[slot][g] = rows;
+      // One wave loads both groups; of two, each a group; of four, K or V of one.
+      if (NW > 1 && (wave & 1) != g) continue;
+      // The extent ends with the last visible row.
+      if (NW < 4 || wave < 2) {
+        const uint64_t ka = kh + (rows ? (uint64_t)id * p.k_page + (uint32_t)row * (uint64_t)p.k_row : 0);
+        const auto kr = make_rsrc((const void*)(uintptr_t)ka, rows ? (rows - 1) * p.k_row + 2 * p.D : 0);
+        if (stream) dma_tile<NGI, true>(kr, m0, koff);
+        else dma_tile<NGI, false>(kr, m0, koff);
+      }
+      if (NW < 4 || wave >= 2) {
+        const uint64_t va = vh + (rows ? (uint64_t)id * p.v_page + (uint32_t)row * (uint64_t)p.v_row : 0);
+        const auto vr = make_rsrc((const void*)(uintptr_t)va, rows ? (rows - 1) * p.v_row + 2 * p.D : 0);
+        if (stream) dma_tile<NGI, true>(vr, m0 + VT * 2, voff);
+        else dma_tile<NGI, false>(vr, m0 + VT * 2, voff);
+      }
     }
     held[slot] = at;
     if (more) {
@@ -435,28 +449,27 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
   };
 
   // The segment under way.
-  u32x4 qf[QB][NDC];    // Q rows as MFMA B operands: lane l = packed row qb * 16 + l % 16
-  f32x4 oacc[QB][NDB];  // O^T: lane l, register r = head dim 16 db + 4 (l / 16) + r of row l % 16
-  float m_i[QB], l_i[QB];
-  Row row[QB];          // this lane's rows
+  u32x4 qf[NDC];    // Q rows as MFMA B operands: lane l = the wave's row l % 16
+  f32x4 oacc[NDB];  // O^T: lane l, register r = head dim 16 db + 4 (l / 16) + r of row l % 16
+  float m_i, l_i;
+  Row row;          // this lane's
   const int most_lag = p.causal ? p.Sq - 1 : 0;
   bool from_start = false;  // whether it began with the row group's first step
 
   auto begin_segment = [&](const Unit& w, auto slot_c) {
     constexpr int slot = decltype(slot_c)::value;
-    const uint16_t* qs = smem + 4 * VT + slot * NQ * 512;
-    const int rb = w.hh % cold().nrb;
+    const uint16_t* qs = smem + 4 * VT + (slot * NW + wave) * NQ * 512;
+    const auto& c = cold();
+    const int rb = w.hh % c.nrb;
     from_start = w.begin == 2;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
+    for (int dc = 0; dc < NDC; ++dc) qf[dc] = lds_read16(qs + Tile::chunk(l16, 4 * dc + g16) * 8);
+    m_i = kNegInf;
+    l_i = 0.f;
+    row = row0;
+    if (rb > 0) row = output_row(c, rb);
 #pragma unroll
-      for (int dc = 0; dc < NDC; ++dc) qf[qb][dc] = lds_read16(qs + Tile::chunk(qb * 16 + l16, 4 * dc + g16) * 8);
-      m_i[qb] = kNegInf;
-      l_i[qb] = 0.f;
-      row[qb] = KEEP && rb == 0 ? row0[0] : output_row(cold(), qb, rb);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) oacc[qb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int db = 0; db < NDB; ++db) oacc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
 
   auto step = [&](const Unit& w, auto slot_c) {
@@ -470,66 +483,58 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
 #pragma unroll
       for (int dc = 0; dc < NDC; ++dc) ka[kb][dc] = lds_read16(Ks + Tile::chunk(kb * 16 + l16, 4 * dc + g16) * 8);
     const bool masked = seen[slot][0] + seen[slot][1] < kStep || w.rem - most_lag < kStep;
-    u32x4 pk[QB];
+    // S^T: lane l, register r = key kb * 16 + 4 (l / 16) + r of row l % 16.
+    f32x4 sc[2];
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      // S^T: lane l, register r = key kb * 16 + 4 (l / 16) + r of row l % 16.
-      f32x4 sc[2];
+    for (int kb = 0; kb < 2; ++kb) {
+      sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        sc[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int dc = 0; dc < NDC; ++dc) sc[kb] = Elem<T>::mfma16(ka[kb][dc], qf[qb][dc], sc[kb]);
-        sc[kb] *= p.scale_log2;
-      }
-      // Masked after the scale, so that a scale of zero leaves -inf.
-      if (masked) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int c = 4 * g16 + r;
-            const bool in = c < seen[slot][kb] && 16 * kb + c < w.rem - row[qb].lag;
-            sc[kb][r] = in ? sc[kb][r] : kNegInf;
-          }
-      }
-      float mx = kNegInf;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[kb][r]);
-      mx = wave_group16_max(mx);
-      if (m_i[qb] == kNegInf) {
-        m_i[qb] = mx;
-      } else {
-        const bool grow = mx > m_i[qb] + kRescaleThreshold;
-        if (wave_any(grow)) {
-          const float alpha = grow ? fast_exp2(m_i[qb] - mx) : 1.f;
-          l_i[qb] *= alpha;
-#pragma unroll
-          for (int db = 0; db < NDB; ++db) oacc[qb][db] *= alpha;
-          m_i[qb] = grow ? mx : m_i[qb];
-        }
-      }
-      // P in 16 bits for the second product. With m up to 8 below the maximum
-      // and the bias, P stays below 2^8 in bf16 and 2^15 in fp16, whose
-      // smallest value 2^-24 is then 2^-31 of the maximum: a long tail of
-      // small P is not lost.
-      const float msub = (m_i[qb] == kNegInf) ? 0.f : m_i[qb] - PBias<T>::v;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[kb][r] = fast_exp2(sc[kb][r] - msub);
-      // P^T as the B operand of O^T += V^T P^T: slot t of lane group g holds
-      // key 4 g + t (t < 4) or 16 + 4 g + t - 4 (t >= 4).
-      pk[qb][0] = pack2<T>(sc[0][0], sc[0][1]);
-      pk[qb][1] = pack2<T>(sc[0][2], sc[0][3]);
-      pk[qb][2] = pack2<T>(sc[1][0], sc[1][1]);
-      pk[qb][3] = pack2<T>(sc[1][2], sc[1][3]);
-      // The denominator sums the rounded P that the second product uses.
-      l_i[qb] += sum2_acc<T>(pk[qb][0], sum2_acc<T>(pk[qb][1], 0.f)) +
-                 sum2_acc<T>(pk[qb][2], sum2_acc<T>(pk[qb][3], 0.f));
+      for (int dc = 0; dc < NDC; ++dc) sc[kb] = Elem<T>::mfma16(ka[kb][dc], qf[dc], sc[kb]);
+      sc[kb] *= p.scale_log2;
     }
+    // Masked after the scale, so that a scale of zero leaves -inf.
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int c = 4 * g16 + r;
+          const bool in = c < seen[slot][kb] && 16 * kb + c < w.rem - row.lag;
+          sc[kb][r] = in ? sc[kb][r] : kNegInf;
+        }
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[kb][r]);
+    mx = wave_group16_max(mx);
+    if (m_i == kNegInf) {
+      m_i = mx;
+    } else {
+      const bool grow = mx > m_i + kRescaleThreshold;
+      if (wave_any(grow)) {
+        const float alpha = grow ? fast_exp2(m_i - mx) : 1.f;
+        l_i *= alpha;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) oacc[db] *= alpha;
+        m_i = grow ? mx : m_i;
+      }
+    }
+    // P in 16 bits for the second product. With m up to 8 below the maximum and
+    // the bias, P stays below 2^8 in bf16 and 2^15 in fp16, whose smallest value
+    // 2^-24 is then 2^-31 of the maximum: a long tail of small P is not lost.
+    const float msub = (m_i == kNegInf) ? 0.f : m_i - PBias<T>::v;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[kb][r] = fast_exp2(sc[kb][r] - msub);
+    // P^T as the B operand of O^T += V^T P^T: slot t of lane group g holds key
+    // 4 g + t (t < 4) or 16 + 4 g + t - 4 (t >= 4).
+    const u32x4 pk = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
+                      pack2<T>(sc[1][0], sc[1][1]), pack2<T>(sc[1][2], sc[1][3])};
+    // The denominator sums the rounded P that the second product uses.
+    l_i += sum2_acc<T>(pk[0], sum2_acc<T>(pk[1], 0.f)) + sum2_acc<T>(pk[2], sum2_acc<T>(pk[3], 0.f));
     // V^T A operands by transposed reads: lane (g, i) receives V[key][16 db + i]
     // for the keys of slot t above.
     auto v_operand = [&](int db) -> u32x4 {
@@ -549,23 +554,14 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
     }
     if (!apart) {
 #pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const u32x4 a = v_operand(db);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) oacc[qb][db] = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
-      }
+      for (int db = 0; db < NDB; ++db) oacc[db] = Elem<T>::mfma16(v_operand(db), pk, oacc[db]);
       return;
     }
     // Then the rows of each limit on their own, V behind it as zeros.
 #pragma unroll 1
     for (int limit = 1; limit <= kStep; ++limit) {
-      bool mine[QB], any = false;
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        mine[qb] = min(w.rem - row[qb].lag, kStep) == limit;
-        any |= mine[qb];
-      }
-      if (!wave_any(any)) continue;
+      const bool mine = min(w.rem - row.lag, kStep) == limit;
+      if (!wave_any(mine)) continue;
       u32x4 keep;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -574,13 +570,9 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       }
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
-        const u32x4 a = v_operand(db) & keep;
+        const f32x4 sum = Elem<T>::mfma16(v_operand(db) & keep, pk, oacc[db]);
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-          const f32x4 sum = Elem<T>::mfma16(a, pk[qb], oacc[qb][db]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) oacc[qb][db][r] = mine[qb] ? sum[r] : oacc[qb][db][r];
-        }
+        for (int r = 0; r < 4; ++r) oacc[db][r] = mine ? sum[r] : oacc[db][r];
       }
     }
   };
@@ -589,59 +581,48 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
   // every case (lanes without an output, and whole stores where there is
   // nothing to say, lie outside their resource), so that the waits can count
   // them instead of waiting for them.
-  constexpr int NS = QB * (NDB + 1) + 1;
+  constexpr int NS = NDB + 2;
   auto end_segment = [&](const Unit& w) {
     const bool whole = from_start && w.rem <= kStep;
     const auto& c = cold();
     const int kvh = w.hh / c.nrb, rb = w.hh - kvh * c.nrb;
     const int group = w.b * c.heads + w.hh;
-    const int64_t slot = (int64_t)(worker + group) * c.rows;
+    const int r = wave * 16 + l16;
+    const float lt = wave_group16_sum(l_i);
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    const float lse = lt > 0.f ? (m_i - PBias<T>::v + fast_log2(lt)) * kLn2 : kNegInf;
     // kOOB is the top bit, which no offset inside a resource has.
-    const uint32_t one_lane = g16 == 0 ? 0u : kOOB;
+    const uint32_t none = row.out & kOOB, one_lane = g16 == 0 ? none : kOOB;
     auto beyond = [&](int d) -> uint32_t { return (uint32_t)(c.D - 1 - d) & kOOB; };
-    float inv[QB], lse[QB];
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      const float lt = wave_group16_sum(l_i[qb]);
-      inv[qb] = lt > 0.f ? 1.f / lt : 0.f;
-      lse[qb] = lt > 0.f ? (m_i[qb] - PBias<T>::v + fast_log2(lt)) * kLn2 : kNegInf;
-    }
     if (whole) {
       const auto orr = make_rsrc(c.o + w.b * c.o_sb + (int64_t)kvh * c.G * c.o_sh, c.o_bytes);
       const auto lrr = make_rsrc(c.lse + ((int64_t)w.b * c.Hq + kvh * c.G) * c.Sq, c.lse ? c.G * c.Sq * 4u : 0u);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const int d = 16 * db + 4 * g16;
-          const f32x4 ov = oacc[qb][db] * inv[qb];
-          const u32x2 o2 = {pack2<T>(ov[0], ov[1]), pack2<T>(ov[2], ov[3])};
-          __builtin_amdgcn_raw_buffer_store_b64(o2, orr, row[qb].out + d * 2u | beyond(d), 0, 0);
-        }
-        const int rho = rb * c.rows + qb * 16 + l16;
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse[qb]), lrr, rho * 4u | (row[qb].out & kOOB) | one_lane, 0, 0);
+      for (int db = 0; db < NDB; ++db) {
+        const int d = 16 * db + 4 * g16;
+        const f32x4 ov = oacc[db] * inv;
+        const u32x2 o2 = {pack2<T>(ov[0], ov[1]), pack2<T>(ov[2], ov[3])};
+        __builtin_amdgcn_raw_buffer_store_b64(o2, orr, (row.out + d * 2u) | beyond(d), 0, 0);
       }
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse), lrr, (rb * c.rows + r) * 4u | one_lane, 0, 0);
     } else {
+      const int64_t slot = (int64_t)(worker + group) * c.rows;
       const auto orr = make_rsrc(c.part_o + slot * c.D, (uint32_t)(c.rows * c.D * 4));
       const auto lrr = make_rsrc(c.part_lse + slot, c.rows * 4u);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const int r = qb * 16 + l16;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const int d = 16 * db + 4 * g16;
-          const f32x4 ov = oacc[qb][db] * inv[qb];
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, ov), orr,
-                                                 (uint32_t)(r * c.D + d) * 4u | (row[qb].out & kOOB) | beyond(d), 0, 0);
-        }
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse[qb]), lrr, r * 4u | (row[qb].out & kOOB) | one_lane, 0, 0);
+      for (int db = 0; db < NDB; ++db) {
+        const int d = 16 * db + 4 * g16;
+        const f32x4 ov = oacc[db] * inv;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, ov), orr,
+                                               (uint32_t)(r * c.D + d) * 4u | none | beyond(d), 0, 0);
       }
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(lse), lrr, r * 4u | one_lane, 0, 0);
     }
     // The row group's first worker says how many there are: the steps behind
     // its own fill whole runs.
     const u32x2 parts = {(uint32_t)worker, (uint32_t)(1 + ((w.rem - 1) / kStep + run - 1) / run)};
     __builtin_amdgcn_raw_buffer_store_b64(parts, make_rsrc(c.parts + 2 * (int64_t)group, 8u),
-                                          from_start && lane == 0 ? 0u : kOOB, 0, 0);
+                                          from_start && threadIdx.x == 0 ? 0u : kOOB, 0, 0);
   };
 
   // Two units are in flight, whatever segments they belong to: a segment's
@@ -667,12 +648,14 @@ __global__ __launch_bounds__(64) void paged_kernel(const PagedParams p) {
       if (j >= 0 && j < count) {
         const bool next = j + 1 < count;
         wait(ended, next ? held[1 - slot].begin ? 2 : 1 : 0);
+        worker_barrier<NW>();  // the other waves' loads of the unit are done too
         const Unit w = held[slot];
         if (w.begin) begin_segment(w, sc);
         step(w, sc);
         ended = !next || w.rem <= kStep;
         if (ended) end_segment(w);
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read,
+        worker_barrier<NW>();                // by the other waves too
       }
       if (j + 2 < count) issue(j + 3 < count, sc);
     });
@@ -746,16 +729,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(cons
   }
 }
 
-// Packed rows per worker: 16-row MFMA blocks, up to four of them.
-static int paged_row_blocks(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
+// Packed rows per row group, and the waves that they take.
 static int paged_rows(int64_t R) { return (int)(R < 64 ? R : 64); }
+static int paged_waves(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
-// Workers: what the LDS of 256 CUs holds of them (160 KB each, given out in
-// pieces of 1280 bytes), at most 8 per CU.
+// Workers: what 256 CUs hold of them at once.
+template <int NW>
+static int workers_of(int DT) {
+  return 256 * (DT == 32 ? workers_per_cu(32, NW) : DT == 64 ? workers_per_cu(64, NW)
+                : DT == 96 ? workers_per_cu(96, NW) : workers_per_cu(128, NW));
+}
 static int paged_workers(int64_t D, int64_t R) {
-  const int lds = (worker_lds(head_tile(D), paged_row_blocks(R)) + 1279) / 1280 * 1280;
-  const int per_cu = 160 * 1024 / lds;
-  return 256 * (per_cu < 8 ? per_cu : 8);
+  const int DT = head_tile(D), NW = paged_waves(R);
+  return NW == 1 ? workers_of<1>(DT) : NW == 2 ? workers_of<2>(DT) : workers_of<4>(DT);
 }
 
 static int64_t paged_slots(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D) {
@@ -787,10 +773,10 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
 template <typename T, int DT>
 static int launch_paged(const PagedParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.workers);
-  switch (paged_row_blocks(p.rows)) {
+  switch (paged_waves(p.rows)) {
     case 1: hipLaunchKernelGGL((paged_kernel<T, DT, 1>), grid, dim3(64), 0, stream, p); break;
-    case 2: hipLaunchKernelGGL((paged_kernel<T, DT, 2>), grid, dim3(64), 0, stream, p); break;
-    default: hipLaunchKernelGGL((paged_kernel<T, DT, 4>), grid, dim3(64), 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((paged_kernel<T, DT, 2>), grid, dim3(128), 0, stream, p); break;
+    default: hipLaunchKernelGGL((paged_kernel<T, DT, 4>), grid, dim3(256), 0, stream, p); break;
   }
   const int rc = check_launch("kf_paged_decode(workers)");
   if (rc) return rc;
