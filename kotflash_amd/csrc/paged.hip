@@ -174,10 +174,12 @@ constexpr int q_loads(int DT) { return 16 * (DT / 8) / 64; }
 // segments.
 constexpr int worker_lds(int DT, int NW) { return 2 * (2 * kStep * DT * 2 + NW * q_loads(DT) * 1024); }
 // Workers that a CU holds: by its 160 KB of LDS, given out in pieces of 1280
-// bytes, and by the registers of two (NW = 1) or three waves per SIMD.
+// bytes, and by waves (two per SIMD, four of four-wave workers: 16 requests up
+// to 16384 tokens, 8 KV heads, D=64, us with 8, 12 and 16 waves: 32 rows 58.2,
+// 61.6 and 61.4, 64 rows 89.4, 77.1 and 72.6; D=128 is bound by the LDS).
 constexpr int workers_per_cu(int DT, int NW) {
   const int by_lds = 160 * 1024 / ((worker_lds(DT, NW) + 1279) / 1280 * 1280);
-  const int by_waves = NW == 1 ? 8 : 12 / NW;
+  const int by_waves = NW == 4 ? 4 : 8 / NW;
   return by_lds < by_waves ? by_lds : by_waves;
 }
 
