@@ -10,26 +10,31 @@
 // How the work is cut. The lengths are known on the GPU only (a captured graph
 // replays with others), so the launch cannot be planned on the host. All
 // requests' keys are numbered in steps of 32: unit u = (request, KV head and
-// row block, step). A fixed number of workers (one wave each, as many as LDS
-// lets the GPU hold) take equal runs of consecutive units, wherever requests
-// begin and end in them: every worker streams the same number of bytes however
-// the lengths differ, which a grid of (request, head, split) does not give.
+// row group of up to 64 packed query rows, step). A fixed number of workers, as
+// many as the GPU holds at once, take equal runs of consecutive units, wherever
+// requests begin and end in them: every worker streams the same number of bytes
+// however the lengths differ, which a grid of (request, head, split) does not
+// give.
 //  * A worker finds its run from the lengths: a sum over the batch, and the
 //    request in which the run begins.
-//  * Within a run the part in one (request, head) is a segment: the packed
-//    query rows of the group against its steps (S^T = K Q^T, online softmax,
-//    O^T += V^T P^T on 16x16x32 MFMAs, as in the contiguous decode). Two units
-//    are in flight in a wave-private LDS ring that direct-to-LDS loads fill,
-//    across the ends of segments: short requests stream like long ones.
+//  * Within a run the part in one (request, row group) is a segment: S^T =
+//    K Q^T, online softmax, O^T += V^T P^T on 16x16x32 MFMAs, as in the
+//    contiguous decode. Two units are in flight in an LDS ring that
+//    direct-to-LDS loads fill, across the ends of segments: short requests
+//    stream like long ones.
+//  * A worker is one wave per 16 packed rows (one, two or four). One wave needs
+//    no barrier; more share the ring with two per unit.
 //  * A segment that is a whole request writes O; others write an fp32 partial
 //    (O, LSE) to slot worker + row group. Both numbers grow along the units
 //    and one of them at every segment, so the slots are distinct, and those of
 //    one row group are consecutive. The second launch merges them in order
 //    (no atomics, same bits every time) and zeroes the rows that see nothing.
-//  * One wave per worker: no barrier anywhere, and while one worker of a CU
-//    starts or ends a segment the others stream.
-//
 //  * A decoding step's new rows may be stored by the same launch (store_new).
+//
+// What it reaches on MI355X (16 packed rows or fewer): 6.3 to 6.6 TB/s behind
+// the first 8 us, which are two dependent launches and, in the first, a chain
+// of loads; reading the same 4 KB pieces in random order without any of the
+// work reaches 6.7 to 6.8.
 //
 // Pages: 16 rows of one page at a time have a buffer resource of their own,
 // from a page number read by the scalar unit, with 64-bit bases (a pool may be
@@ -123,10 +128,10 @@ constexpr int kStep = 32;     // keys per unit
 
 // K/V bytes of a call from which its loads are marked as read once. Such loads
 // do not go through the 256 MB memory-side cache, which costs the others a
-// tenth of their rate (measured, three sets of inputs in turn: 1158 MB 209 us
-// plain and 188 marked, 537 MB 103 and 93, 300 MB 64 and 57, 294 MB 62 and
-// 54); but a call of which the cache still holds a part from the last time is
-// faster plain (59 MB 21 and 23).
+// tenth of their rate (us, plain and marked, three sets of inputs in turn: 1158
+// MB 205 and 185, 537 MB 99 and 89, 300 MB 65 and 59, 294 MB 60 and 54); but a
+// call of which the cache still holds a part from the last time is faster plain
+// (59 MB 19.9 and 20.8).
 constexpr int64_t kStreamBytes = 128 << 20;
 
 __device__ inline int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
@@ -671,7 +676,8 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
 // share, and combine through LDS in their order.
 // Half the partials in flight of the contiguous decode's merge (half the
 // registers, twice the rows at once: 8192 rows of two or three partials 7.3 us
-// with 16, 5.7 with 8, 5.3 with 4; 768 rows of 40 partials 5.3, 4.2 and 4.5).
+// with 16, 5.7 with 8, 5.3 with 4; 131072 keys of one request and one KV head,
+// about 1000 partials a row, want them).
 constexpr int kPartsU = 8;
 // With W = 1, four rows share a workgroup.
 template <typename T, int QL, int W>
@@ -753,10 +759,11 @@ static int64_t paged_slots(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64
 
 // Waves per row of the merge, from the most partials a row group can have: a
 // head's share of the workers (all of them on one request), cut at both ends.
-// More waves cost launch time where they are not needed (1158 MB over 64
-// requests: 4.6 us with one wave, 5.0 with four, 7.2 with eight) and save round
-// trips where one row has many partials (131072 keys of one request, 128
-// partials: 5.9 us with one wave, 4.6 with four).
+// More waves cost launch time where they are not needed and save round trips
+// where one row has many partials. Measured, us with one, four and sixteen
+// waves: 8192 rows of two or three partials 5.7, 9.8 and 30, 2048 of them 4.6,
+// 4.7 and 10; 32 rows of 128 partials 7.6, 4.7 and 5.0; 16 rows of about 1000
+// 37, 11.8 and 9.5.
 template <typename T, int QL>
 static void launch_merge(const PagedParams& p, hipStream_t stream) {
   constexpr int kTrip = kPartsU * (64 / QL);  // partials that a wave takes at once
@@ -766,7 +773,7 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)rows);
   if (most > 16 * kTrip && rows <= 256)
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 16>), grid, dim3(1024), 0, stream, p);
-  else if (most > kTrip && (rows <= 256 || most > 8 * kTrip))
+  else if (most > kTrip && (rows <= 256 || (most > 8 * kTrip && rows <= 2048) || most > 32 * kTrip))
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 4>), grid, dim3(256), 0, stream, p);
   else
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);

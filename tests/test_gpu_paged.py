@@ -769,3 +769,12 @@ def test_gradients_are_refused():
     with torch.no_grad():
         cache.append_and_attend(q, new, new, slots)
     assert (cache.k_pages != 0).any()
+
+
+@pytest.mark.parametrize("batch,hq,hkv,d,longest", [(40, 16, 1, 64, 20000), (40, 16, 1, 128, 9000), (1, 16, 1, 64, 40000),
+                                                    (2, 8, 8, 96, 9000), (300, 16, 1, 128, 700)])
+def test_rows_with_many_partials(batch, hq, hkv, d, longest):
+    """One long request among short ones: few and many rows, few and many
+    partials of a row."""
+    lengths = [longest] + [(7 * i) % 90 for i in range(1, batch)]
+    _check(make_case(batch, hq, hkv, 1, d, 16, lengths, dtype=F16, seed=d, device="cuda"))
