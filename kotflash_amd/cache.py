@@ -10,8 +10,9 @@ fp16/bf16 caches on gfx950, torch copies otherwise).
 
 ``RaggedKVCache`` extends the fixed-capacity cache to per-sequence lengths:
 every sequence appends at its own position in one launch and decode masks
-each sequence to its own prefix. These helpers do not implement paging,
-eviction, batching or model projections.
+each sequence to its own prefix. ``kotflash_amd.paged`` has the cache in pages
+of a common pool. These helpers do not implement eviction, batching or model
+projections.
 """
 from __future__ import annotations
 
