@@ -340,7 +340,8 @@ int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, voi
  * stored at their slots by the workers that read them. The lengths include
  * the new tokens, and a request's named slots (those inside the pool) are, in
  * order, those of its last positions, as kf_page_reserve returned them; rows
- * of a request with fewer positions than named slots may not be stored. The
+ * of a request with fewer positions than named slots may not be stored, and
+ * another request whose table holds the same page may not see them yet. The
  * new rows need a unit head_dim stride, 16-byte aligned bases and strides that
  * are multiples of 8 elements (int64_t[3]), and the pool fewer than 2^31 slots.
  */

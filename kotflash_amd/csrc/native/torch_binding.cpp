@@ -477,7 +477,7 @@ PyObject* py_store_lengths(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // column stride, lengths [B], free_pages [pages] and counters [4], contiguous.
 
 bool int32_on(const Tensor* t, const c10::Device& dev) {
-  return t && t->scalar_type() == at::kInt && t->device() == dev && !t->is_inference();
+  return t && t->scalar_type() == at::kInt && t->device() == dev;
 }
 
 // Pools [pages, Hkv, page, D] that the kernels read and write in place.
@@ -673,9 +673,10 @@ struct TableArgs {
     return true;
   }
   // The version counters of what a call has written, as an in-place torch
-  // operation moves them.
+  // operation moves them. (Tensors made in inference mode have none.)
   void written() const {
-    for (const Tensor* t : {tables, lengths, free_pages, counters}) t->unsafeGetTensorImpl()->bump_version();
+    for (const Tensor* t : {tables, lengths, free_pages, counters})
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   }
 };
 

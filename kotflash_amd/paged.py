@@ -104,9 +104,10 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
     page_size]`` (int32 [B, columns]) of the pools [pages, Hkv, page_size, D];
     its rows see the first ``lengths[b]`` (int32 [B]) positions. With
     ``causal`` the Sq query tokens are the request's last ones (draft tokens,
-    already stored): row i sees the first ``lengths[b] - Sq + 1 + i``. A row
-    that sees nothing gives zeros (LSE -inf); a position whose page number is
-    outside the pool is not seen. MHA, GQA and MQA as in ``attention``.
+    already stored): row i sees the first ``lengths[b] - Sq + 1 + i``, so a
+    request with fewer new tokens than Sq has them in its last rows. A row that
+    sees nothing gives zeros (LSE -inf); a position whose page number is outside
+    the pool is not seen. MHA, GQA and MQA as in ``attention``.
 
     ``hip`` needs gfx950, fp16 or bf16, a head_dim that is a multiple of 8 up
     to 128 and a page_size that is a multiple of 16; ``auto`` takes it where
@@ -256,6 +257,9 @@ class PageTable:
             raise ValueError(f"{name} must be in [0, 2**30)")
         return value
 
+    def _tensor_of(self, value) -> torch.Tensor:
+        return value if isinstance(value, torch.Tensor) else torch.full_like(self.lengths, value)
+
     def reserve(self, counts: Union[int, torch.Tensor], *, width: Optional[int] = None,
                 backend: str = "auto") -> torch.Tensor:
         """Room for ``counts`` more tokens (an int for every request, or int32
@@ -283,6 +287,10 @@ class PageTable:
             raise ValueError("counts must not exceed width")
         state = (self.tables, self.lengths, self.free_pages, self.counters)
         if _store_on_hip(backend, self.tables, half=False):
+            if torch.compiler.is_compiling():
+                from .ops import page_reserve_
+
+                return page_reserve_(*state, self._tensor_of(counts), self.page_size, width)
             return hip_paged.reserve_pages(*state, counts, width, self.page_size)
         return _reserve(*state, counts, width, self.page_size)
 
@@ -298,6 +306,11 @@ class PageTable:
         lengths = self._per_request("lengths", lengths)
         state = (self.tables, self.lengths, self.free_pages, self.counters)
         if _store_on_hip(backend, self.tables, half=False):
+            if torch.compiler.is_compiling():
+                from .ops import page_trim_
+
+                page_trim_(*state, self._tensor_of(lengths), self.page_size)
+                return
             hip_paged.trim_pages(*state, lengths, self.page_size)
         else:
             _trim(*state, lengths, self.page_size)
@@ -381,8 +394,10 @@ class PagedKVCache:
 
         ``append_backend="fused"`` stores the new rows from inside the
         attention's launches (HIP attention, up to 16 tokens a request);
-        ``"auto"`` takes it when it applies. The others store first, in a
-        launch of their own, at any slots.
+        ``"auto"`` takes it when it applies. The new rows must then be seen by
+        their own request alone, as everywhere that no two requests of the call
+        were given the same page. The others store first, in a launch of their
+        own, at any slots.
         """
         fuse = append_backend in ("auto", "fused")
         if (fuse or append_backend in ("hip", "cuda")) and attention_backend in ("auto", "hip", "triton") \

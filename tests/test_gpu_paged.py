@@ -778,3 +778,85 @@ def test_rows_with_many_partials(batch, hq, hkv, d, longest):
     partials of a row."""
     lengths = [longest] + [(7 * i) % 90 for i in range(1, batch)]
     _check(make_case(batch, hq, hkv, 1, d, 16, lengths, dtype=F16, seed=d, device="cuda"))
+
+
+def test_tables_of_inference_mode_take_the_native_path(monkeypatch):
+    """A server that makes its cache under inference_mode gets the same launches."""
+    import kotflash_amd.kernels.hip_paged as hip_paged
+
+    def refuse(*args, **kw):
+        raise AssertionError("the Python path ran")
+
+    for name in ("reserve_pages", "trim_pages", "attention_paged", "append_attention_paged"):
+        monkeypatch.setattr(hip_paged, name, refuse)
+    with torch.inference_mode():
+        table = PageTable(2, 64, num_pages=8)
+        cache = PagedKVCache(table, 2, 64, dtype=F16)
+        new = torch.randn(2, 2, 2, 1, 64, device="cuda").to(F16)
+        q = torch.randn(2, 4, 1, 64, device="cuda").to(F16)
+        out = cache.append_and_attend(q, *new, table.reserve(1))
+        assert table.lengths.tolist() == [1, 1]
+        table.trim(0)
+    assert torch.equal(out, new[1].repeat_interleave(2, 1))
+    assert table.num_free() == 8 and table.lengths.tolist() == [0, 0]
+
+
+def test_a_whole_step_under_torch_compile():
+    """Tables, store and attention compiled together, over page borders,
+    against the same calls without."""
+    results = []
+    for compiled in (False, True):
+        torch.manual_seed(5)
+        table = PageTable(2, 128, num_pages=16)
+        cache = PagedKVCache(table, 2, 64, dtype=F16)
+        cache.k_pages.zero_()
+        cache.v_pages.zero_()
+        most = _counts([20, 100])
+
+        def step(q, n):
+            table.trim(most)
+            slots = table.reserve(1)
+            return cache.append_and_attend(q, n, n, slots, append_backend="hip")
+
+        fn = torch.compile(step, backend="aot_eager") if compiled else step
+        outs = []
+        for _ in range(36):
+            n = torch.randn(2, 2, 1, 64, device="cuda").to(F16)
+            q = torch.randn(2, 4, 1, 64, device="cuda").to(F16)
+            outs.append(fn(q, n))
+        results.append([torch.stack(outs), table.tables, table.lengths, table.free_pages, table.counters,
+                        cache.k_pages, cache.v_pages])
+    assert results[0][2].tolist() == [21, 36]
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("how", ["fused", "hip"])
+def test_drafts_of_their_own_number(how):
+    """Requests with fewer drafts than rows: theirs are the last rows of q, in
+    whatever columns their new rows and slots stand."""
+    n, counts, before = 4, [4, 1, 3, 0, 2], [30, 0, 15, 20, 64]
+    b = len(counts)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    table = PageTable(b, 128, num_pages=40)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.fill_(math.nan)
+    cache.v_pages.fill_(math.nan)
+    old = torch.randn(2, b, 2, max(before), 64, device="cuda", generator=g).to(F16)
+    cache.append(*old, table.reserve(_counts(before), width=max(before)))
+    slots = table.reserve(_counts(counts), width=n)
+    new = torch.randn(2, b, 2, n, 64, device="cuda", generator=g).to(F16)
+    q = torch.randn(b, 8, n, 64, device="cuda", generator=g).to(F16)
+    # Right-aligned, as the rows of q are.
+    last = torch.stack([s.roll(n - c) for s, c in zip(slots, counts)])
+    out = cache.append_and_attend(q, *new, last, causal=True, append_backend=how)
+    own = [torch.cat((old[i], torch.zeros_like(new[i])), 2) for i in range(2)]
+    for i in range(2):
+        for r, (x, c) in enumerate(zip(before, counts)):
+            own[i][r, :, x:x + c] = new[i][r, :, n - c:]
+    ids = torch.arange(b, dtype=torch.int32)[:, None]
+    assert_attention(out, q, *own, ids, torch.tensor([x + c for x, c in zip(before, counts)], dtype=torch.int32),
+                     causal=True)
+    # The token of the request with one draft sees itself alone, in the last row.
+    assert torch.equal(out[1, :, -1], new[1][1, :, -1].repeat_interleave(4, 0))
+    assert (out[1, :, :-1] == 0).all()
