@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define KF_ABI_VERSION 7
+#define KF_ABI_VERSION 8
 
 enum kf_status {
   KF_OK = 0,
@@ -336,16 +336,14 @@ int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, voi
 
 /*
  * kf_paged_append and kf_paged_decode of one decoding step in the launches of
- * the latter: the Snew <= KF_PAGED_STEP_TOKENS new rows of each request are
- * stored at their slots by the workers that read them. The lengths include
- * the new tokens, and a request's named slots (those inside the pool) are, in
- * order, those of its last positions, as kf_page_reserve returned them; rows
- * of a request with fewer positions than named slots may not be stored, and
- * another request whose table holds the same page may not see them yet. The
+ * the latter, with the result of the one after the other: every worker first
+ * writes the new rows among those that it reads, whichever request's slots they
+ * are. Snew <= KF_PAGED_STEP_TOKENS and B * Snew <= KF_PAGED_STEP_SLOTS. The
  * new rows need a unit head_dim stride, 16-byte aligned bases and strides that
  * are multiples of 8 elements (int64_t[3]), and the pool fewer than 2^31 slots.
  */
 #define KF_PAGED_STEP_TOKENS 16
+#define KF_PAGED_STEP_SLOTS 256
 int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const void* new_k,
                            const void* new_v, const int64_t* slots, void* o, float* lse,
                            const int32_t* tables, const int32_t* lengths, int64_t B, int64_t Hq,

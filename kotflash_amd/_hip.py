@@ -20,9 +20,9 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libkotflash_amd.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 KF_F16, KF_BF16 = 0, 1
-KF_PAGED_STEP_TOKENS = 16
+KF_PAGED_STEP_TOKENS, KF_PAGED_STEP_SLOTS = 16, 256
 KF_BWD_DELTA, KF_BWD_DQ, KF_BWD_DKDV, KF_BWD_DKDV_FIXUP = 1, 2, 4, 8
 KF_BWD_ALL = KF_BWD_DELTA | KF_BWD_DQ | KF_BWD_DKDV | KF_BWD_DKDV_FIXUP
 

@@ -611,20 +611,26 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Most new rows that append_backend="auto" has stored by the attention's
+// launches (hip_paged.FUSED_STEP_ROWS).
+constexpr int64_t kFusedStepRows = 64;
+
 // paged_step(q, k_pages, v_pages, tables, lengths, causal, None, new_k, new_v,
-// slots, fuse): the store, then the attention; in the attention's launches
-// with `fuse`, for rows that these take.
+// slots, how): the store, then the attention; how = 0: in a launch of its own,
+// 2: in the attention's launches, 1: there if that is faster.
 PyObject* py_paged_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   PagedArgs a;
   StoreArgs st;
-  bool fuse;
-  if (n != 11 || !exact_bool(args[10], fuse) || !a.read(args)) return not_handled();
+  if (n != 11 || !PyLong_CheckExact(args[10]) || !a.read(args)) return not_handled();
+  const long how = PyLong_AsLong(args[10]);
   PyObject* const store[] = {args[1], args[2], args[7], args[8], args[9]};
   if (!st.read(store)) return not_handled();
-  if (fuse && (st.nk->size(0) != a.q->size(0) || st.nk->size(2) > KF_PAGED_STEP_TOKENS ||
-               st.k->size(0) * st.k->size(2) >= (1ll << 31)))
-    return not_handled();
+  const int64_t rows = st.nk->size(0) * st.nk->size(2);
+  const bool fits = st.nk->size(0) == a.q->size(0) && st.nk->size(2) <= KF_PAGED_STEP_TOKENS &&
+                    rows <= KF_PAGED_STEP_SLOTS && st.k->size(0) * st.k->size(2) < (1ll << 31);
+  if (how == 2 && !fits) return not_handled();
+  const bool fuse = how == 2 || (how == 1 && fits && rows <= kFusedStepRows);
   Tensor out;
   {
     pybind11::gil_scoped_release nogil;

@@ -29,7 +29,7 @@
 //    and one of them at every segment, so the slots are distinct, and those of
 //    one row group are consecutive. The second launch merges them in order
 //    (no atomics, same bits every time) and zeroes the rows that see nothing.
-//  * A decoding step's new rows may be stored by the same launch (store_new).
+//  * A decoding step's new rows may be stored by the same launch (store_hits).
 //
 // What it reaches on MI355X (16 packed rows or fewer): 6.3 to 6.6 TB/s behind
 // the first 8 us, which are two dependent launches and, in the first, a chain
@@ -81,7 +81,8 @@ struct PagedParams {
   uint32_t q_bytes, o_bytes;  // extents of a KV head's queries and outputs
   int causal;
   float scale_log2;
-  // Fused store (nnew > 0): the new rows [B, Hkv, nnew, D] and their slots.
+  // Fused store (nnew > 0): the new rows [B, Hkv, nnew, D], B * nnew <=
+  // KF_PAGED_STEP_SLOTS, and their slots.
   const uint16_t* nk;
   const uint16_t* nv;
   const int64_t* slots;
@@ -89,6 +90,7 @@ struct PagedParams {
   int64_t nk_sb, nk_sh, nk_ss;
   int64_t nv_sb, nv_sh, nv_ss;
   int nnew, page_size;
+  uint32_t nnew_inv;  // 2^16 / nnew + 1
 };
 
 // Direct-to-LDS loads (kf_common.hpp) of whole tiles: N loads of 1 KB, one
@@ -169,6 +171,10 @@ __device__ inline bool any_nonfinite(u32x4 x) {
   return bad;
 }
 
+// i / nnew of a new row's number: exact, as i < 2^8 and nnew <= 2^4.
+template <typename P>
+__device__ inline int new_row_request(const P& c, int i) { return (int)((uint32_t)i * c.nnew_inv >> 16); }
+
 template <typename T> struct PBias;  // P = 2^(s - m + bias), see paged_kernel
 template <> struct PBias<_Float16> { static constexpr float v = 7.f; };
 template <> struct PBias<__bf16> { static constexpr float v = 0.f; };
@@ -221,6 +227,58 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   // pages, keys), 5 us of it in this kernel.
   const int raw0 = p.lengths[min(lane, p.B - 1)];
 
+  // The parameters that only the ends of segments need are read again there:
+  // the scalar registers do not hold them all, and spilled ones cost vector
+  // instructions in every step. (The empty asm keeps the compiler from reading
+  // them once.)
+  auto cold = [&]() -> const PagedParams KF_CONST& {
+    auto ptr = (const PagedParams KF_CONST*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(ptr));
+    return *ptr;
+  };
+  // The fused store. A new row may be read by any request whose table leads to
+  // its slot, at any position, and no order between the workers says who is
+  // first. So every worker that reads 16 rows of a page first writes the new rows
+  // among them itself (store_hits), all of them the same bytes, and none waits
+  // for another. For that each wave keeps the 16-row groups of the call's slots:
+  // slot i's in lane i % 64 of register i / 64, -1 where it is outside the pool.
+  // Rows that nobody reads are stored by the loop below, which has every row
+  // once, shared out from the last wave, idle in a short call, to the first.
+  int fresh[KF_PAGED_STEP_SLOTS / 64] = {-1, -1, -1, -1};
+  static_assert(KF_PAGED_STEP_SLOTS == 4 * 64);
+  auto put_row = [&](const auto& c, int i, int kvh, uint64_t kbase, uint64_t vbase) {  // by 16 lanes
+    const int ch = lane & 15;
+    if (ch * 8 >= c.D) return;
+    const int b = new_row_request(c, i), t = i - b * c.nnew;
+    const int64_t slot = c.slots[b * c.s_sb + t];
+    const u32x4 kk = ldg16(c.nk + b * c.nk_sb + kvh * c.nk_sh + t * c.nk_ss + ch * 8);
+    const u32x4 vv = ldg16(c.nv + b * c.nv_sb + kvh * c.nv_sh + t * c.nv_ss + ch * 8);
+    if (slot < 0 || slot >= (int64_t)c.pages * c.page_size) return;
+    const uint32_t id = (uint32_t)slot / (uint32_t)c.page_size, at = (uint32_t)slot - id * (uint32_t)c.page_size;
+    stg16((char*)(uintptr_t)kbase + (uint64_t)id * c.k_page + (uint64_t)at * c.k_row + ch * 16, kk);
+    stg16((char*)(uintptr_t)vbase + (uint64_t)id * c.v_page + (uint64_t)at * c.v_row + ch * 16, vv);
+  };
+  if (p.nnew > 0) {
+    const auto& c = cold();
+    const int rows = c.B * c.nnew;
+    int64_t slot[4];  // all on their way at once
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(64 * k + lane, rows - 1), b = new_row_request(c, i);
+      slot[k] = c.slots[b * c.s_sb + i - b * c.nnew];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      fresh[k] = 64 * k + lane < rows && slot[k] >= 0 && slot[k] < (int64_t)c.pages * c.page_size ? (int)slot[k] >> 4 : -1;
+    const uint32_t all = (uint32_t)rows * (uint32_t)c.Hkv;
+    for (uint32_t e = ((uint32_t)(c.workers - 1 - (int)blockIdx.x) * NW + wave) * 4 + (lane >> 4); e < all;
+         e += (uint32_t)c.workers * NW * 4) {
+      const int kvh = (int)(e / (uint32_t)rows);
+      put_row(c, (int)(e - (uint32_t)kvh * rows), kvh, (uint64_t)(uintptr_t)(c.k + kvh * c.k_sh),
+              (uint64_t)(uintptr_t)(c.v + kvh * c.v_sh));
+    }
+  }
+
   // Per-lane plan of a group's loads: this lane's 16-byte chunk within the 16
   // rows (kOOB for head-dim padding). The swizzle key has a period of 16 rows,
   // so both groups of a step share it.
@@ -234,16 +292,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     koff[k] = ok ? (uint32_t)r * p.k_row + c * 16u : kOOB;
     voff[k] = ok ? (uint32_t)r * p.v_row + c * 16u : kOOB;
   }
-  // The parameters that only the ends of segments need are read again there:
-  // the scalar registers do not hold them all, and spilled ones cost vector
-  // instructions in every step. (The empty asm keeps the compiler from reading
-  // them once.)
-  auto cold = [&]() -> const PagedParams KF_CONST& {
-    auto ptr = (const PagedParams KF_CONST*)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(ptr));
-    return *ptr;
-  };
-  // And of the wave's Q loads and its lane's row, for the first row group of a
+  // The wave's Q loads and its lane's row, for the first row group of a
   // KV head (of most, the only one).
   auto query_offset = [&](const auto& c, int k, int rb) -> uint32_t {
     const int pc = k * 64 + lane;
@@ -313,7 +362,6 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   int column = 2 * s0 / p.gpp, part = 2 * s0 - column * p.gpp;
 
   const uint32_t lds0 = lds_addr(smem);
-  const int nnew = p.nnew > 0 ? p.nnew : -kStep;  // no unit's rem - kStep lies below it without new rows
   const bool stream = (int64_t)total * p.heads * (kStep * 4 * p.D) > kStreamBytes;
 
   // Of the request and head under way at `at`.
@@ -368,36 +416,29 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   // groups (0 for a page outside the pool).
   Unit held[2] = {at, at};
   int seen[2][2] = {{0, 0}, {0, 0}};
-  // The new rows among a unit's keys, from their own buffer to the pages, before
-  // the unit's loads: each reader of a row has written it itself (row groups of
-  // one KV head the same bytes), so no worker waits for another. The request's
-  // c named slots are those of its last c positions. Only the last units of a
-  // request come here, and wait for their stores: that costs a large call what
-  // the launch of a store would (294 MB over 32 requests 60.7 us per step
-  // either way); a short one is 3 us faster (1500 tokens of one 21.5 -> 18.1).
-  auto store_new = [&] {
+  // The new rows in the two groups of unit `at`, to their slots before the
+  // unit's loads, four at a time. Few units have any; those wait for their
+  // stores. Against the store in a launch of its own, us for both: 1 to 8 short
+  // requests 9.3 and 10.4, 64 of up to 500 tokens 10.7 and 11.8, but 294 MB over
+  // 32 requests 57.3 and 56.3, 64 requests of 4 drafts 69.7 and 64.8, 16 of 16
+  // 23.3 and 20.8.
+  auto store_hits = [&] {
+    const int g0 = (uint32_t)page[0] < (uint32_t)p.pages ? page[0] * p.gpp + part : -2;
+    const int g1 = (uint32_t)page[1] < (uint32_t)p.pages ? page[1] * p.gpp + row1 / 16 : -2;
+    uint32_t off = ~0u;
+#pragma unroll
+    for (int f : fresh) off = min(off, min((uint32_t)(f ^ g0), (uint32_t)(f ^ g1)));
+    if (!wave_any(off == 0)) return;
     const auto& c = cold();
     const int kvh = at.hh / c.nrb;
-    const int ch = lane & 15;
-    const uint16_t* nk = c.nk + at.b * c.nk_sb + kvh * c.nk_sh + ch * 8;
-    const uint16_t* nv = c.nv + at.b * c.nv_sb + kvh * c.nv_sh + ch * 8;
-    const int64_t* row_slots = c.slots + at.b * c.s_sb;
-    const int64_t mine = lane < c.nnew ? row_slots[lane] : -1;
-    for (int t0 = 0; t0 < c.nnew; t0 += 4) {
-      // Four rows at a time, on their way with the slots.
-      const int t = t0 + (lane >> 4);
-      u32x4 kk = zero_u4(), vv = zero_u4();
-      if (t < c.nnew && ch * 8 < c.D) {
-        kk = ldg16(nk + t * c.nk_ss);
-        vv = ldg16(nv + t * c.nv_ss);
-      }
-      const uint64_t named = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < (int64_t)c.pages * c.page_size);
-      const uint32_t slot = (uint32_t)__shfl((int)mine, t);
-      const int key = at.rem - __builtin_popcountll(named) + __builtin_popcountll(named & ((1ull << t) - 1));
-      if ((named >> t & 1) && key >= 0 && key < kStep && ch * 8 < c.D) {
-        const uint32_t id = slot / (uint32_t)c.page_size, row = slot - id * (uint32_t)c.page_size;
-        stg16((char*)(uintptr_t)kh + (uint64_t)id * c.k_page + (uint64_t)row * c.k_row + ch * 16, kk);
-        stg16((char*)(uintptr_t)vh + (uint64_t)id * c.v_page + (uint64_t)row * c.v_row + ch * 16, vv);
+#pragma unroll
+    for (int k = 0; k < KF_PAGED_STEP_SLOTS / 64; ++k) {
+      uint64_t hits = __builtin_amdgcn_ballot_w64(fresh[k] == g0 || fresh[k] == g1);
+      while (hits) {
+        int mine = -1;
+        for (int s = 0; s < 4 && hits; ++s, hits &= hits - 1)
+          if (lane >> 4 == s) mine = __builtin_ctzll(hits);
+        if (mine >= 0) put_row(c, 64 * k + mine, kvh, kh, vh);
       }
     }
     KF_WAIT_VMCNT(0);
@@ -408,7 +449,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   auto issue = [&](bool more, auto slot_c) {
     constexpr int slot = decltype(slot_c)::value;
     const uint32_t kv0 = lds0 + slot * 2 * VT * 2;
-    if (at.rem - kStep < nnew) store_new();
+    if (p.nnew > 0) store_hits();
     if (at.begin) {
       const auto& c = cold();
       const int kvh = at.hh / c.nrb;
@@ -893,6 +934,7 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
   p.scale_log2 = scale * kLog2e;
   p.page_size = (int)page_size;
   p.nnew = (int)fresh.n;
+  p.nnew_inv = fresh.n > 0 ? (uint32_t)(65536 / fresh.n + 1) : 0;
   if (fresh.n > 0) {
     p.nk = (const uint16_t*)fresh.k; p.nv = (const uint16_t*)fresh.v;
     p.slots = fresh.slots; p.s_sb = fresh.slots_stride;
@@ -931,6 +973,10 @@ extern "C" int kf_paged_append_decode(const void* q, void* k_pages, void* v_page
   if (Snew < 1 || Snew > KF_PAGED_STEP_TOKENS)
     return set_error(KF_EUNSUPPORTED, "%s: 1 to %d new tokens per request, got %lld", what, KF_PAGED_STEP_TOKENS,
                      (long long)Snew);
+  if (B > KF_PAGED_STEP_SLOTS / Snew)
+    return set_error(KF_EUNSUPPORTED, "%s: up to %d new tokens in all, got %lld", what, KF_PAGED_STEP_SLOTS,
+                     (long long)(B * Snew));
+  if (Hkv > 0x7fffffff / KF_PAGED_STEP_SLOTS) return set_error(KF_EUNSUPPORTED, "%s: too many heads", what);
   if (page_size > 0 && num_pages > 0x7fffffff / page_size)
     return set_error(KF_EUNSUPPORTED, "%s: a pool of 2^31 slots or more", what);
   const NewRows fresh = {new_k, new_v, slots, Snew, slots_stride, new_k_strides, new_v_strides};

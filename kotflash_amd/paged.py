@@ -389,21 +389,18 @@ class PagedKVCache:
     def append_and_attend(self, q, new_k, new_v, slots, *, causal: bool = False,
                           append_backend: str = "auto", attention_backend: str = "auto"):
         """``append``, then ``attend``: a decoding step of this layer, after
-        the table's ``reserve`` of the step, whose slots these are (those of
-        every request's last tokens).
+        the table's ``reserve`` of the step.
 
         ``append_backend="fused"`` stores the new rows from inside the
-        attention's launches (HIP attention, up to 16 tokens a request);
-        ``"auto"`` takes it when it applies. The new rows must then be seen by
-        their own request alone, as everywhere that no two requests of the call
-        were given the same page. The others store first, in a launch of their
-        own, at any slots.
+        attention's launches, to the same effect (HIP attention, up to 16 tokens
+        a request and 256 in all); ``"auto"`` takes it for up to 64. The others
+        store first, in a launch of their own.
         """
-        fuse = append_backend in ("auto", "fused")
-        if (fuse or append_backend in ("hip", "cuda")) and attention_backend in ("auto", "hip", "triton") \
+        if append_backend in ("auto", "fused", "hip", "cuda") and attention_backend in ("auto", "hip", "triton") \
                 and not torch.compiler.is_compiling():
+            how = 2 if append_backend == "fused" else 1 if append_backend == "auto" else 0
             out = _hip.native().paged_step(q, self.k_pages, self.v_pages, self.table.tables,
-                                           self.table.lengths, causal, None, new_k, new_v, slots, fuse)
+                                           self.table.lengths, causal, None, new_k, new_v, slots, how)
             if out is not NotImplemented:
                 return out
         if append_backend not in STORE_BACKENDS + ("fused",):
@@ -411,16 +408,17 @@ class PagedKVCache:
         # Every check of the attention comes before the store writes anything.
         scale, on_hip = _attention_route(q, self.k_pages, self.v_pages, self.table.tables,
                                          self.table.lengths, causal, None, attention_backend)
-        if fuse and on_hip and not torch.compiler.is_compiling():
+        if append_backend in ("auto", "fused") and on_hip and not torch.compiler.is_compiling():
             hip_paged.check_append(self.k_pages, self.v_pages, new_k, new_v, slots)
             _no_gradients("paged append", new_k, new_v)
-            if slots.shape[0] == q.shape[0] and hip_paged.step_fuses(self.k_pages, new_k):
+            most = _hip.KF_PAGED_STEP_SLOTS if append_backend == "fused" else hip_paged.FUSED_STEP_ROWS
+            if slots.shape[0] == q.shape[0] and hip_paged.step_fuses(self.k_pages, new_k, most):
                 return hip_paged.append_attention_paged(
                     q, self.k_pages, self.v_pages, new_k, new_v, slots, self.table.tables,
                     self.table.lengths, causal=causal, scale=scale)
         if append_backend == "fused":
             raise ValueError("append_backend='fused' needs HIP attention, up to "
-                             f"{_hip.KF_PAGED_STEP_TOKENS} new tokens per request and a pool of "
-                             "fewer than 2**31 slots")
+                             f"{_hip.KF_PAGED_STEP_TOKENS} new tokens per request, "
+                             f"{_hip.KF_PAGED_STEP_SLOTS} in all, and a pool of fewer than 2**31 slots")
         self.append(new_k, new_v, slots, backend=append_backend)
         return self.attend(q, causal=causal, backend=attention_backend)

@@ -860,3 +860,106 @@ def test_drafts_of_their_own_number(how):
     # The token of the request with one draft sees itself alone, in the last row.
     assert torch.equal(out[1, :, -1], new[1][1, :, -1].repeat_interleave(4, 0))
     assert (out[1, :, :-1] == 0).all()
+
+
+def _step_state(dtype=F16, batch=4, hkv=2, d=64, page=16):
+    """A cache whose requests hold 900, 40, 0 and 333 tokens (and so on), and
+    the tokens that they get next."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = PageTable(batch, 1200, num_pages=80 * batch, page_size=page)
+    cache = PagedKVCache(table, hkv, d, dtype=dtype)
+    cache.k_pages.fill_(math.nan)
+    cache.v_pages.fill_(math.nan)
+    held = [(900, 40, 0, 333)[b % 4] for b in range(batch)]
+    old = torch.randn(2, batch, hkv, 900, d, device="cuda", generator=g).to(dtype)
+    cache.append(*old, table.reserve(_counts(held), width=900))
+    return table, cache, g
+
+
+def _steps_agree(prepare, n, *, how="fused", hq=8, **kw):
+    """A step that stores and attends in one launch, against two launches: the
+    output and both pools to the bit. ``prepare(table, cache)`` gives slots."""
+    got = []
+    for backend in (how, "hip"):
+        table, cache, g = _step_state(**kw)
+        slots = prepare(table, cache)
+        b, hkv, d = table.batch, cache.k_pages.shape[1], cache.k_pages.shape[3]
+        new = torch.randn(2, b, hkv, n, d, device="cuda", generator=g).to(cache.k_pages.dtype)
+        q = torch.randn(b, hq, 1, d, device="cuda", generator=g).to(cache.k_pages.dtype)
+        out = cache.append_and_attend(q, *new, slots, append_backend=backend)
+        got.append((out, cache.k_pages, cache.v_pages))
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    return got[0]
+
+
+@pytest.mark.parametrize("how", ["fused", "auto"])
+@pytest.mark.parametrize("kw", [dict(), dict(dtype=BF16, d=128, page=32), dict(hq=64, hkv=1, d=96, page=48),
+                                dict(hq=80, hkv=1, d=40), dict(hq=20, hkv=1, d=128)])
+def test_a_step_with_a_part_of_the_slots(how, kw):
+    """The first of more slots than the step brings tokens: the new rows are
+    not the requests' last ones, and units in front of the last read them."""
+    def some(first):
+        def prepare(table, cache):
+            slots = table.reserve(80)
+            cache.append(*torch.ones(2, table.batch, cache.k_pages.shape[1], 80, cache.k_pages.shape[3], device="cuda",
+                                     dtype=cache.k_pages.dtype), slots)
+            return slots[:, first:first + 4]
+        return prepare
+
+    for first in (0, 5, 40, 76):
+        _steps_agree(some(first), 4, how=how, **kw)
+
+
+@pytest.mark.parametrize("how", ["fused", "auto"])
+def test_a_step_over_pages_of_several_requests(how):
+    """Requests that hold the same pages all see what one of them stores."""
+    def prepare(table, cache):
+        slots = table.reserve(2)
+        table.tables[1:] = table.tables[0]
+        table.lengths[1:] = table.lengths[0] - torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32)
+        slots[1:] = -1
+        return slots
+
+    out, k, v = _steps_agree(prepare, 2, how=how)
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("how", ["fused", "auto"])
+def test_a_step_whose_rows_nobody_sees(how):
+    """New rows behind the lengths, in pages of no request, and of requests
+    that hold nothing are stored."""
+    def shorter(table, cache):
+        slots = table.reserve(3)
+        table.lengths.copy_(_counts([880, 0, 0, 334]))
+        return slots
+
+    def elsewhere(table, cache):
+        slots = table.reserve(3)
+        spare = int(table.free_pages[0])
+        slots[1] = spare * 16 + torch.tensor([15, 0, 7], device="cuda")
+        slots[2] = -1
+        return slots
+
+    def nothing(table, cache):
+        slots = table.reserve(3)
+        table.lengths.zero_()
+        return slots
+
+    for prepare in (shorter, elsewhere, nothing):
+        _, k, v = _steps_agree(prepare, 3, how=how)
+    assert int(torch.isfinite(k).all(-1).sum()) == 2 * (900 + 40 + 0 + 333 + 4 * 3)
+
+
+def test_a_step_of_many_rows():
+    """Up to 256 new rows are stored by the attention, more in front of it."""
+    for batch, n in ((64, 4), (256, 1), (65, 1), (16, 16)):
+        _steps_agree(lambda table, cache: table.reserve(n), n, batch=batch)
+    table, cache, g = _step_state(batch=86)
+    slots = table.reserve(3)
+    new = torch.randn(2, 86, 2, 3, 64, device="cuda").to(F16)
+    q = torch.randn(86, 4, 1, 64, device="cuda").to(F16)
+    with pytest.raises(ValueError, match="256 in all"):
+        cache.append_and_attend(q, *new, slots, append_backend="fused")
+    assert torch.isnan(cache.k_pages[slots // 16, :, slots % 16]).all()
+    _steps_agree(lambda table, cache: table.reserve(3), 3, batch=86, how="auto")

@@ -104,3 +104,15 @@ def test_append_decode(kw, match):
     _expect(_hip.lib().kf_paged_append_decode(P, P, P, a["nk"], P, a["slots"], P, None, P, P, a["B"], 4, 2, 1, a["n"],
                                               64, a["pages"], a["page"], 4, 4, 1, s, s, s, a["ns"], a["ns"], s, 0.1,
                                               0, 0, P, 1 << 40, None), match)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(B=17, n=16), "256 new tokens in all"), (dict(B=257), "256 new tokens in all"),
+    (dict(Hq=2 ** 23, Hkv=2 ** 23), "too many heads"),
+])
+def test_append_decode_sizes(kw, match):
+    a = dict(n=1, B=2, Hq=4, Hkv=2)
+    a.update(kw)
+    s = _arr(2048, 1024, 64)
+    _expect(_hip.lib().kf_paged_append_decode(P, P, P, P, P, P, P, None, P, P, a["B"], a["Hq"], a["Hkv"], 1, a["n"],
+                                              64, 8, 16, 4, 4, 1, s, s, s, s, s, s, 0.1, 0, 0, P, 1 << 40, None), match)
