@@ -321,10 +321,11 @@ size_t kf_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64
  * Attention of q [B, Hq, Sq, D] over the pages: rows of request b see its
  * positions [0, lengths[b]); with causal != 0 its Sq query tokens are the
  * request's last, and row i sees [0, lengths[b] - Sq + 1 + i). A row that sees
- * nothing gives O = 0 and LSE = -inf; positions whose page number is outside
- * [0, num_pages) are not seen, and lengths count as at most columns *
- * page_size. page_size is a multiple of 16. Two launches; the split of the
- * work follows the device lengths. lse (nullable) is fp32 [B, Hq, Sq].
+ * nothing gives O = 0 and LSE = -inf, one that sees a score of NaN or +inf NaN
+ * in both; positions whose page number is outside [0, num_pages) are not seen,
+ * and lengths count as at most columns * page_size. page_size is a multiple of
+ * 16. Two launches; the split of the work follows the device lengths. lse
+ * (nullable) is fp32 [B, Hq, Sq].
  */
 int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,
                     const int32_t* tables, const int32_t* lengths, int64_t B, int64_t Hq,

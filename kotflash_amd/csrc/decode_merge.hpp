@@ -87,18 +87,19 @@ __device__ inline MergeState merge_splits(__amdgpu_buffer_rsrc_t orr, __amdgpu_b
   return {acc, dtot, M};
 }
 
-// O and LSE of the row, from the lanes of the first SW.
+// O and LSE of the row, from the lanes of the first SW. A part whose LSE is NaN
+// has a NaN weight (the maximum leaves it out), and so makes den, O and LSE NaN.
 template <typename T, int QL>
 __device__ inline void merge_store(const MergeState& m, int D, uint16_t* out_row, float* lse_out) {
   const int lane = threadIdx.x & 63;
   const int q = lane % QL;
   if (lane < QL && 4 * q < D) {
-    const float inv = m.den > 0.f ? 1.f / m.den : 0.f;
+    const float inv = m.den == 0.f ? 0.f : 1.f / m.den;
     u32x2 wv;
     wv[0] = pack2<T>(m.acc[0] * inv, m.acc[1] * inv);
     wv[1] = pack2<T>(m.acc[2] * inv, m.acc[3] * inv);
     *reinterpret_cast<u32x2*>(out_row + 4 * q) = wv;
-    if (q == 0 && lse_out) *lse_out = m.den > 0.f ? (m.M + fast_log2(m.den)) * kLn2 : kNegInf;
+    if (q == 0 && lse_out) *lse_out = m.den == 0.f ? kNegInf : (m.M + fast_log2(m.den)) * kLn2;
   }
 }
 

@@ -637,8 +637,10 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     const int group = w.b * c.heads + w.hh;
     const int r = wave * 16 + l16;
     const float lt = wave_group16_sum(l_i);
-    const float inv = lt > 0.f ? 1.f / lt : 0.f;
-    const float lse = lt > 0.f ? (m_i - PBias<T>::v + fast_log2(lt)) * kLn2 : kNegInf;
+    // A row without keys has lt = 0; one that sees a NaN score, or one of
+    // +infinity, has a NaN lt, and passes it on to its O and LSE.
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float lse = lt == 0.f ? kNegInf : (m_i - PBias<T>::v + fast_log2(lt)) * kLn2;
     // kOOB is the top bit, which no offset inside a resource has.
     const uint32_t none = row.out & kOOB, one_lane = g16 == 0 ? none : kOOB;
     auto beyond = [&](int d) -> uint32_t { return (uint32_t)(c.D - 1 - d) & kOOB; };

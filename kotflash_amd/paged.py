@@ -106,8 +106,9 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
     ``causal`` the Sq query tokens are the request's last ones (draft tokens,
     already stored): row i sees the first ``lengths[b] - Sq + 1 + i``, so a
     request with fewer new tokens than Sq has them in its last rows. A row that
-    sees nothing gives zeros (LSE -inf); a position whose page number is outside
-    the pool is not seen. MHA, GQA and MQA as in ``attention``.
+    sees nothing gives zeros (LSE -inf), one that sees a score of NaN or
+    +infinity NaN (LSE not finite); a position whose page number is outside the
+    pool is not seen. MHA, GQA and MQA as in ``attention``.
 
     ``hip`` needs gfx950, fp16 or bf16, a head_dim that is a multiple of 8 up
     to 128 and a page_size that is a multiple of 16; ``auto`` takes it where

@@ -963,3 +963,29 @@ def test_a_step_of_many_rows():
         cache.append_and_attend(q, *new, slots, append_backend="fused")
     assert torch.isnan(cache.k_pages[slots // 16, :, slots % 16]).all()
     _steps_agree(lambda table, cache: table.reserve(3), 3, batch=86, how="auto")
+
+
+@pytest.mark.parametrize("dtype,d", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("lengths", [[100, 100, 100], [30000, 500, 30000]])
+@pytest.mark.parametrize("sq", [1, 8])
+def test_lse_of_rows_that_see_a_nan(dtype, d, lengths, sq):
+    """A NaN score, or one of +infinity, leaves a row with an LSE that is not
+    finite and not that of an empty row, whether one worker wrote the row or
+    several; the rows of others, and those where the score is -infinity, keep
+    theirs."""
+    q, k, v, tables, lens = make_case(3, 16, 2, sq, d, 16, lengths, dtype=dtype, seed=6, device="cuda")
+    clean, clean_lse = _attend(q, k, v, tables, lens)
+    for at in (0, lengths[0] // 2, lengths[0] - 1):
+        for value in (math.nan, math.inf):
+            bad = k.clone()
+            bad[tables[0, at // 16], 0, at % 16, 3] = value
+            o, lse = _attend(q, bad, v, tables, lens)
+            hit = torch.zeros_like(lse, dtype=torch.bool)
+            hit[0, :8] = True if math.isnan(value) else q[0, :8, :, 3] > 0
+            assert torch.isnan(o[hit]).all()
+            assert (torch.isnan(lse[hit]) | (lse[hit] == math.inf)).all()
+            assert torch.isfinite(o[~hit]).all() and torch.isfinite(lse[~hit]).all()
+            hit[0, :8] = True
+            assert torch.equal(o[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+            want = paged_attention(q[:1], bad, v, tables[:1], lens[:1], return_lse=True, backend="sdpa")
+            assert torch.equal(torch.isfinite(want[1]), torch.isfinite(lse[:1]))
