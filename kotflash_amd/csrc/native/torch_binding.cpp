@@ -623,7 +623,8 @@ PyObject* py_paged_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
   PagedArgs a;
   StoreArgs st;
   if (n != 11 || !PyLong_CheckExact(args[10]) || !a.read(args)) return not_handled();
-  const long how = PyLong_AsLong(args[10]);
+  int over = 0;
+  const long how = PyLong_AsLongAndOverflow(args[10], &over);
   PyObject* const store[] = {args[1], args[2], args[7], args[8], args[9]};
   if (!st.read(store)) return not_handled();
   const int64_t rows = st.nk->size(0) * st.nk->size(2);
@@ -675,8 +676,9 @@ struct TableArgs {
       each = t->const_data_ptr<int32_t>();
     }
     if (!PyLong_CheckExact(a[5])) return false;
-    page = PyLong_AsLongLong(a[5]);
-    return true;
+    int over = 0;
+    page = PyLong_AsLongLongAndOverflow(a[5], &over);
+    return !over;
   }
   // The version counters of what a call has written, as an in-place torch
   // operation moves them. (Tensors made in inference mode have none.)
@@ -692,8 +694,9 @@ PyObject* py_page_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TableArgs t;
   if (n != 7 || !PyLong_CheckExact(args[6]) || !t.read(args)) return not_handled();
-  const int64_t width = PyLong_AsLongLong(args[6]);
-  if (width <= 0 || width >= (1 << 30) || (!t.each && t.all > width)) return not_handled();
+  int over = 0;
+  const int64_t width = PyLong_AsLongLongAndOverflow(args[6], &over);
+  if (over || width <= 0 || width >= (1 << 30) || (!t.each && t.all > width)) return not_handled();
   Tensor slots;
   {
     pybind11::gil_scoped_release nogil;

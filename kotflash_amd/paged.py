@@ -284,6 +284,8 @@ class PageTable:
                 raise ValueError("width is needed with per-request counts")
             width = max(counts, 1)
         width = _positive("width", width)
+        if width >= 2 ** 30:
+            raise ValueError("width must be below 2**30")
         if not isinstance(counts, torch.Tensor) and counts > width:
             raise ValueError("counts must not exceed width")
         state = (self.tables, self.lengths, self.free_pages, self.counters)

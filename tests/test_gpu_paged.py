@@ -989,3 +989,11 @@ def test_lse_of_rows_that_see_a_nan(dtype, d, lengths, sq):
             assert torch.equal(o[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
             want = paged_attention(q[:1], bad, v, tables[:1], lens[:1], return_lse=True, backend="sdpa")
             assert torch.equal(torch.isfinite(want[1]), torch.isfinite(lse[:1]))
+
+
+def test_reserve_refuses_a_width_beyond_64_bits():
+    table = PageTable(2, 64, num_pages=8)
+    for width in (2 ** 64, 2 ** 63, 2 ** 40, 2 ** 30, -2 ** 64):
+        with pytest.raises(ValueError, match="width"):
+            table.reserve(1, width=width)
+    assert table.lengths.tolist() == [0, 0] and table.num_free() == 8

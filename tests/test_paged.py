@@ -276,3 +276,11 @@ def test_fused_needs_the_kernels():
     with pytest.raises(ValueError, match="fused"):
         cache.append_and_attend(torch.ones(3, 4, 1, 8), new, new, table.reserve(1), append_backend="fused")
     assert (cache.k_pages == 0).all()
+
+
+def test_reserve_refuses_a_width_beyond_30_bits():
+    table = _table()
+    for width in (2 ** 64, 2 ** 63, 2 ** 30, -2 ** 64):
+        with pytest.raises(ValueError, match="width"):
+            table.reserve(1, width=width)
+    assert table.lengths.tolist() == [0, 0, 0] and table.num_free() == 8
