@@ -95,11 +95,12 @@ __device__ inline Demand demand(const TableParams& p, int b) {
 }
 
 // Slot of position pos of a request whose pages from `first` on lie on the
-// stack from `top` down.
+// stack from `top` down; -1 for a page outside the pool, which only a state that
+// was written from outside can name.
 __device__ inline int64_t slot_of(const TableParams& p, const int32_t* table, int pos, int first, int top) {
   const int col = quotient(pos, p.page);
   const int id = col < first ? table[col] : p.free_pages[top - (col - first)];
-  return id < 0 ? -1 : (int64_t)id * p.page.d + (pos - col * (int)p.page.d);
+  return (uint32_t)id >= (uint32_t)p.pages ? -1 : (int64_t)id * p.page.d + (pos - col * (int)p.page.d);
 }
 
 // The request, of m, that item k belongs to: the last whose first item is not

@@ -319,10 +319,17 @@ class PageTable:
             _trim(*state, lengths, self.page_size)
 
 
+def _bounded(tables, lengths, free_pages, counters, page: int):
+    """The stack's height and the requests' lengths as far as they can be true,
+    as the kernels bound them."""
+    return (counters[0].long().clamp(0, free_pages.numel()),
+            lengths.long().clamp(0, tables.shape[1] * page))
+
+
 def _reserve(tables, lengths, free_pages, counters, counts, width: int, page: int) -> torch.Tensor:
     """``PageTable.reserve`` in torch operations."""
-    columns, height = tables.shape[1], counters[0].long()
-    held = lengths.long()
+    columns = tables.shape[1]
+    height, held = _bounded(tables, lengths, free_pages, counters, page)
     counts = torch.as_tensor(counts, device=tables.device).long().expand_as(held)
     first = (held + page - 1) // page
     fits = (counts >= 0) & (counts <= width) & (held + counts <= columns * page)
@@ -338,9 +345,9 @@ def _reserve(tables, lengths, free_pages, counters, counts, width: int, page: in
     t = torch.arange(width, device=tables.device)
     position = held[:, None] + t
     ids = tables.long().gather(1, (position // page).clamp(max=columns - 1))
-    given = served[:, None] & (t < counts[:, None]) & (ids >= 0)
+    given = served[:, None] & (t < counts[:, None]) & (ids >= 0) & (ids < free_pages.numel())
     slots = torch.where(given, ids * page + position % page, -1)
-    lengths.copy_(held + torch.where(served, counts, 0))
+    lengths.copy_(torch.where(served, held + counts, lengths))
     counters[0] = height - need.sum()
     counters[1] = (~served).sum()
     return slots
@@ -348,17 +355,18 @@ def _reserve(tables, lengths, free_pages, counters, counts, width: int, page: in
 
 def _trim(tables, lengths, free_pages, counters, new_lengths, page: int) -> None:
     """``PageTable.trim`` in torch operations."""
-    height, held = counters[0].long(), lengths.long()
+    height, held = _bounded(tables, lengths, free_pages, counters, page)
     keep = torch.as_tensor(new_lengths, device=tables.device).long().clamp(min=0).minimum(held)
     first, end = (keep + page - 1) // page, (held + page - 1) // page
     freed = end - first
     column = torch.arange(tables.shape[1], device=tables.device)
     gone = (column >= first[:, None]) & (column < end[:, None])
     place = height + freed.sum() - 1 - (freed.cumsum(0) - freed)[:, None] - (column - first[:, None])
-    free_pages[place[gone]] = tables[gone]
+    back = gone & (place < free_pages.numel())
+    free_pages[place[back]] = tables[back]
     tables.masked_fill_(gone, -1)
     lengths.copy_(keep)
-    counters[0] = height + freed.sum()
+    counters[0] = (height + freed.sum()).clamp(max=free_pages.numel())
 
 
 class PagedKVCache:

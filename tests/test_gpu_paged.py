@@ -997,3 +997,34 @@ def test_reserve_refuses_a_width_beyond_64_bits():
         with pytest.raises(ValueError, match="width"):
             table.reserve(1, width=width)
     assert table.lengths.tolist() == [0, 0] and table.num_free() == 8
+
+
+def test_slots_of_a_broken_state_name_places_of_the_pool():
+    """Page numbers outside the pool, in tables and on the stack, give -1."""
+    for width, counts in ((20, 20), (1, 1), (1500, 40)):
+        for entry in (-1, 7, 8, 9, 2 ** 31 - 1, -2 ** 31):
+            table = PageTable(4, 1600, num_pages=8, page_size=16)
+            table.tables.fill_(entry)
+            table.free_pages[::2] = entry
+            table.lengths.copy_(_counts([5, 16, 0, 31]))
+            slots = table.reserve(counts, width=width)
+            assert ((slots >= -1) & (slots < 8 * 16)).all(), (width, entry)
+            assert (slots[0, 0] == 7 * 16 + 5) if entry == 7 else (slots[0, 0] == -1)
+
+
+def test_torch_and_hip_tables_agree_on_broken_states():
+    for height, length, entry in ((10 ** 9, 5, 3), (-4, 10 ** 9, -1), (2, -50, 10 ** 9), (8, 2 ** 31 - 1, -2 ** 31)):
+        tables = [PageTable(4, 96, num_pages=8, page_size=16) for _ in range(2)]
+        for t in tables:
+            t.tables.fill_(entry)
+            t.lengths.copy_(_counts([length, 7, 96, length]))
+            t.free_count.fill_(height)
+        for _ in range(3):
+            slots = [t.reserve(20, backend=b) for t, b in zip(tables, ("hip", "torch"))]
+            assert torch.equal(*slots)
+            for name in ("tables", "lengths", "free_pages", "counters"):
+                assert torch.equal(getattr(tables[0], name), getattr(tables[1], name)), name
+            for t, b in zip(tables, ("hip", "torch")):
+                t.trim(3, backend=b)
+            for name in ("tables", "lengths", "free_pages", "counters"):
+                assert torch.equal(getattr(tables[0], name), getattr(tables[1], name)), name

@@ -284,3 +284,20 @@ def test_reserve_refuses_a_width_beyond_30_bits():
         with pytest.raises(ValueError, match="width"):
             table.reserve(1, width=width)
     assert table.lengths.tolist() == [0, 0, 0] and table.num_free() == 8
+
+
+def test_broken_state_stays_inside():
+    """Lengths, tables, counts and stacks that no allocator leaves behind: slots
+    name places of the pool or -1, and a refused request is left as it was."""
+    for height, length, entry in ((10 ** 9, 5, 3), (-4, 10 ** 9, -1), (2, -50, 10 ** 9), (8, 2 ** 31 - 1, -2 ** 31)):
+        table = _table(4, 96, 8)
+        table.tables.fill_(entry)
+        table.free_pages[::2] = entry
+        table.lengths.fill_(length)
+        table.free_count.fill_(height)
+        slots = table.reserve(20)
+        assert ((slots >= -1) & (slots < 8 * 16)).all()
+        if length > 96:
+            assert (table.lengths == length).all() and int(table.refused) == 4
+        table.trim(3)
+        assert 0 <= table.num_free() <= 8 and (table.lengths <= 3).all() and (table.lengths >= 0).all()
