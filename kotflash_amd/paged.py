@@ -29,6 +29,7 @@ import math
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 from .attention import _sdpa
@@ -47,7 +48,9 @@ def _on_gfx950(t: torch.Tensor) -> bool:
 
 
 def _no_gradients(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+            or not torch.compiler.is_compiling()
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
         raise RuntimeError(f"{what} is inference-only; disable gradients")
 
 

@@ -1028,3 +1028,26 @@ def test_torch_and_hip_tables_agree_on_broken_states():
                 t.trim(3, backend=b)
             for name in ("tables", "lengths", "free_pages", "counters"):
                 assert torch.equal(getattr(tables[0], name), getattr(tables[1], name)), name
+
+
+def test_forward_mode_gradients_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    q, k, v, tables, lengths = make_case(2, 4, 2, 1, 64, 16, [30, 50], dtype=F16, seed=4, device="cuda", junk=0.0)
+    table = PageTable(2, 64, num_pages=k.shape[0])
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.zero_()
+    slots = table.reserve(1)
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=F16)
+    with fwd.dual_level():
+        dual = [fwd.make_dual(t, torch.ones_like(t)) for t in (q, k, new)]
+        for call in (lambda: paged_attention(dual[0], k, v, tables, lengths),
+                     lambda: paged_attention(q, dual[1], v, tables, lengths, backend="sdpa"),
+                     lambda: cache.append(dual[2], new, slots),
+                     lambda: cache.append(dual[2], new, slots, backend="torch"),
+                     lambda: cache.append_and_attend(q, new, dual[2], slots),
+                     lambda: cache.append_and_attend(dual[0], new, new, slots, append_backend="hip")):
+            with pytest.raises(RuntimeError, match="inference-only"):
+                call()
+        assert (cache.k_pages == 0).all()
+    cache.append_and_attend(q, new, new, slots)

@@ -301,3 +301,27 @@ def test_broken_state_stays_inside():
             assert (table.lengths == length).all() and int(table.refused) == 4
         table.trim(3)
         assert 0 <= table.num_free() <= 8 and (table.lengths <= 3).all() and (table.lengths >= 0).all()
+
+
+def test_forward_mode_gradients_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    args = _attention_args()
+    table = _table()
+    cache = PagedKVCache(table, 2, 8, dtype=F32)
+    cache.k_pages.zero_()
+    cache.v_pages.zero_()
+    slots, new = table.reserve(1), torch.ones(3, 2, 1, 8)
+    with fwd.dual_level():
+        dual = fwd.make_dual(new, torch.ones_like(new))
+        for name in ("q", "k_pages", "v_pages"):
+            with pytest.raises(RuntimeError, match="inference-only"):
+                paged_attention(**dict(args, **{name: fwd.make_dual(args[name], torch.ones_like(args[name]))}))
+        for k, v in ((dual, new), (new, dual)):
+            for call in (cache.append, lambda *a: cache.append_and_attend(torch.ones(3, 4, 1, 8), *a)):
+                with pytest.raises(RuntimeError, match="inference-only"):
+                    call(k, v, slots)
+        assert (cache.k_pages == 0).all() and (cache.v_pages == 0).all()
+        paged_attention(**args)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        torch.func.jvp(lambda q: paged_attention(**dict(args, q=q)), (args["q"],), (args["q"],))
