@@ -476,6 +476,13 @@ PyObject* py_store_lengths(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // Paged cache. A page table's state: tables int32 [B, columns] with a unit
 // column stride, lengths [B], free_pages [pages] and counters [4], contiguous.
 
+// Moves the version counters of what a call has written, as an in-place torch
+// operation does. (Tensors made in inference mode have none.)
+void written(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 bool int32_on(const Tensor* t, const c10::Device& dev) {
   return t && t->scalar_type() == at::kInt && t->device() == dev;
 }
@@ -607,6 +614,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const c10::OptionalDeviceGuard guard(a.k->device());
     launch_store(a);
   }
+  written({a.k, a.v});
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -639,6 +647,7 @@ PyObject* py_paged_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!fuse) launch_store(st);
     out = launch_paged(a, nullptr, fuse ? &st : nullptr);
   }
+  written({st.k, st.v});
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -680,12 +689,6 @@ struct TableArgs {
     page = PyLong_AsLongLongAndOverflow(a[5], &over);
     return !over;
   }
-  // The version counters of what a call has written, as an in-place torch
-  // operation moves them. (Tensors made in inference mode have none.)
-  void written() const {
-    for (const Tensor* t : {tables, lengths, free_pages, counters})
-      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-  }
 };
 
 // page_reserve(tables, lengths, free_pages, counters, counts, page_size,
@@ -708,7 +711,7 @@ PyObject* py_page_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           t.tables->stride(0), t.page, t.free_pages->size(0), stream_of(*t.tables)),
           "kf_page_reserve");
   }
-  t.written();
+  written({t.tables, t.lengths, t.counters});
   return THPVariable_Wrap(std::move(slots));
   END_HANDLE_TH_ERRORS
 }
@@ -727,7 +730,7 @@ PyObject* py_page_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
                        t.free_pages->size(0), stream_of(*t.tables)),
           "kf_page_trim");
   }
-  t.written();
+  written({t.tables, t.lengths, t.free_pages, t.counters});
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -103,6 +103,11 @@ def require_readable(q, k_pages, v_pages) -> None:
                          "inner-contiguous, 16-byte aligned K/V pages")
 
 
+def _written(*tensors) -> None:
+    """Moves the tensors' version counters, as an in-place torch operation does."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def attention_paged(q, k_pages, v_pages, tables, lengths, *, causal: bool, scale: float,
                     with_lse: bool = False):
     """O (and LSE) of q over the pages (``kf_paged_decode``); the arguments
@@ -148,6 +153,7 @@ def append_attention_paged(q, k_pages, v_pages, new_k, new_v, slots, tables, len
     ws = _hip.workspace(q.device, _hip.paged_decode_workspace_bytes(b, hq, k_pages.shape[1], sq, d))
     _hip.paged_append_decode(q, k_pages, v_pages, new_k, new_v, slots, out, None, tables, lengths,
                              scale=scale, causal=causal, workspace=ws)
+    _written(k_pages, v_pages)
     return out
 
 
@@ -160,6 +166,7 @@ def append_paged(k_pages, v_pages, new_k, new_v, slots) -> None:
     if slots.stride(1) != 1:
         slots = slots.contiguous()
     _hip.paged_append(k_pages, v_pages, new_k, new_v, slots)
+    _written(k_pages, v_pages)
 
 
 def check_table(tables, lengths, free_pages, counters) -> None:
@@ -193,6 +200,7 @@ def reserve_pages(tables, lengths, free_pages, counters, counts: Union[int, torc
     counts = _per_request("counts", counts, tables)
     slots = torch.empty((tables.shape[0], width), device=tables.device, dtype=torch.int64)
     _hip.page_reserve(tables, lengths, free_pages, counters, counts, slots, page_size=page_size)
+    _written(tables, lengths, counters)
     return slots
 
 
@@ -202,3 +210,4 @@ def trim_pages(tables, lengths, free_pages, counters, new_lengths: Union[int, to
     check_table(tables, lengths, free_pages, counters)
     new_lengths = _per_request("new_lengths", new_lengths, tables)
     _hip.page_trim(tables, lengths, free_pages, counters, new_lengths, page_size=page_size)
+    _written(tables, lengths, free_pages, counters)

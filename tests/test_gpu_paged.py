@@ -1051,3 +1051,32 @@ def test_forward_mode_gradients_are_refused():
                 call()
         assert (cache.k_pages == 0).all()
     cache.append_and_attend(q, new, new, slots)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_what_is_written_changes_its_version(native, monkeypatch):
+    """Autograd sees stores and table calls as it sees in-place operations."""
+    if not native:
+        monkeypatch.setattr(_hip, "_NATIVE", _hip._NoNative())
+    table = PageTable(2, 64, num_pages=8)
+    cache = PagedKVCache(table, 2, 64, dtype=F16)
+    cache.k_pages.zero_()
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=F16)
+    q = torch.ones(2, 4, 1, 64, device="cuda", dtype=F16)
+    x = torch.ones(64, device="cuda", dtype=F16, requires_grad=True)
+    slots = table.reserve(1)
+
+    def moves(tensors, call):
+        before = [t._version for t in tensors]
+        call()
+        return all(t._version > v for t, v in zip(tensors, before))
+
+    pools, state = (cache.k_pages, cache.v_pages), (table.tables, table.lengths, table.counters)
+    assert moves(pools, lambda: cache.append(new, new, slots))
+    for how in ("fused", "hip", "torch"):
+        assert moves(pools, lambda: cache.append_and_attend(q, new, new, slots, append_backend=how))
+    assert moves(state, lambda: table.reserve(1)) and moves(state + (table.free_pages,), lambda: table.trim(0))
+    product = (cache.k_pages[0, 0, 0] * x).sum()
+    cache.append(new, new, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
