@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define KF_ABI_VERSION 8
+#define KF_ABI_VERSION 9
 
 enum kf_status {
   KF_OK = 0,
@@ -316,6 +316,16 @@ int kf_paged_append(void* k_pages, void* v_pages, const void* new_k, const void*
 
 /* Workspace for kf_paged_decode in bytes (fp32 partial O and LSE). */
 size_t kf_paged_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);
+
+/*
+ * Whether the sizes are within what kf_paged_decode addresses (32-bit step,
+ * row and byte numbers; lengths count as what the tables can hold): KF_OK, or
+ * the code that it would return, with o contiguous. Host only.
+ */
+int kf_paged_decode_check(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                          int64_t num_pages, int64_t page_size, int64_t columns,
+                          const int64_t* q_strides, const int64_t* k_strides,
+                          const int64_t* v_strides);
 
 /*
  * Attention of q [B, Hq, Sq, D] over the pages: rows of request b see its

@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libkotflash_amd.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 KF_F16, KF_BF16 = 0, 1
 KF_PAGED_STEP_TOKENS, KF_PAGED_STEP_SLOTS = 16, 256
 KF_BWD_DELTA, KF_BWD_DQ, KF_BWD_DKDV, KF_BWD_DKDV_FIXUP = 1, 2, 4, 8
@@ -65,6 +65,7 @@ _SIGNATURES = {
     "kf_paged_append": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                              _I64P, _I64P, _I64P, _I64P, _I, _P]),
     "kf_paged_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64]),
+    "kf_paged_decode_check": (_I, [_I64] * 8 + [_I64P] * 3),
     "kf_paged_decode": (_I, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                              _I64, _I64, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _SZ, _P]),
     "kf_paged_append_decode": (_I, [_P] * 10 + [_I64] * 11 + [_I64P] * 6
@@ -455,6 +456,16 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots) -> None:
 @lru_cache(maxsize=256)
 def paged_decode_workspace_bytes(b, hq, hkv, sq, d) -> int:
     return int(lib().kf_paged_decode_workspace_bytes(b, hq, hkv, sq, d))
+
+
+def paged_decode_check(q, k_pages, v_pages, columns: int) -> int:
+    """kf_paged_decode_check for tensors that the launcher reads in place (q
+    made contiguous if it does not): 0, or an error for ``_check``."""
+    b, hq, sq, d = q.shape
+    num_pages, hkv, page_size, _ = k_pages.shape
+    q_strides = _strides(q) if layout_ok(q) else _I64x4(hq * sq * d, sq * d, d, 1)
+    return lib().kf_paged_decode_check(b, hq, hkv, sq, d, num_pages, page_size, columns, q_strides,
+                                       _strides(k_pages), _strides(v_pages))
 
 
 def paged_decode(q, k_pages, v_pages, out, lse: Optional[torch.Tensor], tables, lengths, *,

@@ -518,7 +518,15 @@ struct PagedArgs {
     if (a[6] == Py_None) scale = 1.0 / std::sqrt((double)q->size(3));
     else if (PyFloat_CheckExact(a[6])) scale = PyFloat_AS_DOUBLE(a[6]);
     else return false;
-    return std::isfinite(scale);
+    return std::isfinite(scale) && sizes_ok();
+  }
+  // Sizes beyond the kernels' are refused, or run elsewhere, above.
+  bool sizes_ok() const {
+    const int64_t b = q->size(0), hq = q->size(1), sq = q->size(2), d = q->size(3);
+    const int64_t dense[3] = {hq * sq * d, sq * d, d};
+    return kf_paged_decode_check(b, hq, k->size(1), sq, d, k->size(0), k->size(2), tables->size(1),
+                                 layout_ok(*q) ? q->strides().data() : dense, k->strides().data(),
+                                 v->strides().data()) == KF_OK;
   }
 };
 

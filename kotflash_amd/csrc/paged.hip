@@ -816,7 +816,7 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)rows);
   if (most > 16 * kTrip && rows <= 256)
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 16>), grid, dim3(1024), 0, stream, p);
-  else if (most > kTrip && (rows <= 256 || (most > 8 * kTrip && rows <= 2048) || most > 32 * kTrip))
+  else if (most > kTrip && (rows <= 256 || (most > 8 * kTrip && rows <= 2048) || (most > 32 * kTrip && rows < 1 << 24)))
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 4>), grid, dim3(256), 0, stream, p);
   else
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
@@ -868,6 +868,43 @@ struct NewRows {
   const int64_t *k_strides, *v_strides;
 };
 
+// Rows that the merge's launch takes at one wave each: HIP counts a grid's threads
+// in 32 bits.
+constexpr int64_t kMergeRows = (1ll << 32) / 64 - 4;
+
+// Extent of one KV head's queries or outputs.
+static int64_t group_bytes(int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, const int64_t* strides) {
+  return ((Hq / Hkv - 1) * strides[1] + (Sq - 1) * strides[2] + D) * 2;
+}
+
+// The sizes and strides that the kernels address.
+static int check_paged_sizes(const char* what, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                             int64_t num_pages, int64_t page_size, int64_t columns, const int64_t* q_strides,
+                             const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides) {
+  if (num_pages <= 0 || columns <= 0 || num_pages > 0x7fffffff)
+    return set_error(KF_EINVAL, "%s: num_pages and table columns must be positive", what);
+  if (page_size <= 0 || page_size % 16 != 0)
+    return set_error(KF_EUNSUPPORTED, "%s: page_size must be a multiple of 16, got %lld", what, (long long)page_size);
+  if (page_size > 0x3fffffff / columns)
+    return set_error(KF_EUNSUPPORTED, "%s: a table of %lld pages of %lld tokens is beyond 32-bit positions", what,
+                     (long long)columns, (long long)page_size);
+  const int64_t R = Hq / Hkv * Sq;
+  if (R > 0x3fffffff) return set_error(KF_EUNSUPPORTED, "%s: too many query rows", what);
+  const int rows = paged_rows(R);
+  const int64_t nrb = (R + rows - 1) / rows, heads = Hkv * nrb;
+  const int64_t cap = columns * page_size;
+  if (heads * ((cap + kStep - 1) / kStep) > 0x7f000000 / B)
+    return set_error(KF_EUNSUPPORTED, "%s: %lld tables of %lld tokens are beyond 32-bit step numbers", what,
+                     (long long)B, (long long)cap);
+  if (B * heads * rows > kMergeRows) return set_error(KF_EUNSUPPORTED, "%s: grid too large", what);
+  if (group_bytes(Hq, Hkv, Sq, D, q_strides) > 0x7fffffff || group_bytes(Hq, Hkv, Sq, D, o_strides) > 0x7fffffff)
+    return set_error(KF_EUNSUPPORTED, "%s: one KV group of q or o spans more than 2 GiB", what);
+  for (const int64_t* st : {k_strides, v_strides})
+    if ((15 * st[2] + D) * 2 > 0x7fffffffLL || st[0] > 0x7fffffffLL)
+      return set_error(KF_EUNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB, or a page more than 4", what);
+  return KF_OK;
+}
+
 static int paged_entry(const char* what, const void* q, const void* k_pages, const void* v_pages,
                        const NewRows& fresh, void* o, float* lse, const int32_t* tables, const int32_t* lengths,
                        int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t num_pages,
@@ -882,35 +919,19 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
   if (tables == nullptr || lengths == nullptr)
     return set_error(KF_EINVAL, "%s: tables and lengths must be non-null", what);
   if (!(scale == scale) || scale - scale != 0.f) return set_error(KF_EINVAL, "%s: scale must be finite", what);
-  if (num_pages <= 0 || columns <= 0 || num_pages > 0x7fffffff)
-    return set_error(KF_EINVAL, "%s: num_pages and table columns must be positive", what);
-  if (page_size <= 0 || page_size % 16 != 0)
-    return set_error(KF_EUNSUPPORTED, "%s: page_size must be a multiple of 16, got %lld", what, (long long)page_size);
   if (columns > 1 && table_stride < 0) return set_error(KF_EINVAL, "%s: negative table stride", what);
-  if (page_size > 0x3fffffff / columns)
-    return set_error(KF_EUNSUPPORTED, "%s: a table of %lld pages of %lld tokens is beyond 32-bit positions", what,
-                     (long long)columns, (long long)page_size);
-  const int64_t R = Hq / Hkv * Sq;
-  if (R > 0x3fffffff) return set_error(KF_EUNSUPPORTED, "%s: too many query rows", what);
-  const int rows = paged_rows(R);
-  const int64_t nrb = (R + rows - 1) / rows, heads = Hkv * nrb;
-  const int64_t cap = columns * page_size;
-  if (heads * ((cap + kStep - 1) / kStep) > 0x7f000000 / B)
-    return set_error(KF_EUNSUPPORTED, "%s: %lld tables of %lld tokens are beyond 32-bit step numbers", what,
-                     (long long)B, (long long)cap);
-  if (B * heads * rows > 0x7fffffff) return set_error(KF_EUNSUPPORTED, "%s: grid too large", what);
-  const int64_t q_bytes = ((Hq / Hkv - 1) * q_strides[1] + (Sq - 1) * q_strides[2] + D) * 2;
-  const int64_t o_bytes = ((Hq / Hkv - 1) * o_strides[1] + (Sq - 1) * o_strides[2] + D) * 2;
-  if (q_bytes > 0x7fffffff || o_bytes > 0x7fffffff)
-    return set_error(KF_EUNSUPPORTED, "%s: one KV group of q or o spans more than 2 GiB", what);
-  for (const int64_t* st : {k_strides, v_strides})
-    if ((15 * st[2] + D) * 2 > 0x7fffffffLL || st[0] > 0x7fffffffLL)
-      return set_error(KF_EUNSUPPORTED, "%s: 16 rows of a page span more than 2 GiB, or a page more than 4", what);
+  if ((rc = check_paged_sizes(what, B, Hq, Hkv, Sq, D, num_pages, page_size, columns, q_strides, k_strides, v_strides,
+                              o_strides)))
+    return rc;
   const size_t need = kf_paged_decode_workspace_bytes(B, Hq, Hkv, Sq, D);
   if (workspace == nullptr || workspace_bytes < need)
     return set_error(KF_EINVAL, "%s: workspace of %zu bytes required, got %zu", what, need,
                      workspace == nullptr ? (size_t)0 : workspace_bytes);
   if (!aligned16(workspace)) return set_error(KF_EINVAL, "%s: workspace must be 16-byte aligned", what);
+  const int64_t R = Hq / Hkv * Sq, cap = columns * page_size;
+  const int rows = paged_rows(R);
+  const int64_t nrb = (R + rows - 1) / rows, heads = Hkv * nrb;
+  const int64_t q_bytes = group_bytes(Hq, Hkv, Sq, D, q_strides), o_bytes = group_bytes(Hq, Hkv, Sq, D, o_strides);
   PagedParams p{};
   p.q = (const uint16_t*)q; p.k = (const uint16_t*)k_pages; p.v = (const uint16_t*)v_pages;
   p.o = (uint16_t*)o; p.lse = lse; p.tables = tables; p.lengths = lengths;
@@ -945,6 +966,18 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
   }
   hipStream_t s = (hipStream_t)stream;
   return dtype == KF_F16 ? dispatch_paged<_Float16>(p, s) : dispatch_paged<__bf16>(p, s);
+}
+
+extern "C" int kf_paged_decode_check(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t num_pages,
+                                     int64_t page_size, int64_t columns, const int64_t* q_strides,
+                                     const int64_t* k_strides, const int64_t* v_strides) {
+  const char* what = "kf_paged_decode";
+  const int rc = check_attn_common(what, B, Hq, Hkv, Sq, 1, D, KF_F16);
+  if (rc) return rc;
+  if (!q_strides || !k_strides || !v_strides) return set_error(KF_EINVAL, "%s: null strides", what);
+  const int64_t o_strides[3] = {Hq * Sq * D, Sq * D, D};
+  return check_paged_sizes(what, B, Hq, Hkv, Sq, D, num_pages, page_size, columns, q_strides, k_strides, v_strides,
+                           o_strides);
 }
 
 extern "C" int kf_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, float* lse,

@@ -94,13 +94,21 @@ def pages_readable(k_pages, v_pages) -> bool:
             and _hip.layout_ok(k_pages) and _hip.layout_ok(v_pages))
 
 
-def require_readable(q, k_pages, v_pages) -> None:
+def sizes_ok(q, k_pages, v_pages, tables) -> bool:
+    """Whether the decode kernel addresses these sizes (pools that pass
+    ``pages_readable``). Under torch.compile it is left to the call."""
+    return torch.compiler.is_compiling() or _hip.paged_decode_check(q, k_pages, v_pages, tables.shape[1]) == 0
+
+
+def require_readable(q, k_pages, v_pages, tables) -> None:
     require_hip_tensors("paged attention", q, k_pages, v_pages)
     if k_pages.shape[2] % PAGE_GRANULE:
         raise ValueError(f"paged attention needs a page_size that is a multiple of {PAGE_GRANULE}")
     if not pages_readable(k_pages, v_pages):
         raise ValueError("paged attention needs head_dim a multiple of 8 in [8, 128] and "
                          "inner-contiguous, 16-byte aligned K/V pages")
+    if not torch.compiler.is_compiling():
+        _hip._check(_hip.paged_decode_check(q, k_pages, v_pages, tables.shape[1]), "kf_paged_decode")
 
 
 def _written(*tensors) -> None:

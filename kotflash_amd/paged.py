@@ -114,7 +114,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
     pool is not seen. MHA, GQA and MQA as in ``attention``.
 
     ``hip`` needs gfx950, fp16 or bf16, a head_dim that is a multiple of 8 up
-    to 128 and a page_size that is a multiple of 16; ``auto`` takes it where
+    to 128, a page_size that is a multiple of 16 and tables of fewer than 2**31
+    steps of 32 positions, over all requests and KV heads; ``auto`` takes it where
     these hold and ``sdpa`` (one call per request, lengths on the host)
     elsewhere. With ``return_lse``, returns (O, LSE), LSE in fp32 [B, Hq, Sq].
     """
@@ -157,10 +158,11 @@ def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backen
         return scale, False
     if backend == "auto":
         return scale, (_on_gfx950(q) and q.dtype in _HALF
-                       and hip_paged.pages_readable(k_pages, v_pages))
+                       and hip_paged.pages_readable(k_pages, v_pages)
+                       and hip_paged.sizes_ok(q, k_pages, v_pages, tables))
     if not _on_gfx950(q):
         raise RuntimeError("HIP backend requires an AMD MI355X (gfx950) GPU")
-    hip_paged.require_readable(q, k_pages, v_pages)
+    hip_paged.require_readable(q, k_pages, v_pages, tables)
     return scale, True
 
 

@@ -1080,3 +1080,43 @@ def test_what_is_written_changes_its_version(native, monkeypatch):
     cache.append(new, new, slots)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         product.backward()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_sizes_beyond_the_kernels(native, monkeypatch):
+    """Tables whose steps pass 32-bit numbers: auto takes sdpa, hip refuses, a
+    step before it stores anything."""
+    if not native:
+        monkeypatch.setattr(_hip, "_NATIVE", _hip._NoNative())
+    b, hkv, page, d = 16, 8, 2 ** 20, 8
+    k = torch.zeros(2, hkv, page, d, dtype=F16, device="cuda")
+    v = torch.zeros_like(k)
+    g = torch.Generator().manual_seed(3)
+    few = torch.randn(2, hkv, 40, d, generator=g).to(F16)
+    k[1, :, :40], v[1, :, :40] = few[0].cuda(), few[1].cuda()
+    tables = torch.full((b, 512), -1, dtype=torch.int32, device="cuda")
+    tables[:, 0] = 1
+    lengths = (torch.arange(b, dtype=torch.int32) * 2 + 1).cuda()
+    q = torch.randn(b, hkv, 1, d, generator=g).to(F16).cuda()
+    o, lse = paged_attention(q, k, v, tables, lengths, return_lse=True)
+    small = torch.zeros(b, 1, dtype=torch.int32)
+    assert_attention(o, q, few[0][None], few[1][None], small, lengths, lse=lse)
+    with pytest.raises(RuntimeError, match="32-bit step numbers"):
+        paged_attention(q, k, v, tables, lengths, backend="hip")
+    table = PageTable(b, 64, num_pages=2)
+    cache = PagedKVCache(table, hkv, d, dtype=F16)
+    cache.k_pages, cache.v_pages = k, v
+    table.tables, table.lengths = tables, lengths
+    new = torch.ones(b, hkv, 1, d, dtype=F16, device="cuda")
+    slots = torch.arange(b, device="cuda")[:, None] + 50
+    for how in ("hip", "auto", "fused"):
+        with pytest.raises(RuntimeError, match="32-bit step numbers"):
+            cache.append_and_attend(q, new, new, slots, append_backend=how, attention_backend="hip")
+    assert (k[0, :, :100] == 0).all()
+    with pytest.raises(ValueError, match="fused"):
+        cache.append_and_attend(q, new, new, slots, append_backend="fused")
+    assert (k[0, :, :100] == 0).all()
+    out = cache.append_and_attend(q, new, new, slots)
+    assert torch.equal(out, o) and (k[0, :, 50:50 + b] == 1).all() and int((k[0] != 0).sum()) == b * hkv * d
+    del k, v, cache
+    torch.cuda.empty_cache()

@@ -116,3 +116,23 @@ def test_append_decode_sizes(kw, match):
     s = _arr(2048, 1024, 64)
     _expect(_hip.lib().kf_paged_append_decode(P, P, P, P, P, P, P, None, P, P, a["B"], a["Hq"], a["Hkv"], 1, a["n"],
                                               64, 8, 16, 4, 4, 1, s, s, s, s, s, s, 0.1, 0, 0, P, 1 << 40, None), match)
+
+
+@pytest.mark.parametrize("kw,match", [
+    ({}, None), (dict(B=0), "positive"), (dict(D=76), "multiple of 8"), (dict(page=24), "multiple of 16"),
+    (dict(pages=0), "num_pages"), (dict(columns=0), "columns"), (dict(columns=2 ** 27), "32-bit positions"),
+    (dict(B=16, columns=2 ** 25), None), (dict(B=64, columns=2 ** 25), "step numbers"), (dict(qs=None), "strides"),
+    (dict(B=63, columns=2 ** 25), None), (dict(Sq=2 ** 20, Hkv=1), None), (dict(Sq=2 ** 24, Hkv=1), "grid"),
+    (dict(ks=_arr(2 ** 31, 1024, 64)), "page more than 4"), (dict(qs=_arr(512, 2 ** 31, 64)), "2 GiB"),
+    (dict(B=1, Hq=1, Hkv=1, Sq=2 ** 24, D=128, qs=_arr(64, 64, 64)), "2 GiB"),
+])
+def test_decode_check(kw, match):
+    """The host's own answer, before any tensor is made."""
+    a = dict(B=2, Hq=4, Hkv=2, Sq=1, D=64, pages=8, page=16, columns=4, qs=_arr(256, 64, 64), ks=_arr(2048, 1024, 64))
+    a.update(kw)
+    rc = _hip.lib().kf_paged_decode_check(a["B"], a["Hq"], a["Hkv"], a["Sq"], a["D"], a["pages"], a["page"],
+                                          a["columns"], a["qs"], a["ks"], _arr(2048, 1024, 64))
+    if match is None:
+        assert rc == 0, _hip.lib().kf_last_error()
+    else:
+        _expect(rc, match)
