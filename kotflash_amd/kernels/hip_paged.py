@@ -91,7 +91,15 @@ def pages_readable(k_pages, v_pages) -> bool:
     """Whether the decode kernel reads these pools in place."""
     return (k_pages.shape[2] % PAGE_GRANULE == 0 and k_pages.shape[3] % 8 == 0
             and gfx950_head_dim_ok(k_pages.shape[3])
-            and _hip.layout_ok(k_pages) and _hip.layout_ok(v_pages))
+            and _in_place(k_pages) and _in_place(v_pages))
+
+
+def _in_place(t) -> bool:
+    if not torch.compiler.is_compiling():
+        return _hip.layout_ok(t)
+    # There is no address under torch.compile; the op copies a pool that begins
+    # off a 16-byte border.
+    return t.stride(3) == 1 and not any(s % 8 for s in t.stride()[:3])
 
 
 def sizes_ok(q, k_pages, v_pages, tables) -> bool:

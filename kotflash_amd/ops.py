@@ -158,6 +158,7 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     """Attention over the pages (``kotflash_amd.paged.paged_attention`` on the
     HIP kernels): O and LSE; inference only."""
     check_attention(q, k_pages, v_pages, tables, lengths)
+    k_pages, v_pages = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (k_pages, v_pages))
     require_readable(q, k_pages, v_pages, tables)
     return attention_paged(q, k_pages, v_pages, tables, lengths, causal=causal, scale=scale,
                            with_lse=True)

@@ -424,14 +424,16 @@ class PagedKVCache:
         # Every check of the attention comes before the store writes anything.
         scale, on_hip = _attention_route(q, self.k_pages, self.v_pages, self.table.tables,
                                          self.table.lengths, causal, None, attention_backend)
-        if append_backend in ("auto", "fused") and on_hip and not torch.compiler.is_compiling():
+        if append_backend in ("auto", "fused") and on_hip:
             hip_paged.check_append(self.k_pages, self.v_pages, new_k, new_v, slots)
             _no_gradients("paged append", new_k, new_v)
             most = _hip.KF_PAGED_STEP_SLOTS if append_backend == "fused" else hip_paged.FUSED_STEP_ROWS
             if slots.shape[0] == q.shape[0] and hip_paged.step_fuses(self.k_pages, new_k, most):
-                return hip_paged.append_attention_paged(
-                    q, self.k_pages, self.v_pages, new_k, new_v, slots, self.table.tables,
-                    self.table.lengths, causal=causal, scale=scale)
+                if not torch.compiler.is_compiling():
+                    return hip_paged.append_attention_paged(
+                        q, self.k_pages, self.v_pages, new_k, new_v, slots, self.table.tables,
+                        self.table.lengths, causal=causal, scale=scale)
+                append_backend = "hip"  # two ops: none stores and attends
         if append_backend == "fused":
             raise ValueError("append_backend='fused' needs HIP attention, up to "
                              f"{_hip.KF_PAGED_STEP_TOKENS} new tokens per request, "

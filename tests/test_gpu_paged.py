@@ -1120,3 +1120,47 @@ def test_sizes_beyond_the_kernels(native, monkeypatch):
     assert torch.equal(out, o) and (k[0, :, 50:50 + b] == 1).all() and int((k[0] != 0).sum()) == b * hkv * d
     del k, v, cache
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("how", ["auto", "fused", "hip"])
+@pytest.mark.parametrize("offset", [0, 4])
+def test_a_compiled_step_is_one_graph_of_the_ops(how, offset):
+    """Compiled with fullgraph, random keys and values, causal drafts over page
+    borders, pools off a 16-byte border too: each step against eager calls."""
+    from torch._dynamo.backends.registry import lookup_backend
+
+    seen = []
+
+    def backend(gm, inputs):
+        seen.append([str(n.target).split(".")[1] for n in gm.graph.nodes if "kotflash_amd" in str(n.target)])
+        return lookup_backend("aot_eager")(gm, inputs)
+
+    results = []
+    for compiled in (False, True):
+        torch.manual_seed(5)
+        table = PageTable(2, 128, num_pages=16)
+        cache = PagedKVCache(table, 2, 64, dtype=F16)
+        if compiled and offset:
+            n = cache.k_pages.numel()
+            cache.k_pages, cache.v_pages = (torch.empty(n + 8, device="cuda", dtype=F16)[offset:offset + n].view(16, 2, 16, 64)
+                                            for _ in range(2))
+        cache.k_pages.zero_()
+        cache.v_pages.zero_()
+        most = _counts([21, 100])
+
+        def step(q, k, v):
+            table.trim(most)
+            return cache.append_and_attend(q, k, v, table.reserve(3), causal=True, append_backend=how)
+
+        torch._dynamo.reset()
+        fn = torch.compile(step, backend=backend, fullgraph=True) if compiled else step
+        outs = []
+        for _ in range(20):
+            k, v = torch.randn(2, 2, 2, 3, 64, device="cuda").to(F16)
+            outs.append(fn(torch.randn(2, 4, 3, 64, device="cuda").to(F16), k, v))
+        results.append([torch.stack(outs), table.tables, table.lengths, table.free_pages, table.counters,
+                        cache.k_pages, cache.v_pages])
+    assert seen == [["page_trim_", "page_reserve_", "paged_append_", "paged_decode"]]
+    assert results[0][2].tolist() == [24, 60]
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

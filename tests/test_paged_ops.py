@@ -97,3 +97,37 @@ def test_reference_import_path():
     import kotflash
 
     assert importlib.import_module("kotflash.paged") is importlib.import_module("kotflash_amd.paged") is kotflash.paged
+
+
+@pytest.mark.parametrize("how", ["auto", "fused", "hip"])
+def test_a_step_traces_without_graph_breaks(how, monkeypatch):
+    """Table, store and attention as the custom ops, in one graph. Nothing runs
+    here: the kernels need a GPU."""
+    from kotflash_amd import paged
+
+    monkeypatch.setattr(paged, "_on_gfx950", lambda t: True)
+    table = PageTable(2, 64, num_pages=8, device="cpu")
+    cache = paged.PagedKVCache(table, 2, 64, dtype=torch.float16)
+    most = torch.tensor([20, 40], dtype=torch.int32)
+
+    class Traced(Exception):
+        pass
+
+    seen = []
+
+    def backend(gm, inputs):
+        seen.extend(str(n.target) for n in gm.graph.nodes if "kotflash_amd" in str(n.target))
+
+        def run(*args):
+            raise Traced
+        return run
+
+    def step(q, n):
+        table.trim(most)
+        return cache.append_and_attend(q, n, n, table.reserve(1), append_backend=how)
+
+    torch._dynamo.reset()
+    with pytest.raises(Traced):
+        torch.compile(step, backend=backend, fullgraph=True)(torch.zeros(2, 4, 1, 64).half(),
+                                                             torch.zeros(2, 2, 1, 64).half())
+    assert [s.split(".")[1] for s in seen] == ["page_trim_", "page_reserve_", "paged_append_", "paged_decode"]
