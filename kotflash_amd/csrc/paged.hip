@@ -77,7 +77,7 @@ struct PagedParams {
   int cap;         // tokens that a table has columns for
   int rows, nrb;   // packed rows per row group, row groups per KV head
   int heads;       // Hkv * nrb
-  int workers, least;
+  int workers;
   uint32_t q_bytes, o_bytes;  // extents of a KV head's queries and outputs
   int causal;
   float scale_log2;
@@ -109,6 +109,7 @@ struct PagedParams {
 #define KF_TILE4(nt) KF_TILE3(nt) KF_NEXT("%5", "%1", nt)
 template <int N, bool STREAM>
 __device__ inline void dma_tile(__amdgpu_buffer_rsrc_t r, uint32_t to, const uint32_t* off) {
+  static_assert(N >= 1 && N <= 4);
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(to);
 #define KF_EMIT(text, ...)                                                                        \
   do {                                                                                            \
@@ -118,11 +119,7 @@ __device__ inline void dma_tile(__amdgpu_buffer_rsrc_t r, uint32_t to, const uin
   if constexpr (N == 1) KF_EMIT(KF_TILE1, "v"(off[0]));
   else if constexpr (N == 2) KF_EMIT(KF_TILE2, "v"(off[0]), "v"(off[1]));
   else if constexpr (N == 3) KF_EMIT(KF_TILE3, "v"(off[0]), "v"(off[1]), "v"(off[2]));
-  else if constexpr (N == 4) KF_EMIT(KF_TILE4, "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]));
-  else {
-    dma_tile<4, STREAM>(r, to, off);
-    dma_tile<N - 4, STREAM>(r, to + 4096u, off + 4);
-  }
+  else KF_EMIT(KF_TILE4, "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]));
 #undef KF_EMIT
 }
 
@@ -151,7 +148,7 @@ __device__ inline int steps_from(const PagedParams& p, int b0, int lane) {
 }
 // Units per worker.
 __device__ inline int run_length(const PagedParams& p, int total) {
-  return max(p.least, (total * p.heads + p.workers - 1) / p.workers);
+  return (total * p.heads + p.workers - 1) / p.workers;
 }
 
 // A unit: a step of row group hh of request b, with `rem` keys of the request
@@ -270,7 +267,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       fresh[k] = 64 * k + lane < rows && slot[k] >= 0 && slot[k] < (int64_t)c.pages * c.page_size ? (int)slot[k] >> 4 : -1;
-    const uint32_t all = (uint32_t)rows * (uint32_t)c.Hkv;
+    const uint32_t all = (uint32_t)rows * (uint32_t)c.Hkv;  // at most 2^30: B Hkv <= kMergeRows
     for (uint32_t e = ((uint32_t)(c.workers - 1 - (int)blockIdx.x) * NW + wave) * 4 + (lane >> 4); e < all;
          e += (uint32_t)c.workers * NW * 4) {
       const int kvh = (int)(e / (uint32_t)rows);
@@ -950,7 +947,6 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
   p.cap = (int)cap;
   p.rows = rows; p.nrb = (int)nrb; p.heads = (int)heads;
   p.workers = paged_workers(D, R);
-  p.least = 1;
   p.q_bytes = (uint32_t)q_bytes;
   p.o_bytes = (uint32_t)o_bytes;
   p.causal = causal != 0;
@@ -1011,7 +1007,6 @@ extern "C" int kf_paged_append_decode(const void* q, void* k_pages, void* v_page
   if (B > KF_PAGED_STEP_SLOTS / Snew)
     return set_error(KF_EUNSUPPORTED, "%s: up to %d new tokens in all, got %lld", what, KF_PAGED_STEP_SLOTS,
                      (long long)(B * Snew));
-  if (Hkv > 0x7fffffff / KF_PAGED_STEP_SLOTS) return set_error(KF_EUNSUPPORTED, "%s: too many heads", what);
   if (page_size > 0 && num_pages > 0x7fffffff / page_size)
     return set_error(KF_EUNSUPPORTED, "%s: a pool of 2^31 slots or more", what);
   const NewRows fresh = {new_k, new_v, slots, Snew, slots_stride, new_k_strides, new_v_strides};

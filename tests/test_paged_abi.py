@@ -108,7 +108,7 @@ def test_append_decode(kw, match):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(B=17, n=16), "256 new tokens in all"), (dict(B=257), "256 new tokens in all"),
-    (dict(Hq=2 ** 23, Hkv=2 ** 23), "too many heads"),
+    (dict(Hq=2 ** 26, Hkv=2 ** 26), "grid"),
 ])
 def test_append_decode_sizes(kw, match):
     a = dict(n=1, B=2, Hq=4, Hkv=2)
