@@ -199,8 +199,10 @@ __device__ inline void worker_barrier() {
 }
 
 // NW waves per worker, 16 packed rows each: they share the ring, every wave
-// loading a part of each step, and read all of it.
-template <typename T, int DT, int NW>
+// loading a part of each step, and read all of it. FUSED: with the store of new
+// rows (in one kernel it costs calls without any up to 0.2 us, for scalars that
+// no longer fit the registers).
+template <typename T, int DT, int NW, bool FUSED>
 __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) void paged_kernel(const PagedParams p) {
   constexpr int CPR = DT / 8;         // 16-byte chunks per row
   constexpr int NDC = DT / 32;        // 32-wide head-dim chunks (S contraction)
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     stg16((char*)(uintptr_t)kbase + (uint64_t)id * c.k_page + (uint64_t)at * c.k_row + ch * 16, kk);
     stg16((char*)(uintptr_t)vbase + (uint64_t)id * c.v_page + (uint64_t)at * c.v_row + ch * 16, vv);
   };
-  if (p.nnew > 0) {
+  if constexpr (FUSED) {
     const auto& c = cold();
     const int rows = c.B * c.nnew;
     int64_t slot[4];  // all on their way at once
@@ -416,9 +418,9 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   // The new rows in the two groups of unit `at`, to their slots before the
   // unit's loads, four at a time. Few units have any; those wait for their
   // stores. Against the store in a launch of its own, us for both: 1 to 8 short
-  // requests 9.3 and 10.4, 64 of up to 500 tokens 10.7 and 11.8, but 294 MB over
-  // 32 requests 57.3 and 56.3, 64 requests of 4 drafts 69.7 and 64.8, 16 of 16
-  // 23.3 and 20.8.
+  // requests 9.8 and 11.5, 64 of up to 500 tokens 10.8 and 12.4, but 294 MB over
+  // 32 requests 57.1 and 56.1, 64 requests of 4 drafts 70.5 and 65.7, 16 of 16
+  // 23.0 and 20.6.
   auto store_hits = [&] {
     const int g0 = (uint32_t)page[0] < (uint32_t)p.pages ? page[0] * p.gpp + part : -2;
     const int g1 = (uint32_t)page[1] < (uint32_t)p.pages ? page[1] * p.gpp + row1 / 16 : -2;
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
   auto issue = [&](bool more, auto slot_c) {
     constexpr int slot = decltype(slot_c)::value;
     const uint32_t kv0 = lds0 + slot * 2 * VT * 2;
-    if (p.nnew > 0) store_hits();
+    if constexpr (FUSED) store_hits();
     if (at.begin) {
       const auto& c = cold();
       const int kvh = at.hh / c.nrb;
@@ -819,13 +821,19 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((paged_merge_kernel<T, QL, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
 }
 
+template <typename T, int DT, int NW>
+static void launch_workers(const PagedParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)p.workers), block(64 * NW);
+  if (p.nnew > 0) hipLaunchKernelGGL((paged_kernel<T, DT, NW, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((paged_kernel<T, DT, NW, false>), grid, block, 0, stream, p);
+}
+
 template <typename T, int DT>
 static int launch_paged(const PagedParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)p.workers);
   switch (paged_waves(p.rows)) {
-    case 1: hipLaunchKernelGGL((paged_kernel<T, DT, 1>), grid, dim3(64), 0, stream, p); break;
-    case 2: hipLaunchKernelGGL((paged_kernel<T, DT, 2>), grid, dim3(128), 0, stream, p); break;
-    default: hipLaunchKernelGGL((paged_kernel<T, DT, 4>), grid, dim3(256), 0, stream, p); break;
+    case 1: launch_workers<T, DT, 1>(p, stream); break;
+    case 2: launch_workers<T, DT, 2>(p, stream); break;
+    default: launch_workers<T, DT, 4>(p, stream); break;
   }
   const int rc = check_launch("kf_paged_decode(workers)");
   if (rc) return rc;

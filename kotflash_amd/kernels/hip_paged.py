@@ -14,9 +14,9 @@ from ._layout import require_hip_tensors
 PAGE_GRANULE = 16  # rows that the decode kernel loads from one page at a time
 
 # Most new rows that ``append_backend="auto"`` has stored by the attention's
-# launches: those save a launch and 1.1 us of GPU time for short requests and
+# launches: those save a launch and 1.6 us of GPU time for short requests and
 # cost a large call 1 us of 57; beyond this many they cost more than they save
-# (256 of them 69.7 us and 64.8, also 23.3 and 20.8).
+# (256 rows 70.5 us and 65.7, also 23.0 and 20.6).
 FUSED_STEP_ROWS = 64
 
 
