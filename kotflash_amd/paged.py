@@ -74,7 +74,10 @@ def paged_append(k_pages, v_pages, new_k, new_v, slots, *, backend: str = "auto"
     at ``slots`` (int64 [B, S]: page * page_size + row): K and V bit-exact, in
     one launch. Slots outside the pool (-1 in the padding of ``reserve``) are
     skipped. Two tokens of a call must not share a slot (what it holds then is
-    either's, or a mixture), and new_k/new_v must not lie in the pools."""
+    either's, or a mixture), and new_k/new_v must not lie in the pools.
+
+    ``auto`` takes ``hip`` for fp16 and bf16 on gfx950, which needs pools with a
+    unit head_dim stride and refuses others; ``torch`` takes any."""
     # The ordinary GPU call is checked and launched natively; anything else (and
     # every error) takes the checks below. So do the calls further down.
     if backend in ("auto", "hip", "cuda") and not torch.compiler.is_compiling() \
