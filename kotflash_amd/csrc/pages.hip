@@ -415,7 +415,9 @@ extern "C" int kf_page_trim(int32_t* tables, int32_t* lengths, int32_t* free_pag
   if (rc) return rc;
   if (new_lengths == nullptr && new_length < 0)
     return set_error(KF_EINVAL, "%s: the new length must not be negative", what);
-  const TableParams p = table_params(tables, lengths, free_pages, counters, new_lengths, new_length, B, columns,
+  // No request is longer than 2^30, which check_table sees to.
+  const int64_t keep = new_length < 0x3fffffff ? new_length : 0x3fffffff;
+  const TableParams p = table_params(tables, lengths, free_pages, counters, new_lengths, keep, B, columns,
                                      table_stride, page_size, num_pages);
   // More threads for larger tables, which may give back many pages at once
   // (64 requests of 512 tokens 14.2 us with 256, 12.2 with 1024; 256 of 5 8.2

@@ -1164,3 +1164,16 @@ def test_a_compiled_step_is_one_graph_of_the_ops(how, offset):
     assert results[0][2].tolist() == [24, 60]
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_library_trims_to_lengths_beyond_32_bits():
+    table = PageTable(2, 64, num_pages=8)
+    table.reserve(40)
+    state = (table.tables, table.lengths, table.free_pages, table.counters)
+    before = [t.clone() for t in state]
+    for length in (2 ** 30, 2 ** 31, 2 ** 32 + 3, 2 ** 62):
+        _hip.page_trim(*state, length, page_size=16)
+        for t, b in zip(state, before):
+            assert torch.equal(t, b), length
+    _hip.page_trim(*state, 20, page_size=16)
+    assert table.lengths.tolist() == [20, 20] and table.num_free() == 4
