@@ -366,6 +366,25 @@ int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const vo
                            const int64_t* o_strides, float scale, int causal, int dtype,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions: q_out and k_out are q [B, Hq, S, D] and k [B, Hk, S, D]
+ * (Hk = 0: no keys, null) with pair i of the first R dims of every head, (x, y),
+ * turned to (x cos a - y sin a, x sin a + y cos a) * amplitude at a = 2 pi n
+ * turns[i] / 2^64 (device int64 [R / 2]; n turns[i] wraps, so that far positions
+ * keep their angles); inverse != 0 turns by -a, which is the transpose and so
+ * the gradient. Pairs are (i, i + R / 2), or (2 i, 2 i + 1) with interleaved;
+ * dims from R on are copied. n = positions[b * strides[0] + t * strides[1]] (device
+ * int32, int64 with wide != 0; null: `first`), plus t with step != 0. All
+ * tensors may have any strides (int64_t[4]); the outputs must not overlap the
+ * inputs or themselves. No reference counterpart.
+ */
+int kf_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* turns,
+              const void* positions, int wide, int64_t first, int step, int64_t B, int64_t Hq,
+              int64_t Hk, int64_t S, int64_t D, int64_t R, const int64_t* q_strides4,
+              const int64_t* k_strides4, const int64_t* q_out_strides4,
+              const int64_t* k_out_strides4, const int64_t* position_strides2, float amplitude,
+              int interleaved, int inverse, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,7 @@ _SIGNATURES = {
                              _I64, _I64, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _SZ, _P]),
     "kf_paged_append_decode": (_I, [_P] * 10 + [_I64] * 11 + [_I64P] * 6
                                + [_F, _I, _I, _P, _SZ, _P]),
+    "kf_rotary": (_I, [_P] * 6 + [_I, _I64, _I] + [_I64] * 6 + [_I64P] * 5 + [_F, _I, _I, _I, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -499,3 +500,28 @@ def paged_append_decode(q, k_pages, v_pages, new_k, new_v, slots, out, lse: Opti
             workspace.nbytes, _stream(q.device),
         )
     _check(rc, "kf_paged_append_decode")
+
+
+def rotary(q, k: Optional[torch.Tensor], q_out, k_out: Optional[torch.Tensor], turns, positions, *,
+           interleaved: bool, inverse: bool, amplitude: float) -> None:
+    """kf_rotary: ``positions`` an int or a device int32 or int64 tensor of
+    shape [B] (each request's first), [B, S] or [1, S]."""
+    b, hq, s, d = q.shape
+    on_device = isinstance(positions, torch.Tensor)
+    first = not on_device or positions.ndim == 1
+    where = None
+    if on_device:
+        per_request = positions.stride(0) if positions.shape[0] > 1 else 0
+        where = (ctypes.c_int64 * 2)(per_request, 0 if first else positions.stride(1))
+    none = k is None
+    with _DeviceGuard(q.device):
+        rc = lib().kf_rotary(
+            q.data_ptr(), None if none else k.data_ptr(), q_out.data_ptr(),
+            None if none else k_out.data_ptr(), turns.data_ptr(),
+            positions.data_ptr() if on_device else None,
+            int(on_device and positions.dtype == torch.int64), 0 if on_device else positions, int(first),
+            b, hq, 0 if none else k.shape[1], s, d, 2 * turns.numel(), _strides(q),
+            None if none else _strides(k), _strides(q_out), None if none else _strides(k_out), where,
+            float(amplitude), int(interleaved), int(inverse), dtype_code(q.dtype), _stream(q.device),
+        )
+    _check(rc, "kf_rotary")

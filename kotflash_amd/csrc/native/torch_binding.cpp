@@ -236,6 +236,14 @@ double forward_flops(const Tensor& q, const Tensor& k, bool causal) {
 
 PyObject* not_handled() { Py_RETURN_NOTIMPLEMENTED; }
 
+PyObject* pair_of(Tensor a, Tensor b) {
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) throw python_error();
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(b)));
+  return pair;
+}
+
 bool exact_bool(PyObject* o, bool& v) {
   v = o == Py_True;
   return o == Py_True || o == Py_False;
@@ -604,11 +612,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     out = launch_paged(a, with_lse ? &lse : nullptr, nullptr);
   }
   if (!with_lse) return THPVariable_Wrap(std::move(out));
-  PyObject* pair = PyTuple_New(2);
-  if (pair == nullptr) throw python_error();
-  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
-  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
-  return pair;
+  return pair_of(std::move(out), std::move(lse));
   END_HANDLE_TH_ERRORS
 }
 
@@ -743,7 +747,133 @@ PyObject* py_page_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// Rotary positions.
+
+struct RotaryWhere {
+  Tensor turns, positions;  // positions undefined: `first`
+  int64_t first;
+  bool interleaved;
+  double amplitude;
+};
+
+// q and, where defined, k turned, as fresh contiguous tensors.
+torch::autograd::variable_list launch_rotary(const Tensor& q, const Tensor& k, const RotaryWhere& w, bool inverse) {
+  const bool keys = k.defined(), table = w.positions.defined();
+  Tensor qo = at::empty(q.sizes(), q.options());
+  Tensor ko;
+  if (keys) ko = at::empty(k.sizes(), k.options());
+  int64_t where[2] = {0, 0};
+  if (table) {
+    where[0] = w.positions.size(0) > 1 ? w.positions.stride(0) : 0;
+    where[1] = w.positions.dim() > 1 ? w.positions.stride(1) : 0;
+  }
+  check(kf_rotary(q.const_data_ptr(), keys ? k.const_data_ptr() : nullptr, qo.data_ptr(),
+                  keys ? ko.data_ptr() : nullptr, w.turns.const_data_ptr<int64_t>(),
+                  table ? w.positions.const_data_ptr() : nullptr,
+                  table && w.positions.scalar_type() == at::kLong, w.first, !table || w.positions.dim() == 1,
+                  q.size(0), q.size(1), keys ? k.size(1) : 0, q.size(2), q.size(3), 2 * w.turns.numel(),
+                  q.strides().data(), keys ? k.strides().data() : nullptr, qo.strides().data(),
+                  keys ? ko.strides().data() : nullptr, where, (float)w.amplitude, w.interleaved, inverse,
+                  dtype_code(q), stream_of(q)),
+        "kf_rotary");
+  if (keys) return {qo, ko};
+  return {qo};
+}
+
+// A custom function takes no undefined tensors.
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// Linear in q and k: its gradient is itself, turned back, and has gradients too.
+struct HipRotary : torch::autograd::Function<HipRotary> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q,
+                                                const std::optional<Tensor>& keys, const Tensor& turns,
+                                                const std::optional<Tensor>& table, int64_t first,
+                                                bool interleaved, bool inverse, double amplitude) {
+    const Tensor k = keys.value_or(Tensor()), positions = table.value_or(Tensor());
+    ctx->save_for_backward({turns, positions});
+    ctx->saved_data["first"] = first;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["amplitude"] = amplitude;
+    ctx->set_materialize_grads(false);
+    return launch_rotary(q, k, {turns, positions, first, interleaved, amplitude}, inverse);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t first = ctx->saved_data["first"].toInt();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = ctx->saved_data["inverse"].toBool();
+    const double amplitude = ctx->saved_data["amplitude"].toDouble();
+    torch::autograd::variable_list out(8), there;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) there.push_back(grads[i]);
+    if (there.empty()) return out;
+    const c10::OptionalDeviceGuard guard(there[0].device());
+    const Tensor second = there.size() > 1 ? there[1] : Tensor();
+    const auto turned = at::GradMode::is_enabled()
+                            ? HipRotary::apply(there[0], given(second), saved[0], given(saved[1]), first, interleaved,
+                                               !inverse, amplitude)
+                            : launch_rotary(there[0], second, {saved[0], saved[1], first, interleaved, amplitude}, !inverse);
+    size_t next = 0;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) out[i] = turned[next++];
+    return out;
+  }
+};
+
+// rotary(q, k or None, turns, positions (int or tensor), head_dim,
+// interleaved, amplitude): (q, k), or q without k.
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  RotaryWhere w;
+  if (n != 7 || !PyLong_CheckExact(args[4]) || !exact_bool(args[5], w.interleaved) || !PyFloat_CheckExact(args[6]))
+    return not_handled();
+  const bool keys = args[1] != Py_None;
+  const Tensor *q = plain_tensor(args[0]), *k = keys ? plain_tensor(args[1]) : nullptr, *turns = plain_tensor(args[2]);
+  if (!q || (keys && !k) || !turns || !plain_mode() || q->dim() != 4 || q->numel() == 0 || !half_type(*q) ||
+      !is_gfx950(q->device().index()))
+    return not_handled();
+  if (keys && (k->dim() != 4 || k->scalar_type() != q->scalar_type() || k->device() != q->device() ||
+               k->size(0) != q->size(0) || k->size(1) == 0 || k->size(2) != q->size(2) || k->size(3) != q->size(3)))
+    return not_handled();
+  int over = 0;
+  if (q->size(3) != PyLong_AsLongLongAndOverflow(args[4], &over) || over) return not_handled();
+  if (turns->scalar_type() != at::kLong || turns->dim() != 1 || turns->device() != q->device() ||
+      !turns->is_contiguous() || turns->numel() == 0 || 2 * turns->numel() > q->size(3))
+    return not_handled();
+  w.first = 0;
+  if (PyLong_CheckExact(args[3])) {
+    w.first = PyLong_AsLongLongAndOverflow(args[3], &over);
+    if (over || w.first < -(1ll << 62) || w.first >= (1ll << 62)) return not_handled();
+  } else {
+    const Tensor* at = plain_tensor(args[3]);
+    if (!at || at->device() != q->device() || (at->scalar_type() != at::kInt && at->scalar_type() != at::kLong))
+      return not_handled();
+    const bool each = at->dim() == 2 && at->size(1) == q->size(2) && (at->size(0) == q->size(0) || at->size(0) == 1);
+    if (!each && !(at->dim() == 1 && at->size(0) == q->size(0))) return not_handled();
+    w.positions = *at;
+  }
+  w.turns = *turns;
+  w.amplitude = PyFloat_AS_DOUBLE(args[6]);
+  const bool grad = keys ? wants_grad({q, k}) : wants_grad({q});
+  torch::autograd::variable_list out;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(q->device());
+    const Tensor second = keys ? *k : Tensor();
+    out = grad ? HipRotary::apply(*q, given(second), w.turns, given(w.positions), w.first, w.interleaved, false,
+                                  w.amplitude)
+               : launch_rotary(*q, second, w, false);
+  }
+  if (!keys) return THPVariable_Wrap(std::move(out[0]));
+  return pair_of(std::move(out[0]), std::move(out[1]));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
+    {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},
     {"paged_step", (PyCFunction)(void (*)(void))py_paged_step, METH_FASTCALL, nullptr},

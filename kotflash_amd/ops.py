@@ -22,6 +22,9 @@ implementation and, for attention, a registered backward:
   new_lengths, page_size) -> ()`` (the paged cache of ``kotflash_amd.paged``,
   no reference counterpart; ``paged_append_`` mutates both pools, the last two
   the page table's state)
+- ``kotflash_amd::rotary(q, k, turns, positions, first, interleaved, inverse,
+  amplitude) -> (q, k)`` (``kotflash_amd.rotary``, no reference counterpart;
+  autograd differentiates it through itself, turned back)
 
 ``torch.compile`` traces through them without graph breaks: the fake
 implementations give it output shapes, dtypes and strides, and autograd
@@ -30,7 +33,7 @@ fresh contiguous tensors, as the fake implementations state.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -42,8 +45,10 @@ from .kernels.hip_paged import (
     trim_pages,
 )
 
+from .kernels.hip_rotary import check_rotary, rotate
+
 __all__ = ["attn_fwd", "attn_bwd", "decode", "kv_append_", "append_decode_", "paged_decode",
-           "paged_append_", "page_reserve_", "page_trim_"]
+           "paged_append_", "page_reserve_", "page_trim_", "rotary"]
 
 
 def _contig(t: torch.Tensor) -> torch.Tensor:
@@ -208,3 +213,40 @@ def page_trim_(tables: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Te
 @page_trim_.register_fake
 def _page_trim_fake(tables, lengths, free_pages, counters, new_lengths, page_size):
     return None
+
+
+@torch.library.custom_op("kotflash_amd::rotary", mutates_args=())
+def rotary(q: torch.Tensor, k: torch.Tensor, turns: torch.Tensor, positions: Optional[torch.Tensor],
+           first: int, interleaved: bool, inverse: bool,
+           amplitude: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q and k (of no heads: none) turned by their positions
+    (``kotflash_amd.rotary.Rotary`` on the HIP kernel)."""
+    where = first if positions is None else positions
+    keys = k if k.shape[1] else None
+    check_rotary(q, keys, q.shape[3], where, turns.device)
+    if turns.dtype != torch.int64 or turns.ndim != 1 or not 0 < 2 * turns.numel() <= q.shape[3]:
+        raise ValueError("turns must be an int64 tensor of shape [rotary_dim / 2]")
+    q_out, k_out = rotate(q, keys, turns.contiguous(), where, interleaved=interleaved,
+                          inverse=inverse, amplitude=amplitude)
+    return q_out, torch.empty_like(k) if k_out is None else k_out
+
+
+@rotary.register_fake
+def _rotary_fake(q, k, turns, positions, first, interleaved, inverse, amplitude):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+def _rotary_setup_context(ctx, inputs, output):
+    q, k, turns, positions, first, interleaved, inverse, amplitude = inputs
+    ctx.save_for_backward(turns, positions)
+    ctx.rest = first, interleaved, inverse, amplitude
+
+
+def _rotary_backward(ctx, dq, dk):
+    turns, positions = ctx.saved_tensors
+    first, interleaved, inverse, amplitude = ctx.rest
+    dq, dk = rotary(dq, dk, turns, positions, first, interleaved, not inverse, amplitude)
+    return dq, dk, None, None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup_context)
