@@ -367,6 +367,47 @@ int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const vo
                            void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * The paged cache in 8 bits. Pools of e4m3 codes (OCP), laid out as the 16-bit
+ * ones (strides in elements, multiples of 16; D a multiple of 16 up to 128,
+ * page_size of 16), and scales: fp32 [num_pages, Hkv, page_size / 16, 2]
+ * (scale_strides {page, head}, the rest contiguous), one for K and one for V of
+ * every block of 16 rows of a page and head. A value is code * scale; scales
+ * are powers of two in [2^-126, 2^120], or 0 before anything was stored. No
+ * reference counterpart.
+ *
+ * kf_fp8_append quantises new[b, h, t, :] into slot slots[b, t], K and V in one
+ * launch; a slot outside the pool is skipped. The scale of a block is the least
+ * power of two s >= 2^-126 with |x| <= 448 s for all finite x that come into
+ * it, or, unless its row 0 is among them, the one it has if that is more; where
+ * that grows, the block's other rows are divided by the ratio and rounded. Codes
+ * are rounded to even; infinities become NaN; a code that would stand for 2^16
+ * (fp16) or 2^128 (bf16) is the one below. Slots that are not skipped must differ,
+ * and those of one block be of one request and follow one another. new_k/new_v
+ * have a unit head_dim stride, 16-byte aligned bases and strides that are
+ * multiples of 8 elements (int64_t[3]).
+ */
+int kf_fp8_append(void* k_pages, void* v_pages, float* scales, const void* new_k, const void* new_v,
+                  const int64_t* slots, int64_t B, int64_t H, int64_t Snew, int64_t D,
+                  int64_t num_pages, int64_t page_size, int64_t slots_stride,
+                  const int64_t* k_strides, const int64_t* v_strides, const int64_t* scale_strides,
+                  const int64_t* new_k_strides, const int64_t* new_v_strides, int dtype,
+                  void* stream);
+
+/*
+ * k_out[b, h, t, :] and v_out (16-bit, [B, H, width, D], strides as new_k's) are
+ * position starts[b] + t (device int32; null: `start`; at least 0) of request
+ * b; zeros from min(lengths[b], columns * page_size) on, and where the table names
+ * no page of the pool.
+ */
+int kf_fp8_read(const void* k_pages, const void* v_pages, const float* scales, void* k_out,
+                void* v_out, const int32_t* tables, const int32_t* lengths, const int32_t* starts,
+                int64_t start, int64_t B, int64_t H, int64_t width, int64_t D, int64_t num_pages,
+                int64_t page_size, int64_t columns, int64_t table_stride, const int64_t* k_strides,
+                const int64_t* v_strides, const int64_t* scale_strides,
+                const int64_t* k_out_strides, const int64_t* v_out_strides, int dtype,
+                void* stream);
+
+/*
  * Rotary positions: q_out and k_out are q [B, Hq, S, D] and k [B, Hk, S, D]
  * (Hk = 0: no keys, null) with pair i of the first R dims of every head, (x, y),
  * turned to (x cos a - y sin a, x sin a + y cos a) * amplitude at a = 2 pi n

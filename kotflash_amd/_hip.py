@@ -70,6 +70,8 @@ _SIGNATURES = {
                              _I64, _I64, _I64P, _I64P, _I64P, _I64P, _F, _I, _I, _P, _SZ, _P]),
     "kf_paged_append_decode": (_I, [_P] * 10 + [_I64] * 11 + [_I64P] * 6
                                + [_F, _I, _I, _P, _SZ, _P]),
+    "kf_fp8_append": (_I, [_P] * 6 + [_I64] * 7 + [_I64P] * 5 + [_I, _P]),
+    "kf_fp8_read": (_I, [_P] * 8 + [_I64] * 9 + [_I64P] * 5 + [_I, _P]),
     "kf_rotary": (_I, [_P] * 6 + [_I, _I64, _I] + [_I64] * 6 + [_I64P] * 5 + [_F, _I, _I, _I, _P]),
 }
 
@@ -525,3 +527,30 @@ def rotary(q, k: Optional[torch.Tensor], q_out, k_out: Optional[torch.Tensor], t
             float(amplitude), int(interleaved), int(inverse), dtype_code(q.dtype), _stream(q.device),
         )
     _check(rc, "kf_rotary")
+
+
+def fp8_append(k_pages, v_pages, scales, new_k, new_v, slots) -> None:
+    b, h, n, d = new_k.shape
+    with _DeviceGuard(k_pages.device):
+        rc = lib().kf_fp8_append(
+            k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), new_k.data_ptr(), new_v.data_ptr(),
+            slots.data_ptr(), b, h, n, d, k_pages.shape[0], k_pages.shape[2], slots.stride(0),
+            _strides(k_pages), _strides(v_pages), _strides(scales), _strides(new_k), _strides(new_v),
+            dtype_code(new_k.dtype), _stream(k_pages.device),
+        )
+    _check(rc, "kf_fp8_append")
+
+
+def fp8_read(k_pages, v_pages, scales, k_out, v_out, tables, lengths, start) -> None:
+    """kf_fp8_read: ``start`` an int or a device int32 [B] tensor."""
+    b, h, width, d = k_out.shape
+    on_device = isinstance(start, torch.Tensor)
+    with _DeviceGuard(k_pages.device):
+        rc = lib().kf_fp8_read(
+            k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+            tables.data_ptr(), lengths.data_ptr(), start.data_ptr() if on_device else None,
+            0 if on_device else start, b, h, width, d, k_pages.shape[0], k_pages.shape[2], tables.shape[1],
+            tables.stride(0), _strides(k_pages), _strides(v_pages), _strides(scales), _strides(k_out),
+            _strides(v_out), dtype_code(k_out.dtype), _stream(k_pages.device),
+        )
+    _check(rc, "kf_fp8_read")

@@ -748,6 +748,129 @@ PyObject* py_page_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ---------------------------------------------------------------------------
+// Paged cache in 8 bits.
+
+// Pools [pages, Hkv, page, D] of e4m3 and their scales [pages, Hkv, page / 16,
+// 2], as the kernels address them.
+struct Fp8Pools {
+  const Tensor *k, *v, *scales;
+  bool read(PyObject* const* a) {
+    k = plain_tensor(a[0]); v = plain_tensor(a[1]); scales = plain_tensor(a[2]);
+    if (!k || !v || !scales || !plain_mode() || k->dim() != 4 || k->sizes() != v->sizes() || k->numel() == 0 ||
+        k->scalar_type() != at::kFloat8_e4m3fn || v->scalar_type() != at::kFloat8_e4m3fn ||
+        scales->scalar_type() != at::kFloat || wants_grad({scales}) || v->device() != k->device() || scales->device() != k->device())
+      return false;
+    const auto s = k->sizes();
+    const int64_t want[4] = {s[0], s[1], s[2] / 16, 2};
+    if (s[2] % 16 || s[3] % 16 || s[3] > 128 || scales->sizes() != at::IntArrayRef(want, 4)) return false;
+    for (const Tensor* t : {k, v})
+      if (t->stride(3) != 1 || t->stride(0) % 16 || t->stride(1) % 16 || t->stride(2) % 16 ||
+          reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16)
+        return false;
+    return scales->stride(3) == 1 && scales->stride(2) == 2 && scales->stride(1) % 2 == 0 &&
+           scales->stride(0) % 2 == 0 && reinterpret_cast<uintptr_t>(scales->const_data_ptr()) % 8 == 0 &&
+           is_gfx950(k->device().index());
+  }
+  bool writable() const {
+    for (const Tensor* t : {k, v, scales})
+      for (int i = 0; i < 4; ++i)
+        if (t->stride(i) == 0 && t->size(i) > 1) return false;
+    return true;
+  }
+};
+
+struct Fp8Store {
+  Fp8Pools p;
+  const Tensor *nk, *nv, *slots;
+  // Arguments from `a`: k_pages, v_pages, scales; from `n`: new_k, new_v, slots.
+  bool read(PyObject* const* a, PyObject* const* n) {
+    nk = plain_tensor(n[0]); nv = plain_tensor(n[1]); slots = plain_tensor(n[2]);
+    if (!nk || !nv || !slots || !p.read(a) || !p.writable()) return false;
+    if (nk->dim() != 4 || nk->sizes() != nv->sizes() || nk->numel() == 0 || nk->size(1) != p.k->size(1) ||
+        nk->size(3) != p.k->size(3) || !half_type(*nk) || nv->scalar_type() != nk->scalar_type() ||
+        nk->device() != p.k->device() || nv->device() != p.k->device() || wants_grad({nk, nv}))
+      return false;
+    return slots->scalar_type() == at::kLong && slots->dim() == 2 && slots->size(0) == nk->size(0) &&
+           slots->size(1) == nk->size(2) && slots->stride(1) == 1 && slots->device() == nk->device();
+  }
+};
+
+void launch_fp8_store(const Fp8Store& a) {
+  const Tensor nk = readable(*a.nk), nv = readable(*a.nv);
+  check(kf_fp8_append(a.p.k->data_ptr(), a.p.v->data_ptr(), a.p.scales->data_ptr<float>(), nk.const_data_ptr(),
+                      nv.const_data_ptr(), a.slots->const_data_ptr<int64_t>(), nk.size(0), nk.size(1), nk.size(2),
+                      nk.size(3), a.p.k->size(0), a.p.k->size(2), a.slots->stride(0), a.p.k->strides().data(),
+                      a.p.v->strides().data(), a.p.scales->strides().data(), nk.strides().data(),
+                      nv.strides().data(), dtype_code(nk), stream_of(nk)),
+        "kf_fp8_append");
+}
+
+// fp8_append(k_pages, v_pages, scales, new_k, new_v, slots).
+PyObject* py_fp8_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Fp8Store a;
+  if (n != 6 || !a.read(args, args + 3)) return not_handled();
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.nk->device());
+    launch_fp8_store(a);
+  }
+  written({a.p.k, a.p.v, a.p.scales});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// Tables int32 [B, columns] and lengths [B] as the kernels address them.
+bool tables_ok(const Tensor* tables, const Tensor* lengths, const c10::Device& dev) {
+  return int32_on(tables, dev) && int32_on(lengths, dev) && tables->dim() == 2 && lengths->dim() == 1 &&
+         tables->numel() > 0 && lengths->size(0) == tables->size(0) && tables->stride(1) == 1 &&
+         tables->stride(0) >= 0 && lengths->is_contiguous();
+}
+
+// fp8_read(k_pages, v_pages, scales, tables, lengths, width, start (int or
+// tensor), half, 16 bits): K and V.
+PyObject* py_fp8_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Fp8Pools p;
+  bool half, sixteen;
+  if (n != 9 || !exact_bool(args[7], half) || !exact_bool(args[8], sixteen) || !sixteen ||
+      !PyLong_CheckExact(args[5]) || !p.read(args))
+    return not_handled();
+  const Tensor *tables = plain_tensor(args[3]), *lengths = plain_tensor(args[4]), *starts = nullptr;
+  if (!tables || !lengths || !tables_ok(tables, lengths, p.k->device())) return not_handled();
+  int over = 0;
+  const int64_t width = PyLong_AsLongLongAndOverflow(args[5], &over);
+  if (over || width <= 0 || width >= (1 << 30)) return not_handled();
+  int64_t start = 0;
+  if (PyLong_CheckExact(args[6])) {
+    start = PyLong_AsLongLongAndOverflow(args[6], &over);
+    if (over || start < 0 || start >= (1 << 30)) return not_handled();
+  } else {
+    starts = plain_tensor(args[6]);
+    if (!int32_on(starts, p.k->device()) || starts->dim() != 1 || starts->size(0) != tables->size(0) ||
+        !starts->is_contiguous())
+      return not_handled();
+  }
+  Tensor k, v;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(p.k->device());
+    const auto options = p.k->options().dtype(half ? at::kHalf : at::kBFloat16);
+    k = at::empty({tables->size(0), p.k->size(1), width, p.k->size(3)}, options);
+    v = at::empty(k.sizes(), options);
+    check(kf_fp8_read(p.k->const_data_ptr(), p.v->const_data_ptr(), p.scales->const_data_ptr<float>(), k.data_ptr(),
+                      v.data_ptr(), tables->const_data_ptr<int32_t>(), lengths->const_data_ptr<int32_t>(),
+                      starts ? starts->const_data_ptr<int32_t>() : nullptr, start, k.size(0), k.size(1), width,
+                      k.size(3), p.k->size(0), p.k->size(2), tables->size(1), tables->stride(0),
+                      p.k->strides().data(), p.v->strides().data(), p.scales->strides().data(),
+                      k.strides().data(), v.strides().data(), dtype_code(k), stream_of(k)),
+          "kf_fp8_read");
+  }
+  return pair_of(std::move(k), std::move(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------
 // Rotary positions.
 
 struct RotaryWhere {
@@ -873,6 +996,8 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef kMethods[] = {
+    {"fp8_append", (PyCFunction)(void (*)(void))py_fp8_append, METH_FASTCALL, nullptr},
+    {"fp8_read", (PyCFunction)(void (*)(void))py_fp8_read, METH_FASTCALL, nullptr},
     {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},

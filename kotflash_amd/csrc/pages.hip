@@ -24,19 +24,6 @@
 
 namespace kf {
 
-// n / d for n < 2^31 by a multiplication (Granlund and Montgomery 1994): with
-// 2^(s-1) < d <= 2^s, m = ceil(2^(31+s) / d) is exact for 31-bit n.
-struct Divisor {
-  uint32_t d, m;
-  int shift;
-};
-static Divisor divisor(uint32_t d) {
-  int s = 0;
-  while ((1ull << s) < d) ++s;
-  return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
-}
-__device__ inline int quotient(int n, const Divisor& v) { return (int)(((uint64_t)(uint32_t)n * v.m) >> v.shift); }
-
 struct TableParams {
   int32_t* tables;
   int32_t* lengths;

@@ -22,6 +22,10 @@ implementation and, for attention, a registered backward:
   new_lengths, page_size) -> ()`` (the paged cache of ``kotflash_amd.paged``,
   no reference counterpart; ``paged_append_`` mutates both pools, the last two
   the page table's state)
+- ``kotflash_amd::fp8_append_(k_pages, v_pages, scales, new_k, new_v, slots) -> ()``
+  and ``kotflash_amd::fp8_read(k_pages, v_pages, scales, tables, lengths,
+  start, width, dtype) -> (k, v)`` (the 8-bit cache of ``kotflash_amd.paged_fp8``,
+  no reference counterpart; the first mutates pools and scales)
 - ``kotflash_amd::rotary(q, k, turns, positions, first, interleaved, inverse,
   amplitude) -> (q, k)`` (``kotflash_amd.rotary``, no reference counterpart;
   autograd differentiates it through itself, turned back)
@@ -45,10 +49,11 @@ from .kernels.hip_paged import (
     trim_pages,
 )
 
+from .kernels import hip_paged_fp8
 from .kernels.hip_rotary import check_rotary, rotate
 
 __all__ = ["attn_fwd", "attn_bwd", "decode", "kv_append_", "append_decode_", "paged_decode",
-           "paged_append_", "page_reserve_", "page_trim_", "rotary"]
+           "paged_append_", "page_reserve_", "page_trim_", "fp8_append_", "fp8_read", "rotary"]
 
 
 def _contig(t: torch.Tensor) -> torch.Tensor:
@@ -213,6 +218,35 @@ def page_trim_(tables: torch.Tensor, lengths: torch.Tensor, free_pages: torch.Te
 @page_trim_.register_fake
 def _page_trim_fake(tables, lengths, free_pages, counters, new_lengths, page_size):
     return None
+
+
+@torch.library.custom_op("kotflash_amd::fp8_append_", mutates_args=("k_pages", "v_pages", "scales"))
+def fp8_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, new_k: torch.Tensor,
+                new_v: torch.Tensor, slots: torch.Tensor) -> None:
+    """new_k/new_v [B, Hkv, S, D] quantised into their slots of the pools."""
+    hip_paged_fp8.check_append(k_pages, v_pages, scales, new_k, new_v, slots)
+    hip_paged_fp8.append_fp8(k_pages, v_pages, scales, new_k, new_v, slots)
+
+
+@fp8_append_.register_fake
+def _fp8_append_fake(k_pages, v_pages, scales, new_k, new_v, slots):
+    return None
+
+
+@torch.library.custom_op("kotflash_amd::fp8_read", mutates_args=())
+def fp8_read(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor, tables: torch.Tensor,
+             lengths: torch.Tensor, start: torch.Tensor, width: int,
+             dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V of every request from its start on
+    (``kotflash_amd.paged_fp8.fp8_read`` on the HIP kernel)."""
+    hip_paged_fp8.check_read(k_pages, v_pages, scales, tables, lengths, width, start, dtype)
+    return hip_paged_fp8.read_fp8(k_pages, v_pages, scales, tables, lengths, width, start, dtype)
+
+
+@fp8_read.register_fake
+def _fp8_read_fake(k_pages, v_pages, scales, tables, lengths, start, width, dtype):
+    shape = (tables.shape[0], k_pages.shape[1], width, k_pages.shape[3])
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
 
 @torch.library.custom_op("kotflash_amd::rotary", mutates_args=())

@@ -1,0 +1,256 @@
+"""The 8-bit paged cache's kernels on the GPU, against the definition."""
+import math
+
+import pytest
+import torch
+
+import kotflash_amd.ops  # noqa: F401
+from kotflash_amd.kernels import hip_paged_fp8
+from kotflash_amd.paged import PageTable
+from kotflash_amd.paged_fp8 import PagedKVCacheFP8, fp8_append, fp8_read
+from tests.fp8_oracle import Cache, make_cache
+
+pytestmark = pytest.mark.gpu
+F16, BF16, FP8 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _randn(*shape, dtype=F16, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).cuda()
+
+
+def _cache(batch, hkv, d, page, max_len, dtype=F16, seed=0):
+    table = PageTable(batch, max_len, num_pages=batch * -(-max_len // page) + 2, page_size=page, device="cuda")
+    order = torch.randperm(table.num_pages, generator=torch.Generator().manual_seed(seed))
+    table.free_pages.copy_(order.to(torch.int32))
+    return PagedKVCacheFP8(table, hkv, d, dtype=dtype)
+
+
+def _same(a, b):
+    return torch.equal(a.double().nan_to_num(7), b.to(a.device).double().nan_to_num(7))
+
+
+# --- store -------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+def test_append_dims(dtype, d):
+    """Prompts, tokens and drafts that make blocks grow."""
+    cache = _cache(3, 2, d, 32, 160, dtype, seed=d)
+    table = cache.table
+    ref = Cache(cache.k_pages, cache.v_pages, cache.scales)
+    rows = torch.zeros(0, dtype=torch.int64)
+    for step, (counts, width) in enumerate((((37, 1, 0), 37), ((1, 1, 1), 1), ((2, 5, 0), 5), ((1, 1, 1), 1),
+                                            ((40, 17, 33), 40), ((1, 1, 1), 1))):
+        k, v = (_randn(3, 2, width, d, dtype=dtype, seed=10 * step + i, scale=2.5 ** step) for i in range(2))
+        slots = table.reserve(torch.tensor(counts, dtype=torch.int32, device="cuda"), width=width)
+        cache.append(k, v, slots, backend="hip")
+        ref.append(k, v, slots)
+        rows = torch.cat((rows, slots[slots >= 0].cpu()))
+        ref.assert_matches(cache.k_pages, cache.v_pages, cache.scales, rows)
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 33, 100])
+@pytest.mark.parametrize("first", [0, 1, 15, 16, 21])
+def test_append_lengths(n, first):
+    """Runs that begin and end anywhere in a block and in a window."""
+    cache = _cache(2, 3, 64, 16, 160, BF16, seed=n)
+    ref = Cache(cache.k_pages, cache.v_pages, cache.scales)
+    rows = []
+    for i, width in enumerate((first, n)):
+        if width:
+            k, v = (_randn(2, 3, width, 64, dtype=BF16, seed=i + j, scale=10.0 ** i) for j in range(2))
+            slots = cache.table.reserve(width)
+            cache.append(k, v, slots, backend="hip")
+            ref.append(k, v, slots)
+            rows.append(slots.flatten().cpu())
+    ref.assert_matches(cache.k_pages, cache.v_pages, cache.scales, torch.cat(rows))
+
+
+def test_append_any_slots():
+    """Single tokens and runs at any slots of different blocks, slots outside
+    the pool among them; everything else stays as it was."""
+    k8, v8, scales, _, _ = make_cache(1, 4, 128, 48, [48 * 40], dtype=F16, seed=3, device="cuda")
+    ref = Cache(k8, v8, scales)
+    places = k8.shape[0] * 48
+    g = torch.Generator().manual_seed(1)
+    blocks = torch.randperm(places // 16, generator=g)[:90].view(6, 15)
+    slots = blocks * 16 + torch.randint(0, 16, blocks.shape, generator=g)
+    slots[0, ::4], slots[1, 3], slots[2, 0], slots[3, 14] = -1, places, -2 ** 40, 2 ** 62
+    slots[4, 4:9] = int(blocks[4, 4]) * 16 + torch.tensor([7, 3, 12, 0, 9])  # a run in no order
+    k, v = _randn(6, 4, 15, 128, scale=30.0), _randn(6, 4, 15, 128, seed=1, scale=0.01)
+    fp8_append(k8, v8, scales, k, v, slots.cuda(), backend="hip")
+    ref.append(k, v, slots)
+    ref.assert_matches(k8, v8, scales)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_append_special_values(dtype):
+    k = torch.zeros(2, 1, 18, 64, dtype=dtype)
+    k[0, 0, 0, :8] = torch.tensor([math.inf, -math.inf, math.nan, torch.finfo(dtype).max, -torch.finfo(dtype).max, 1,
+                                   torch.finfo(dtype).smallest_normal, -0.0])
+    k[0, 0, 17, 3] = math.inf
+    k[1, 0, 0] = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps * torch.arange(-32, 32)
+    k[1, 0, 16] = torch.linspace(-448, 448, 64)
+    k[1, 0, 17] = 448.5
+    v = k.flip(3)
+    cache = _cache(2, 1, 64, 16, 64, dtype)
+    slots = cache.table.reserve(18)
+    ref = Cache(cache.k_pages, cache.v_pages, cache.scales)
+    cache.append(k.cuda(), v.cuda(), slots, backend="hip")
+    ref.append(k, v, slots)
+    ref.assert_matches(cache.k_pages, cache.v_pages, cache.scales, slots.flatten().cpu())
+    # A grown block with NaN in it, and one that nothing was stored to.
+    for n, scale in ((1, 300.0), (1, 0.0)):
+        k = (_randn(2, 1, n, 64, dtype=dtype) * scale).nan_to_num(0, 1, 1)
+        slots = torch.cat((slots, cache.table.reserve(n)), 1)
+        cache.append(k, k, slots[:, -n:], backend="hip")
+        ref.append(k, k, slots[:, -n:])
+        ref.assert_matches(cache.k_pages, cache.v_pages, cache.scales, slots.flatten().cpu())
+
+
+def test_append_layouts():
+    """Transposed views, rows off 16-byte borders, strided pools and slots."""
+    shape = (6, 2, 32, 64)
+    wide = torch.zeros(6, 2, 2, 32, 128, dtype=torch.uint8, device="cuda").view(FP8)
+    k8, v8 = wide[:, 0, :, :, :64], wide[:, 1, :, :, 64:]
+    scales = torch.zeros(6, 3, 2, 2, 2, device="cuda")[:, 1]
+    assert k8.shape == shape and not k8.is_contiguous()
+    ref = Cache(k8, v8, scales)
+    k, v = _randn(3, 20, 2, 64).transpose(1, 2), _randn(3, 2, 20, 68, seed=1)[..., 4:]
+    slots = torch.arange(0, 60, device="cuda").view(3, 20) + torch.tensor([[0], [12 + 32], [24 + 64]], device="cuda")
+    other = torch.stack((slots, slots), 2)[..., 0]
+    fp8_append(k8, v8, scales, k, v, other, backend="hip")
+    ref.append(k, v, slots)
+    ref.assert_matches(k8, v8, scales)
+    beside = wide.view(torch.uint8).clone()
+    beside[:, 0, :, :, :64] = beside[:, 1, :, :, 64:] = 0
+    assert not beside.any()
+
+
+# --- read --------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d,page", [(16, 16), (48, 48), (64, 16), (80, 32), (128, 16), (128, 256)])
+def test_read(dtype, d, page):
+    lengths = [0, 1, 15, 16, 17, 100, 300]
+    k8, v8, scales, tables, lens = make_cache(7, 2, d, page, lengths, dtype=dtype, seed=d, device="cuda")
+    tables[5, 0] = -3
+    tables[6, 0] = 10 ** 6
+    ref = Cache(k8, v8, scales)
+    starts = torch.tensor([0, -5, 3, 16, 10 ** 9, 41, 250], dtype=torch.int32, device="cuda")
+    for width, start in ((1, 0), (37, 0), (300, 0), (40, 90), (64, starts), (5, 2 ** 29)):
+        first = starts.tolist() if isinstance(start, torch.Tensor) else [start] * 7
+        got = fp8_read(k8, v8, scales, tables, lens, width, start=start, dtype=dtype, backend="hip")
+        want = ref.read(tables.cpu(), lens, width, first, dtype)
+        for g, w in zip(got, want):
+            assert g.dtype == dtype and g.is_contiguous() and _same(w, g.cpu())
+
+
+def test_read_codes_and_scales():
+    """Every code, scales from end to end of the type."""
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 1, 16, 16).expand(31, 1, 16, 16).contiguous().cuda().view(FP8)
+    for dtype, low, high in ((F16, -33, 8), (BF16, -126, 120)):
+        scales = torch.exp2(torch.linspace(low, high, 31).round()).view(31, 1, 1, 1).expand(31, 1, 1, 2).contiguous().cuda()
+        tables = torch.arange(31, dtype=torch.int32, device="cuda")[None]
+        lens = torch.tensor([31 * 16], dtype=torch.int32, device="cuda")
+        k, v = fp8_read(codes, codes, scales, tables, lens, 31 * 16, dtype=dtype, backend="hip")
+        want = (codes.cpu().float().double() * scales.cpu().double()[..., :1]).to(dtype)
+        assert _same(want.view(496, 16), k[0, 0].cpu()) and torch.equal(k.view(torch.int16), v.view(torch.int16))
+
+
+def test_paths_agree():
+    """The native call, the ctypes one, the op and torch.compile."""
+    args = make_cache(3, 2, 64, 32, [40, 7, 90], dtype=F16, seed=2, device="cuda")
+    want = fp8_read(*args, 90, dtype=F16)
+    pools, start = args[:3], torch.zeros(3, dtype=torch.int32, device="cuda")
+    for got in (hip_paged_fp8.read_fp8(*args, 90, 0, F16), hip_paged_fp8.read_fp8(*args, 90, start, F16),
+                torch.ops.kotflash_amd.fp8_read(*args, start, 90, F16),
+                torch.compile(lambda *a: fp8_read(*a, 90, dtype=F16), fullgraph=True, backend="aot_eager")(*args)):
+        assert all(_same(a, b) for a, b in zip(want, got))
+    k, v = _randn(3, 2, 4, 64), _randn(3, 2, 4, 64, seed=1)
+    slots = (torch.arange(12, device="cuda") * 16 + 5).view(3, 4)
+    results = []
+    for store in (fp8_append, hip_paged_fp8.append_fp8, torch.ops.kotflash_amd.fp8_append_,
+                  torch.compile(fp8_append, fullgraph=True, backend="aot_eager")):
+        mine = [t.clone() for t in pools]
+        store(*mine, k, v, slots)
+        results.append([mine[0].view(torch.uint8), mine[1].view(torch.uint8), mine[2]])
+    for r in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], r))
+
+
+def test_versions_and_refusals():
+    k8, v8, scales, tables, lens = make_cache(2, 2, 64, 16, [5, 20], dtype=F16, seed=2, device="cuda")
+    k, slots = _randn(2, 2, 1, 64), torch.tensor([[0], [16]], device="cuda")
+    before = [t._version for t in (k8, v8, scales)]
+    fp8_append(k8, v8, scales, k, k, slots)
+    assert all(t._version > n for t, n in zip((k8, v8, scales), before))
+    with pytest.raises(ValueError, match="head_dim a multiple of 16"):
+        odd = [torch.zeros(2, 1, 16, 24, device="cuda").to(FP8) for _ in range(2)]
+        fp8_read(*odd, torch.zeros(2, 1, 1, 2, device="cuda"), tables, lens, 4, dtype=F16, backend="hip")
+    with pytest.raises(TypeError, match="float16 and bfloat16"):
+        fp8_read(k8, v8, scales, tables, lens, 4, dtype=torch.float32, backend="hip")
+    with pytest.raises(RuntimeError, match="inference"):
+        fp8_append(k8, v8, scales, k.clone().requires_grad_(), k, slots)
+    with pytest.raises(ValueError, match="device"):
+        fp8_append(k8, v8, scales, k, k, slots.cpu())
+    # What the kernels do not take, auto runs in torch.
+    odd = [torch.zeros(2, 1, 16, 24, device="cuda").to(FP8) for _ in range(2)]
+    sc = torch.zeros(2, 1, 1, 2, device="cuda")
+    new = _randn(2, 1, 1, 24)
+    ref = Cache(*odd, sc)
+    fp8_append(*odd, sc, new, new, slots)
+    ref.append(new, new, slots)
+    ref.assert_matches(*odd, sc)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of more than 4 GiB: pages at its far end."""
+    pages = (5 << 30) // (2 * 16 * 128)
+    k8 = torch.empty(pages, 2, 16, 128, dtype=torch.uint8, device="cuda").view(FP8)
+    v8 = torch.empty_like(k8)
+    scales = torch.zeros(pages, 2, 1, 2, device="cuda")
+    tables = torch.tensor([[pages - 1, 3, pages - 7]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([43], dtype=torch.int32, device="cuda")
+    t = torch.arange(43, device="cuda")
+    slots = (tables[0].long()[t // 16] * 16 + t % 16)[None]
+    k, v = _randn(1, 2, 43, 128), _randn(1, 2, 43, 128, seed=1)
+    fp8_append(k8, v8, scales, k, v, slots, backend="hip")
+    small = [torch.zeros(3, 2, 16, 128, device="cuda").to(FP8) for _ in range(2)]
+    ss = torch.zeros(3, 2, 1, 2, device="cuda")
+    fp8_append(*small, ss, k, v, t[None], backend="torch")
+    got = fp8_read(k8, v8, scales, tables, lens, 43, dtype=F16, backend="hip")
+    want = fp8_read(*small, ss, torch.arange(3, dtype=torch.int32, device="cuda")[None], lens, 43, dtype=F16, backend="torch")
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graph_replays():
+    """A captured reserve, append and read follows the requests as they grow."""
+    cache = _cache(2, 2, 64, 16, 200)
+    table = cache.table
+    k, v = _randn(2, 2, 3, 64), _randn(2, 2, 3, 64, seed=1)
+
+    def call():
+        slots = table.reserve(3)
+        cache.append(k, v, slots)
+        return cache.read(32)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    table.trim(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    ref = _cache(2, 2, 64, 16, 200)
+    for step in range(6):
+        k.copy_(_randn(2, 2, 3, 64, seed=step, scale=1.5 ** step))
+        v.copy_(_randn(2, 2, 3, 64, seed=step + 50))
+        graph.replay()
+        torch.cuda.synchronize()
+        slots = ref.table.reserve(3)
+        ref.append(k, v, slots)
+        want = ref.read(32)
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
