@@ -408,6 +408,24 @@ int kf_fp8_read(const void* k_pages, const void* v_pages, const float* scales, v
                 void* stream);
 
 /*
+ * Attention of q (16-bit) over pools of codes as they read back in its type:
+ * kf_paged_decode otherwise, with the scales and their strides. The workspace
+ * has a size of its own.
+ */
+size_t kf_fp8_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);
+int kf_fp8_decode_check(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,
+                        int64_t num_pages, int64_t page_size, int64_t columns,
+                        const int64_t* q_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, const int64_t* scale_strides);
+int kf_fp8_decode(const void* q, const void* k_pages, const void* v_pages, const float* scales,
+                  void* o, float* lse, const int32_t* tables, const int32_t* lengths, int64_t B,
+                  int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, int64_t num_pages,
+                  int64_t page_size, int64_t columns, int64_t table_stride,
+                  const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                  const int64_t* scale_strides, const int64_t* o_strides, float scale, int causal,
+                  int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Rotary positions: q_out and k_out are q [B, Hq, S, D] and k [B, Hk, S, D]
  * (Hk = 0: no keys, null) with pair i of the first R dims of every head, (x, y),
  * turned to (x cos a - y sin a, x sin a + y cos a) * amplitude at a = 2 pi n

@@ -72,6 +72,9 @@ _SIGNATURES = {
                                + [_F, _I, _I, _P, _SZ, _P]),
     "kf_fp8_append": (_I, [_P] * 6 + [_I64] * 7 + [_I64P] * 5 + [_I, _P]),
     "kf_fp8_read": (_I, [_P] * 8 + [_I64] * 9 + [_I64P] * 5 + [_I, _P]),
+    "kf_fp8_decode_workspace_bytes": (_SZ, [_I64] * 5),
+    "kf_fp8_decode_check": (_I, [_I64] * 8 + [_I64P] * 4),
+    "kf_fp8_decode": (_I, [_P] * 8 + [_I64] * 9 + [_I64P] * 5 + [_F, _I, _I, _P, _SZ, _P]),
     "kf_rotary": (_I, [_P] * 6 + [_I, _I64, _I] + [_I64] * 6 + [_I64P] * 5 + [_F, _I, _I, _I, _P]),
 }
 
@@ -554,3 +557,34 @@ def fp8_read(k_pages, v_pages, scales, k_out, v_out, tables, lengths, start) -> 
             _strides(v_out), dtype_code(k_out.dtype), _stream(k_pages.device),
         )
     _check(rc, "kf_fp8_read")
+
+
+@lru_cache(maxsize=256)
+def fp8_decode_workspace_bytes(b, hq, hkv, sq, d) -> int:
+    return int(lib().kf_fp8_decode_workspace_bytes(b, hq, hkv, sq, d))
+
+
+def fp8_decode_check(q, k_pages, v_pages, scales, columns: int) -> int:
+    """kf_fp8_decode_check for tensors that the launcher reads in place (q made
+    contiguous if it does not): 0, or an error for ``_check``."""
+    b, hq, sq, d = q.shape
+    num_pages, hkv, page_size, _ = k_pages.shape
+    q_strides = _strides(q) if layout_ok(q) else _I64x4(hq * sq * d, sq * d, d, 1)
+    return lib().kf_fp8_decode_check(b, hq, hkv, sq, d, num_pages, page_size, columns, q_strides,
+                                     _strides(k_pages), _strides(v_pages), _strides(scales))
+
+
+def fp8_decode(q, k_pages, v_pages, scales, out, lse: Optional[torch.Tensor], tables, lengths, *,
+               scale: float, causal: bool, workspace: torch.Tensor) -> None:
+    b, hq, sq, d = q.shape
+    num_pages, hkv, page_size, _ = k_pages.shape
+    with _DeviceGuard(q.device):
+        rc = lib().kf_fp8_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), out.data_ptr(),
+            lse.data_ptr() if lse is not None else None, tables.data_ptr(), lengths.data_ptr(),
+            b, hq, hkv, sq, d, num_pages, page_size, tables.shape[1], tables.stride(0),
+            _strides(q), _strides(k_pages), _strides(v_pages), _strides(scales), _strides(out),
+            float(scale), int(bool(causal)), dtype_code(q.dtype), workspace.data_ptr(),
+            workspace.nbytes, _stream(q.device),
+        )
+    _check(rc, "kf_fp8_decode")

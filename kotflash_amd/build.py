@@ -55,6 +55,7 @@ FILE_FLAGS = {
     "fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -17,4 +17,12 @@ __device__ inline uint32_t dequantise2(uint32_t codes, float scale) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, HIGH));
 }
 
+// Transposed read of an 8 x 16 block of bytes (ds_read_b64_tr_b8): inside each
+// group of 16 lanes, lanes 2 r and 2 r + 1 address the halves of row r, and lane i
+// receives column i. Checked on the device.
+__device__ inline u32x2 lds_read_tr8(const uint8_t* p) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((KF_LDS i32x2*)(p)));
+}
+
 }  // namespace kf

@@ -870,6 +870,86 @@ PyObject* py_fp8_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+struct Fp8Attention {
+  Fp8Pools p;
+  const Tensor *q, *tables, *lengths;
+  double scale;
+  bool causal;
+  // Arguments from `a`: q, k_pages, v_pages, scales, tables, lengths, causal,
+  // scale or None.
+  bool read(PyObject* const* a) {
+    q = plain_tensor(a[0]); tables = plain_tensor(a[4]); lengths = plain_tensor(a[5]);
+    if (!q || !tables || !lengths || !exact_bool(a[6], causal) || !p.read(a + 1)) return false;
+    if (q->dim() != 4 || q->numel() == 0 || !half_type(*q) || q->size(3) != p.k->size(3) ||
+        q->size(1) % p.k->size(1) || q->device() != p.k->device() || wants_grad({q}) ||
+        !tables_ok(tables, lengths, q->device()) || tables->size(0) != q->size(0))
+      return false;
+    if (a[7] == Py_None) scale = 1.0 / std::sqrt((double)q->size(3));
+    else if (PyFloat_CheckExact(a[7])) scale = PyFloat_AS_DOUBLE(a[7]);
+    else return false;
+    if (!std::isfinite(scale)) return false;
+    const int64_t hq = q->size(1), sq = q->size(2), d = q->size(3), dense[3] = {hq * sq * d, sq * d, d};
+    return kf_fp8_decode_check(q->size(0), hq, p.k->size(1), sq, d, p.k->size(0), p.k->size(2), tables->size(1),
+                               layout_ok(*q) ? q->strides().data() : dense, p.k->strides().data(),
+                               p.v->strides().data(), p.scales->strides().data()) == KF_OK;
+  }
+};
+
+Tensor launch_fp8(const Fp8Attention& a, Tensor* lse) {
+  const Tensor q = readable(*a.q);
+  const Tensor &k = *a.p.k, &v = *a.p.v;
+  const int64_t b = q.size(0), hq = q.size(1), sq = q.size(2), d = q.size(3), hkv = k.size(1);
+  Tensor out = at::empty({b, hq, sq, d}, q.options());
+  if (lse) *lse = at::empty({b, hq, sq}, q.options().dtype(at::kFloat));
+  Tensor ws = bytes_like(q, kf_fp8_decode_workspace_bytes(b, hq, hkv, sq, d));
+  check(kf_fp8_decode(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), a.p.scales->const_data_ptr<float>(),
+                      out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr, a.tables->const_data_ptr<int32_t>(),
+                      a.lengths->const_data_ptr<int32_t>(), b, hq, hkv, sq, d, k.size(0), k.size(2),
+                      a.tables->size(1), a.tables->stride(0), q.strides().data(), k.strides().data(),
+                      v.strides().data(), a.p.scales->strides().data(), out.strides().data(), (float)a.scale,
+                      a.causal, dtype_code(q), ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
+        "kf_fp8_decode");
+  return out;
+}
+
+// fp8_attention(q, k_pages, v_pages, scales, tables, lengths, causal, scale or
+// None, return_lse).
+PyObject* py_fp8_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Fp8Attention a;
+  bool with_lse;
+  if (n != 9 || !exact_bool(args[8], with_lse) || !a.read(args)) return not_handled();
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.q->device());
+    out = launch_fp8(a, with_lse ? &lse : nullptr);
+  }
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  return pair_of(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// fp8_step(q, k_pages, v_pages, scales, tables, lengths, causal, None, new_k,
+// new_v, slots): the store, then the attention.
+PyObject* py_fp8_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Fp8Attention a;
+  Fp8Store st;
+  if (n != 11 || !a.read(args) || !st.read(args + 1, args + 8) || st.nk->scalar_type() != a.q->scalar_type())
+    return not_handled();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release nogil;
+    const c10::OptionalDeviceGuard guard(a.q->device());
+    launch_fp8_store(st);
+    out = launch_fp8(a, nullptr);
+  }
+  written({st.p.k, st.p.v, st.p.scales});
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // ---------------------------------------------------------------------------
 // Rotary positions.
 
@@ -998,6 +1078,8 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     {"fp8_append", (PyCFunction)(void (*)(void))py_fp8_append, METH_FASTCALL, nullptr},
     {"fp8_read", (PyCFunction)(void (*)(void))py_fp8_read, METH_FASTCALL, nullptr},
+    {"fp8_attention", (PyCFunction)(void (*)(void))py_fp8_attention, METH_FASTCALL, nullptr},
+    {"fp8_step", (PyCFunction)(void (*)(void))py_fp8_step, METH_FASTCALL, nullptr},
     {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},

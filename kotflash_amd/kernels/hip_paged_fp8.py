@@ -86,6 +86,56 @@ def check_read(k_pages, v_pages, scales, tables, lengths, width, start, dtype) -
         raise ValueError("dtype must be float16, bfloat16 or float32")
 
 
+def check_attention(q, k_pages, v_pages, scales, tables, lengths) -> None:
+    """The contract of ``fp8_attention``, whatever runs it."""
+    check_pools(k_pages, v_pages, scales)
+    if not isinstance(q, torch.Tensor) or q.ndim != 4:
+        raise ValueError("q must use [B, Hq, Sq, D] layout")
+    if min(q.shape) == 0:
+        raise ValueError("q must be non-empty")
+    if q.shape[3] != k_pages.shape[3]:
+        raise ValueError("Query head dimension must match the K/V pages")
+    if q.shape[1] % k_pages.shape[1]:
+        raise ValueError("Query heads must be divisible by the K/V pages' head count")
+    if q.device != k_pages.device:
+        raise ValueError("Query device must match the K/V pages")
+    if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise ValueError("q must be float16, bfloat16 or float32")
+    check_tables(tables, lengths, q.device)
+    if tables.shape[0] != q.shape[0]:
+        raise ValueError("tables must be an int32 tensor of shape [B, columns]")
+
+
+def sizes_ok(q, k_pages, v_pages, scales, tables) -> bool:
+    """Whether the decode kernel addresses these sizes (pools that pass
+    ``pages_in_place``). Under torch.compile it is left to the call."""
+    return (torch.compiler.is_compiling()
+            or _hip.fp8_decode_check(q, k_pages, v_pages, scales, tables.shape[1]) == 0)
+
+
+def require_readable(q, k_pages, v_pages, scales, tables) -> None:
+    require_hip_tensors("8-bit attention", q)
+    require_in_place("8-bit attention", k_pages, v_pages, scales)
+    if not torch.compiler.is_compiling():
+        _hip._check(_hip.fp8_decode_check(q, k_pages, v_pages, scales, tables.shape[1]), "kf_fp8_decode")
+
+
+def attention_fp8(q, k_pages, v_pages, scales, tables, lengths, *, causal: bool, scale: float,
+                  with_lse: bool = False):
+    """O (and LSE) of q over the pages (``kf_fp8_decode``); the arguments have
+    passed ``check_attention`` and ``require_readable``."""
+    if not _hip.layout_ok(q):
+        q = q.contiguous()
+    tables, lengths = dense_tables(tables, lengths)
+    b, hq, sq, d = q.shape
+    out = torch.empty((b, hq, sq, d), device=q.device, dtype=q.dtype)
+    lse = torch.empty((b, hq, sq), device=q.device, dtype=torch.float32) if with_lse else None
+    ws = _hip.workspace(q.device, _hip.fp8_decode_workspace_bytes(b, hq, k_pages.shape[1], sq, d))
+    _hip.fp8_decode(q, k_pages, v_pages, scales, out, lse, tables, lengths, scale=scale, causal=causal,
+                    workspace=ws)
+    return (out, lse) if with_lse else out
+
+
 def pages_in_place(k_pages, v_pages, scales) -> bool:
     """Whether the kernels read and write these pools as they are."""
     if k_pages.shape[3] % 16 or k_pages.shape[3] > 128:

@@ -22,9 +22,10 @@ implementation and, for attention, a registered backward:
   new_lengths, page_size) -> ()`` (the paged cache of ``kotflash_amd.paged``,
   no reference counterpart; ``paged_append_`` mutates both pools, the last two
   the page table's state)
-- ``kotflash_amd::fp8_append_(k_pages, v_pages, scales, new_k, new_v, slots) -> ()``
-  and ``kotflash_amd::fp8_read(k_pages, v_pages, scales, tables, lengths,
-  start, width, dtype) -> (k, v)`` (the 8-bit cache of ``kotflash_amd.paged_fp8``,
+- ``kotflash_amd::fp8_append_(k_pages, v_pages, scales, new_k, new_v, slots) -> ()``,
+  ``kotflash_amd::fp8_read(k_pages, v_pages, scales, tables, lengths, start,
+  width, dtype) -> (k, v)`` and ``kotflash_amd::fp8_decode(q, k_pages, v_pages,
+  scales, tables, lengths, causal, scale) -> (out, lse)`` (the 8-bit cache of ``kotflash_amd.paged_fp8``,
   no reference counterpart; the first mutates pools and scales)
 - ``kotflash_amd::rotary(q, k, turns, positions, first, interleaved, inverse,
   amplitude) -> (q, k)`` (``kotflash_amd.rotary``, no reference counterpart;
@@ -53,7 +54,7 @@ from .kernels import hip_paged_fp8
 from .kernels.hip_rotary import check_rotary, rotate
 
 __all__ = ["attn_fwd", "attn_bwd", "decode", "kv_append_", "append_decode_", "paged_decode",
-           "paged_append_", "page_reserve_", "page_trim_", "fp8_append_", "fp8_read", "rotary"]
+           "paged_append_", "page_reserve_", "page_trim_", "fp8_append_", "fp8_read", "fp8_decode", "rotary"]
 
 
 def _contig(t: torch.Tensor) -> torch.Tensor:
@@ -247,6 +248,24 @@ def fp8_read(k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
 def _fp8_read_fake(k_pages, v_pages, scales, tables, lengths, start, width, dtype):
     shape = (tables.shape[0], k_pages.shape[1], width, k_pages.shape[3])
     return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("kotflash_amd::fp8_decode", mutates_args=())
+def fp8_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scales: torch.Tensor,
+               tables: torch.Tensor, lengths: torch.Tensor, causal: bool,
+               scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention over the pages (``kotflash_amd.paged_fp8.fp8_attention`` on
+    the HIP kernels): O and LSE; inference only."""
+    hip_paged_fp8.check_attention(q, k_pages, v_pages, scales, tables, lengths)
+    hip_paged_fp8.require_readable(q, k_pages, v_pages, scales, tables)
+    return hip_paged_fp8.attention_fp8(q, k_pages, v_pages, scales, tables, lengths, causal=causal,
+                                       scale=scale, with_lse=True)
+
+
+@fp8_decode.register_fake
+def _fp8_decode_fake(q, k_pages, v_pages, scales, tables, lengths, causal, scale):
+    b, hq, sq, d = q.shape
+    return q.new_empty((b, hq, sq, d)), q.new_empty((b, hq, sq), dtype=torch.float32)
 
 
 @torch.library.custom_op("kotflash_amd::rotary", mutates_args=())

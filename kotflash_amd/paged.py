@@ -139,10 +139,8 @@ def paged_attention(q, k_pages, v_pages, tables, lengths, *, causal: bool = Fals
     return _sdpa_paged(q, k_pages, v_pages, tables, lengths, causal, scale, return_lse)
 
 
-def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backend):
-    """Every check of ``paged_attention``; its scale, and whether the HIP
-    kernel takes it."""
-    hip_paged.check_attention(q, k_pages, v_pages, tables, lengths)
+def _options(q, causal, scale, backend) -> float:
+    """Checks of what an attention call takes beside its tensors; the scale."""
     if not isinstance(causal, bool):
         raise TypeError("causal must be a bool")
     if scale is None:
@@ -156,6 +154,14 @@ def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backen
             raise ValueError("scale must be finite")
     if backend not in PAGED_BACKENDS:
         raise ValueError("backend must be one of: auto, hip, triton, sdpa")
+    return scale
+
+
+def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backend):
+    """Every check of ``paged_attention``; its scale, and whether the HIP
+    kernel takes it."""
+    hip_paged.check_attention(q, k_pages, v_pages, tables, lengths)
+    scale = _options(q, causal, scale, backend)
     _no_gradients("paged attention", q, k_pages, v_pages)
     if backend == "sdpa":
         return scale, False
@@ -169,7 +175,10 @@ def _attention_route(q, k_pages, v_pages, tables, lengths, causal, scale, backen
     return scale, True
 
 
-def _sdpa_paged(q, k_pages, v_pages, tables, lengths, causal: bool, scale: float, return_lse: bool):
+def _sdpa_paged(q, k_pages, v_pages, tables, lengths, causal: bool, scale: float, return_lse: bool,
+                rows_of=None):
+    """``rows_of``: K and V of rows of pages, where the pools do not hold them
+    as they are."""
     b, hq, sq, d = q.shape
     pages, hkv, page, _ = k_pages.shape
     out = torch.zeros((b, hq, sq, d), device=q.device, dtype=q.dtype)
@@ -180,7 +189,9 @@ def _sdpa_paged(q, k_pages, v_pages, tables, lengths, causal: bool, scale: float
         position = torch.arange(n, device=q.device)
         inside = (ids >= 0) & (ids < pages)
         position, ids = position[inside], ids[inside]
-        k, v = (pool[ids, :, position % page].transpose(0, 1)[None] for pool in (k_pages, v_pages))
+        k, v = (x.transpose(0, 1)[None] for x in
+                (rows_of(ids, position % page) if rows_of is not None else
+                 (pool[ids, :, position % page] for pool in (k_pages, v_pages))))
         # Rows grouped by what they see: all of them alike, or (causal) one
         # group per row.
         for r in range(sq) if causal else [slice(None)]:

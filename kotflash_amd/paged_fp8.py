@@ -31,7 +31,9 @@ import torch
 from . import _hip
 from .kernels import hip_paged_fp8
 from .kernels.hip_paged_fp8 import BLOCK, FP8
-from .paged import _HALF, PageTable, _no_gradients, _on_gfx950, _positive
+from .paged import (
+    _HALF, PageTable, _no_gradients, _on_gfx950, _options, _positive, _sdpa_paged,
+)
 
 STORE_BACKENDS = ("auto", "hip", "torch")
 
@@ -103,6 +105,58 @@ def fp8_read(k_pages, v_pages, scales, tables, lengths, width: int, *,
     return hip_paged_fp8.read_fp8(k_pages, v_pages, scales, tables, lengths, width, start, dtype)
 
 
+def fp8_attention(q, k_pages, v_pages, scales, tables, lengths, *, causal: bool = False,
+                  scale: Optional[float] = None, return_lse: bool = False, backend: str = "auto"):
+    """Attention of q [B, Hq, Sq, D] over each request's pages of codes, as
+    they read back in q's type: ``paged_attention`` in every other respect.
+
+    ``hip`` needs gfx950, q in fp16 or bf16 and pools as ``fp8_append``'s;
+    ``auto`` takes it where these hold and ``sdpa`` (one call per request,
+    lengths on the host) elsewhere."""
+    if backend in ("auto", "hip", "triton") and not torch.compiler.is_compiling():
+        out = _hip.native().fp8_attention(q, k_pages, v_pages, scales, tables, lengths, causal, scale,
+                                          return_lse)
+        if out is not NotImplemented:
+            return out
+    scale, on_hip = _attention_route(q, k_pages, v_pages, scales, tables, lengths, causal, scale, backend)
+    if on_hip and torch.compiler.is_compiling():
+        from .ops import fp8_decode
+
+        both = fp8_decode(q, k_pages, v_pages, scales, tables, lengths, causal, scale)
+        return both if return_lse else both[0]
+    if on_hip:
+        return hip_paged_fp8.attention_fp8(q, k_pages, v_pages, scales, tables, lengths, causal=causal,
+                                           scale=scale, with_lse=return_lse)
+
+    def rows_of(ids, rows):
+        return (_values(pool, scales, i, ids, rows).to(q.dtype) for i, pool in enumerate((k_pages, v_pages)))
+
+    return _sdpa_paged(q, k_pages, v_pages, tables, lengths, causal, scale, return_lse, rows_of)
+
+
+def _attention_route(q, k_pages, v_pages, scales, tables, lengths, causal, scale, backend):
+    """Every check of ``fp8_attention``; its scale, and whether the HIP kernel
+    takes it."""
+    hip_paged_fp8.check_attention(q, k_pages, v_pages, scales, tables, lengths)
+    scale = _options(q, causal, scale, backend)
+    _no_gradients("8-bit attention", q, scales)
+    if backend == "sdpa":
+        return scale, False
+    if backend == "auto":
+        return scale, (_on_gfx950(q) and q.dtype in _HALF
+                       and hip_paged_fp8.pages_in_place(k_pages, v_pages, scales)
+                       and hip_paged_fp8.sizes_ok(q, k_pages, v_pages, scales, tables))
+    if not _on_gfx950(q):
+        raise RuntimeError("HIP backend requires an AMD MI355X (gfx950) GPU")
+    hip_paged_fp8.require_readable(q, k_pages, v_pages, scales, tables)
+    return scale, True
+
+
+def _values(pool, scales, which: int, ids, rows):
+    """What rows of pages stand for, in fp32: [..., Hkv, D]."""
+    return pool.view(torch.uint8)[ids, :, rows].view(FP8).float() * scales[ids, :, rows // BLOCK, which][..., None]
+
+
 def _scale_for(largest):
     """The least power of two s >= 2^-126 with largest <= 448 s (fp32)."""
     mantissa, exponent = torch.frexp(largest)  # mantissa in [0.5, 1)
@@ -156,7 +210,7 @@ def _read(k_pages, v_pages, scales, tables, lengths, width: int, start, dtype):
     ids, row = ids.clamp(0, pages - 1), at % page
     out = []
     for i, pool in enumerate((k_pages, v_pages)):
-        x = pool.view(torch.uint8)[ids, :, row].view(FP8).float() * scales[ids, :, row // BLOCK, i][..., None]
+        x = _values(pool, scales, i, ids, row)
         out.append(torch.where(there[..., None, None], x, 0).to(dtype).transpose(1, 2).contiguous())
     return tuple(out)
 
@@ -200,3 +254,31 @@ class PagedKVCacheFP8:
         on, zeros behind its last (``fp8_read``)."""
         return fp8_read(self.k_pages, self.v_pages, self.scales, self.table.tables,
                         self.table.lengths, width, start=start, dtype=self.dtype, backend=backend)
+
+    def attend(self, q, *, causal: bool = False, scale: Optional[float] = None,
+               return_lse: bool = False, backend: str = "auto"):
+        """Attention of q [B, Hq, Sq, D] over what each request holds
+        (``fp8_attention``)."""
+        if getattr(q, "dtype", self.dtype) != self.dtype:
+            raise ValueError("q's dtype must match the cache's")
+        return fp8_attention(q, self.k_pages, self.v_pages, self.scales, self.table.tables,
+                             self.table.lengths, causal=causal, scale=scale, return_lse=return_lse,
+                             backend=backend)
+
+    def append_and_attend(self, q, new_k, new_v, slots, *, causal: bool = False,
+                          append_backend: str = "auto", attention_backend: str = "auto"):
+        """``append``, then ``attend``: a decoding step of this layer, after the
+        table's ``reserve`` of the step."""
+        pools = self.k_pages, self.v_pages, self.scales
+        if append_backend in ("auto", "hip") and attention_backend in ("auto", "hip", "triton") \
+                and not torch.compiler.is_compiling() and getattr(q, "dtype", None) == self.dtype:
+            out = _hip.native().fp8_step(q, *pools, self.table.tables, self.table.lengths, causal, None,
+                                         new_k, new_v, slots)
+            if out is not NotImplemented:
+                return out
+        # Every check of the attention comes before the store writes anything.
+        _attention_route(q, *pools, self.table.tables, self.table.lengths, causal, None, attention_backend)
+        if q.dtype != self.dtype:
+            raise ValueError("q's dtype must match the cache's")
+        self.append(new_k, new_v, slots, backend=append_backend)
+        return self.attend(q, causal=causal, backend=attention_backend)

@@ -4,6 +4,8 @@ import math
 
 import torch
 
+from tests.paged_oracle import attention64
+
 BLOCK = 16
 # Values of the codes 0 to 126 (127 is NaN): 3 bits of mantissa, exponents from
 # -6 on, subnormal below.
@@ -129,3 +131,23 @@ def make_cache(batch, hkv, d, page, lengths, *, dtype, seed, device="cpu", spare
     pools = [torch.where(mine[:, None, :, None], c, 127).to(torch.uint8).view(torch.float8_e4m3fn) for c in codes]
     lens = torch.tensor(lengths, dtype=torch.int32)
     return tuple(t.to(device) for t in (*pools, scales, tables, lens))
+
+
+def assert_attention(got, q, k, v, tables, lengths, *, lse=None, **kw):
+    """``paged_oracle``'s bound, and the rounding of an output below the type's
+    smallest normal value, where blocks of tiny values lead: there a step is
+    smallest_normal * eps, not eps of the value, and half of it is the error
+    (fp16: 2^-14 2^-10 / 2 = 2^-25)."""
+    o, ls, tol, ls_tol = attention64(q, k, v, tables, lengths, **kw)
+    info = torch.finfo(got.dtype)
+    tol = tol + info.smallest_normal * info.eps / 2
+    err = (got.cpu().double() - o).abs()
+    worst = int((err - tol).flatten().nan_to_num(math.inf).argmax())
+    assert bool((err <= tol).all()), (
+        f"{int((~(err <= tol)).sum())} of {err.numel()} outside; worst at {worst}: got "
+        f"{float(got.flatten()[worst])} want {float(o.flatten()[worst])} +- {float(tol.flatten()[worst])}")
+    if lse is not None:
+        x = lse.cpu().double()
+        assert torch.equal(x == -math.inf, ls == -math.inf)
+        fin = ls > -math.inf
+        assert bool(((x - ls).abs()[fin] <= ls_tol[fin]).all()), float((x - ls).abs()[fin].max())

@@ -7,8 +7,9 @@ import torch
 import kotflash_amd.ops  # noqa: F401
 from kotflash_amd.kernels import hip_paged_fp8
 from kotflash_amd.paged import PageTable
-from kotflash_amd.paged_fp8 import PagedKVCacheFP8, fp8_append, fp8_read
-from tests.fp8_oracle import Cache, make_cache
+from kotflash_amd.paged_fp8 import PagedKVCacheFP8, fp8_append, fp8_attention, fp8_read
+from kotflash_amd.rotary import Rotary
+from tests.fp8_oracle import Cache, assert_attention, make_cache
 
 pytestmark = pytest.mark.gpu
 F16, BF16, FP8 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
@@ -254,3 +255,244 @@ def test_graph_replays():
         ref.append(k, v, slots)
         want = ref.read(32)
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+# --- attention ---------------------------------------------------------------
+
+def _case(batch, hq, hkv, sq, d, page, lengths, *, dtype, seed, wild=False):
+    pools = make_cache(batch, hkv, d, page, lengths, dtype=dtype, seed=seed, device="cuda", wild=wild)
+    return (_randn(batch, hq, sq, d, dtype=dtype, seed=seed + 1), *pools)
+
+
+def _check(case, causal=False, scale=None, **kw):
+    q, k8, v8, scales, tables, lens = case
+    o, lse = fp8_attention(*case, causal=causal, scale=scale, return_lse=True, backend="hip", **kw)
+    k, v = Cache(k8, v8, scales).held(q.dtype)
+    assert_attention(o, q, k, v, tables, lens, lse=lse, causal=causal, scale=scale)
+    return o, lse
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("wild", [False, True])
+def test_attention_dims(dtype, d, wild):
+    _check(_case(4, 8, 2, 1, d, 16, [1, 70, 333, 1000], dtype=dtype, seed=d, wild=wild))
+
+
+@pytest.mark.parametrize("length", [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 79, 80, 127, 128, 129, 257])
+@pytest.mark.parametrize("page", [16, 48])
+def test_attention_lengths(length, page):
+    """One request alone, and beside others."""
+    _check(_case(1, 4, 2, 1, 64, page, [length], dtype=F16, seed=length))
+    _check(_case(5, 4, 2, 1, 128, page, [length, 0, 40, length, 0], dtype=BF16, seed=length))
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 80, 112, 256, 1024])
+def test_attention_page_sizes(page):
+    _check(_case(3, 8, 4, 1, 64, page, [page - 1, page, 3 * page + 5], dtype=F16, seed=page))
+
+
+@pytest.mark.parametrize("hq,hkv,sq", [(1, 1, 1), (16, 1, 1), (17, 1, 1), (28, 4, 1), (33, 1, 1), (64, 1, 1),
+                                       (65, 1, 1), (8, 8, 3), (8, 2, 5), (16, 2, 4), (32, 2, 16), (4, 1, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_rows(hq, hkv, sq, causal, d):
+    """1 to 256 packed rows per KV head: one, two and four waves, and several
+    row groups; causal rows of which the first see nothing."""
+    _check(_case(4, hq, hkv, sq, d, 16, [3, 0, 100, 259], dtype=F16, seed=hq + sq), causal=causal)
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 200])
+def test_attention_batches(batch):
+    """Runs of units over many requests, empty ones among them."""
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 300, (batch,), generator=g).tolist()
+    lengths[::7] = [0] * len(lengths[::7])
+    _check(_case(batch, 4, 2, 1, 64, 32, lengths, dtype=BF16, seed=batch))
+
+
+@pytest.mark.parametrize("hq,hkv,d,n", [(8, 8, 128, 70000), (16, 1, 64, 200000), (32, 1, 96, 40000)])
+def test_attention_long(hq, hkv, d, n):
+    """Runs of many units: one request over all workers, and beside a short."""
+    _check(_case(2, hq, hkv, 1, d, 64, [n, 100], dtype=BF16, seed=n))
+
+
+@pytest.mark.parametrize("sq", [2, 4, 16])
+@pytest.mark.parametrize("rest", [0, 1, 15, 16, 17, 40, 63])
+def test_attention_drafts(sq, rest):
+    """Causal limits anywhere in a step of 64 positions."""
+    _check(_case(3, 8, 2, sq, 128, 16, [128 + rest, 64 + rest, rest], dtype=F16, seed=sq + rest), causal=True)
+
+
+def test_attention_scales():
+    case = _case(2, 4, 2, 1, 64, 16, [70, 200], dtype=F16, seed=5)
+    for scale in (0.0, 1.0, -0.5, 1e-4):
+        _check(case, scale=scale)
+
+
+def test_attention_empty_batch_and_rows():
+    o, lse = _check(_case(3, 4, 2, 2, 64, 16, [0, 0, 0], dtype=F16, seed=1), causal=True)
+    assert not o.any() and bool((lse == -math.inf).all())
+
+
+def test_attention_junk_is_not_read():
+    """NaN codes behind a request's last row, pages of nobody, page numbers
+    outside the pool, and lengths beyond the table or below zero."""
+    q, k8, v8, scales, tables, lens = _case(4, 8, 2, 1, 64, 32, [100, 40, 64, 7], dtype=F16, seed=3)
+    scales[k8.view(torch.uint8).eq(127).all(-1).all(-1).all(-1)] = math.nan
+    tables[0, 1], tables[1, 0] = 10 ** 6, -2 ** 31
+    lens[2], lens[3] = 10 ** 6, -5
+    tables[2, 2:] = -1
+    o, lse = fp8_attention(q, k8, v8, scales, tables, lens, return_lse=True, backend="hip")
+    k, v = Cache(k8, v8, scales.nan_to_num(1)).held(F16)
+    assert_attention(o, q, k, v, tables, lens, lse=lse)
+
+
+@pytest.mark.parametrize("where", ["key", "value"])
+def test_attention_nan_in_sight(where):
+    """A NaN that a row sees makes it NaN; causal rows in front of it, and the
+    other requests and heads, stay as they are."""
+    q, k8, v8, scales, tables, lens = _case(2, 4, 2, 4, 128, 16, [90, 90], dtype=F16, seed=9)
+    clean, clean_lse = fp8_attention(q, k8, v8, scales, tables, lens, causal=True, return_lse=True, backend="hip")
+    pool = (k8 if where == "key" else v8).view(torch.uint8)
+    pool[int(tables[0, 88 // 16]), 1, 88 % 16, 5] = 0x7f
+    o, lse = fp8_attention(q, k8, v8, scales, tables, lens, causal=True, return_lse=True, backend="hip")
+    assert torch.equal(o[1], clean[1]) and torch.equal(o[0, :2], clean[0, :2])
+    assert torch.equal(o[0, 2:, :2], clean[0, 2:, :2])  # rows that see up to 86 and 87
+    if where == "key":
+        assert o[0, 2:, 2:].isnan().all() and not lse[0, 2:, 2:].isfinite().any()
+    else:
+        assert o[0, 2:, 2:, 5].isnan().all() and o[0, 2:, 2:, 6:].isfinite().all()
+
+
+def test_attention_repeats_bit_for_bit():
+    case = _case(5, 32, 4, 1, 128, 16, [4000, 1, 900, 0, 2500], dtype=BF16, seed=2)
+    first = fp8_attention(*case, return_lse=True)
+    for _ in range(5):
+        again = fp8_attention(*case, return_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_attention_layouts():
+    """Strided queries, tables and pools."""
+    q, k8, v8, scales, tables, lens = _case(3, 8, 2, 2, 64, 16, [50, 130, 9], dtype=F16, seed=4)
+    want = fp8_attention(q, k8, v8, scales, tables, lens, return_lse=True, backend="hip")
+    q2 = q.transpose(1, 2).contiguous().transpose(1, 2)
+    wide = torch.stack((k8.view(torch.uint8), v8.view(torch.uint8)), 1).view(FP8)
+    sc2 = torch.stack((scales, scales), 1)[:, 1]
+    t2 = torch.stack((tables, tables), 2)[..., 0]
+    l2 = torch.stack((lens, lens), 1)[:, 0]
+    for args in ((q2, wide[:, 0], wide[:, 1], sc2, tables, lens), (q, k8, v8, scales, t2, l2),
+                 (torch.cat((q, q), 3)[..., :64], k8, v8, scales, tables, lens)):
+        got = fp8_attention(*args, return_lse=True, backend="hip")
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_attention_paths_agree():
+    case = _case(3, 8, 2, 2, 64, 16, [50, 130, 9], dtype=F16, seed=4)
+    want = fp8_attention(*case, causal=True, return_lse=True)
+    got = hip_paged_fp8.attention_fp8(*case, causal=True, scale=0.125, with_lse=True)
+    op = torch.ops.kotflash_amd.fp8_decode(*case, True, 0.125)
+    compiled = torch.compile(lambda *a: fp8_attention(*a, causal=True, return_lse=True), fullgraph=True,
+                             backend="aot_eager")(*case)
+    for other in (got, op, compiled):
+        assert all(torch.equal(a, b) for a, b in zip(want, other))
+    sdpa = fp8_attention(*case, causal=True, return_lse=True, backend="sdpa")
+    assert (sdpa[0] - want[0]).abs().max() < 4e-3 and (sdpa[1] - want[1]).abs().max() < 2e-3
+    # What the kernels do not take, auto runs there.
+    odd = make_cache(2, 1, 24, 16, [5, 30], dtype=F16, seed=1, device="cuda")
+    out = fp8_attention(_randn(2, 4, 1, 24), *odd)
+    assert_attention(out, _randn(2, 4, 1, 24), *Cache(*odd[:3]).held(F16), *odd[3:])
+    with pytest.raises(ValueError, match="head_dim"):
+        fp8_attention(_randn(2, 4, 1, 24), *odd, backend="hip")
+
+
+def test_attention_beyond_32_bits():
+    """Pages at the far end of a pool of more than 4 GiB."""
+    pages = (5 << 30) // (2 * 16 * 128)
+    k8 = torch.empty(pages, 2, 16, 128, dtype=torch.uint8, device="cuda").view(FP8)
+    v8 = torch.empty_like(k8)
+    scales = torch.empty(pages, 2, 1, 2, device="cuda")
+    q, ks, vs, sc, tables, lens = _case(1, 4, 2, 1, 128, 16, [70], dtype=F16, seed=1)
+    far = tables.clone()
+    for c in range(5):
+        p, to = int(tables[0, c]), pages - 1 - 3 * c
+        far[0, c] = to
+        for pool, small in ((k8, ks), (v8, vs)):
+            pool.view(torch.uint8)[to] = small.view(torch.uint8)[p]
+        scales[to] = sc[p]
+    assert torch.equal(fp8_attention(q, k8, v8, scales, far, lens), fp8_attention(q, ks, vs, sc, tables, lens))
+
+
+# --- a step ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_steps_of_a_server(dtype):
+    """Rotary positions, room, store and attention together, as requests come,
+    grow and leave; against the definition over what the cache holds."""
+    batch, hq, hkv, d = 3, 8, 2, 64
+    cache = _cache(batch, hkv, d, 32, 300, dtype)
+    rot = Rotary(d, base=500.0)
+    ref = Cache(cache.k_pages, cache.v_pages, cache.scales)
+    table = cache.table
+    for step, (counts, width) in enumerate((((70, 100, 0), 100), ((1, 1, 1), 1), ((4, 2, 3), 4), ((1, 1, 1), 1), ((0, 0, 90), 90),
+                                            ((1, 1, 1), 1))):
+        if step == 3:
+            table.trim(torch.tensor([73, 102, 0], dtype=torch.int32, device="cuda"))
+        if step == 4:
+            table.trim(torch.tensor([0, 2 ** 20, 1], dtype=torch.int32, device="cuda"))
+        q, k, v = (_randn(batch, h, width, d, dtype=dtype, seed=10 * step + i) for i, h in enumerate((hq, hkv, hkv)))
+        q, k = rot(q, k, positions=table.lengths)
+        slots = table.reserve(torch.tensor(counts, dtype=torch.int32, device="cuda"), width=width)
+        o = cache.append_and_attend(q, k, v, slots)
+        ref.append(k, v, slots)
+        kd, vd = ref.held(dtype)
+        assert_attention(o, q, kd, vd, table.tables, table.lengths)
+        apart = cache.attend(q, return_lse=True)
+        assert torch.equal(o, apart[0])
+
+
+def test_step_refuses_before_it_stores():
+    cache = _cache(2, 2, 64, 16, 100)
+    slots = cache.table.reserve(1)
+    before = cache.scales.clone()
+    q, k = _randn(2, 4, 1, 64), _randn(2, 2, 1, 64)
+    for bad, error in ((dict(q=q.float()), ValueError), (dict(q=q[:, :3]), ValueError), (dict(causal=1), TypeError),
+                       (dict(attention_backend="x"), ValueError), (dict(append_backend="fused"), ValueError),
+                       (dict(new_k=k.bfloat16(), new_v=k.bfloat16()), ValueError), (dict(slots=slots.int()), ValueError)):
+        args = {"q": q, "new_k": k, "new_v": k, "slots": slots, **bad}
+        with pytest.raises(error):
+            cache.append_and_attend(args.pop("q"), args.pop("new_k"), args.pop("new_v"), args.pop("slots"), **args)
+        assert torch.equal(cache.scales, before)
+
+
+def test_step_graph_replays():
+    """A captured step follows the requests as they grow."""
+    cache, plain = (_cache(2, 2, 64, 16, 300) for _ in range(2))
+    rot = Rotary(64)
+    q0, k0, v0 = _randn(2, 8, 1, 64), _randn(2, 2, 1, 64, seed=1), _randn(2, 2, 1, 64, seed=2)
+
+    def step(c):
+        q, k = rot(q0, k0, positions=c.table.lengths)
+        slots = c.table.reserve(1)
+        return c.append_and_attend(q, k, v0, slots)
+
+    for c in (cache, plain):
+        k = _randn(2, 2, 120, 64, seed=7)
+        c.append(k, k, c.table.reserve(120))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(cache)
+    torch.cuda.current_stream().wait_stream(stream)
+    cache.table.trim(120)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(cache)
+    for i in range(20):
+        for t, s in ((q0, 0), (k0, 1), (v0, 2)):
+            t.copy_(_randn(*t.shape, seed=100 * i + s))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(plain)
+        assert torch.equal(held, want), i

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 from kotflash_amd.paged import PagedKVCache, PageTable
-from kotflash_amd.paged_fp8 import PagedKVCacheFP8, fp8_append, fp8_read
-from tests.fp8_oracle import Cache, make_cache, round_e4m3, scale_of
+from kotflash_amd.paged_fp8 import PagedKVCacheFP8, fp8_append, fp8_attention, fp8_read
+from tests.fp8_oracle import Cache, assert_attention, make_cache, round_e4m3, scale_of
 
 F16, BF16, F32, FP8 = torch.float16, torch.bfloat16, torch.float32, torch.float8_e4m3fn
 
@@ -193,3 +193,51 @@ def test_tables_that_name_no_page():
     want = ref.read(tables, lengths, 80, [0, 0], F16)
     for g, w in zip(got, want):
         assert torch.equal(g.double().nan_to_num(7), w.nan_to_num(7))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention(causal):
+    """The torch path against the definition, with its bound."""
+    k8, v8, scales, tables, lens = make_cache(3, 2, 32, 16, [0, 5, 70], dtype=F16, seed=1, wild=False)
+    q = _randn(3, 4, 3, 32)
+    k, v = Cache(k8, v8, scales).held(F32)
+    o, lse = fp8_attention(q.float(), k8, v8, scales, tables, lens, causal=causal, return_lse=True)
+    assert_attention(o, q.float(), k, v, tables, lens, lse=lse, causal=causal)
+
+
+def test_append_and_attend():
+    cache = _cache(dtype=F32, d=32)
+    ref = Cache(cache.k_pages, cache.v_pages, cache.scales)
+    for step, n in enumerate((20, 1, 3)):
+        q, k, v = (_randn(2, h, n, 32, dtype=F32, seed=10 * step + h) for h in (4, 2, 2))
+        slots = cache.table.reserve(n)
+        o = cache.append_and_attend(q, k, v, slots, causal=True)
+        ref.append(k, v, slots)
+        assert_attention(o, q, *ref.held(F32), cache.table.tables, cache.table.lengths, causal=True)
+
+
+@pytest.mark.parametrize("change,error,match", [
+    (dict(q=torch.zeros(2, 4, 32)), ValueError, "layout"), (dict(q=torch.zeros(2, 4, 0, 32)), ValueError, "non-empty"),
+    (dict(q=torch.zeros(2, 4, 1, 16)), ValueError, "head dimension"), (dict(q=torch.zeros(2, 3, 1, 32)), ValueError, "divisible"),
+    (dict(q=torch.zeros(2, 4, 1, 32).double()), ValueError, "float16"), (dict(q=torch.zeros(3, 4, 1, 32)), ValueError, "tables"),
+    (dict(causal=1), TypeError, "causal"), (dict(scale="x"), TypeError, "scale"), (dict(scale=math.inf), ValueError, "finite"),
+    (dict(backend="torch"), ValueError, "backend"), (dict(backend="hip"), RuntimeError, "gfx950"),
+    (dict(q=torch.zeros(2, 4, 1, 32).requires_grad_()), RuntimeError, "inference"),
+])
+def test_attention_refusals(change, error, match):
+    k, v, scales, tables, lengths = make_cache(2, 2, 32, 16, [3, 20], dtype=F16, seed=0)
+    a = dict(q=torch.zeros(2, 4, 1, 32))
+    a.update(change)
+    with pytest.raises(error, match=match):
+        fp8_attention(a.pop("q"), k, v, scales, tables, lengths, **a)
+
+
+def test_step_refuses_before_it_stores():
+    cache = _cache()
+    slots = cache.table.reserve(1)
+    q, k = _randn(2, 4, 1, 32), _randn(2, 2, 1, 32)
+    for args, kw in (((q.float(), k, k, slots), {}), ((q, k.float(), k.float(), slots), {}), ((q, k, k, slots), dict(causal=2)),
+                     ((q, k, k, slots), dict(append_backend="fused"))):
+        with pytest.raises((ValueError, TypeError)):
+            cache.append_and_attend(*args, **kw)
+        assert not cache.scales.any()
