@@ -267,6 +267,7 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
     p.scales = scales.at;
     p.sc_page = (uint32_t)(4 * scales.strides[0]);
     p.sc_head = (uint32_t)(4 * scales.strides[1]);
+    p.row_rest = (int)(k_strides[2] - D);
   }
   p.o_sb = o_strides[0]; p.o_sh = o_strides[1]; p.o_ss = o_strides[2];
   p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.Sq = (int)Sq; p.D = (int)D; p.G = (int)(Hq / Hkv);
@@ -350,6 +351,10 @@ static int check_fp8_sizes(const char* what, int64_t Hkv, int64_t D, const int64
   for (const int64_t* s : {k_strides, v_strides})
     if (s[0] % 16 || s[1] % 16 || s[2] % 16)
       return set_error(KF_EINVAL, "%s: pool strides must be multiples of 16 bytes", what);
+  if (k_strides[0] != v_strides[0] || k_strides[1] != v_strides[1] || k_strides[2] != v_strides[2])
+    return set_error(KF_EINVAL, "%s: K and V pools must have the same strides", what);
+  if (k_strides[2] < D || 16 * k_strides[2] > 0x7fffffff)
+    return set_error(KF_EUNSUPPORTED, "%s: rows of a page overlap, or span more than 2 GiB", what);
   if (scale_strides[0] % 2 || scale_strides[1] % 2)
     return set_error(KF_EINVAL, "%s: scale strides must be multiples of a pair", what);
   if (scale_strides[0] < 0 || scale_strides[0] >= 1 << 30 || scale_strides[1] < 0 || scale_strides[1] >= 1 << 30)

@@ -92,6 +92,7 @@ struct PagedParams {
   // 8-bit pools: the blocks' scales, in pairs (K, V); bytes per page and head.
   const float* scales;
   uint32_t sc_page, sc_head;
+  int row_rest;  // k_row without the row's own bytes
 };
 
 // Direct-to-LDS loads (kf_common.hpp) of whole tiles: N loads of 1 KB, one
@@ -480,8 +481,6 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     constexpr int slot = decltype(slot_c)::value;
     const uint32_t kv0 = lds0 + slot * 2 * VT * 2;
     if constexpr (FUSED) store_hits();
-    int q = part;
-    if constexpr (KV8) valid[slot] = 0;
     if (at.begin) {
       const auto& c = cold();
       const int kvh = at.hh / c.nrb;
@@ -497,28 +496,60 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
         dma_tile<NQ, false>(qr, q0, off);
       }
     }
+    if constexpr (KV8) {
+      // K and V have the same strides, and the scalar unit, which has twice the
+      // groups of a 16-bit step to look after, computes a group's offset once.
+      uint32_t id[GROUPS], row[GROUPS];
+      int left[GROUPS];  // visible rows from the group on
+      int q = part, ok = 0;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
+      for (int g = 0; g < GROUPS; ++g) {
+        id[g] = __builtin_amdgcn_readfirstlane(page[g]);
+        const bool in = id[g] < (uint32_t)p.pages;
+        ok |= (int)in << g;
+        id[g] = in ? id[g] : 0;
+        left[g] = in ? at.rem - 16 * g : 0;
+        row[g] = q * 16;
+        q = q + 1 == p.gpp ? 0 : q + 1;
+        scale8[slot][g] = *(const f32x2 KF_CONST*)(sh + (uint64_t)id[g] * p.sc_page + row[g] / 2);
+      }
+      valid[slot] = ok;
+      // One wave loads all groups; of two, each every other; of four, K or V of
+      // those. The extent ends with the last visible row; none of a page outside
+      // the pool is.
+      const int odd = wave & 1;
+      auto send = [&](auto nt) {
+#pragma unroll
+        for (int j = 0; j < (NW > 1 ? GROUPS / 2 : GROUPS); ++j) {
+          const int g = NW > 1 ? 2 * j : j, mine = NW > 1 ? g + odd : g;
+          const uint32_t i = NW > 1 && odd ? id[g + 1] : id[g], r = NW > 1 && odd ? row[g + 1] : row[g];
+          const uint64_t off = (uint64_t)i * p.k_page + r * p.k_row;
+          const int rows = min(NW > 1 && odd ? left[g + 1] : left[g], 16);
+          const int extent = max(rows * (int)p.k_row - p.row_rest, 0);
+          const uint32_t m0 = kv0 + mine * 16 * DT;
+          if (NW < 4) {
+            dma_tile<NGI, decltype(nt)::value>(make_rsrc((const void*)(uintptr_t)(kh + off), extent), m0, koff);
+            dma_tile<NGI, decltype(nt)::value>(make_rsrc((const void*)(uintptr_t)(vh + off), extent), m0 + VT * 2, koff);
+          } else {
+            const uint64_t base = wave < 2 ? kh : vh;
+            dma_tile<NGI, decltype(nt)::value>(make_rsrc((const void*)(uintptr_t)(base + off), extent),
+                                               m0 + (wave < 2 ? 0 : VT * 2), koff);
+          }
+        }
+      };
+      if (stream) send(std::true_type{});
+      else send(std::false_type{});
+    }
+#pragma unroll
+    for (int g = 0; g < (KV8 ? 0 : GROUPS); ++g) {
       const uint32_t m0 = kv0 + g * 16 * DT * EB;
       const uint32_t id = __builtin_amdgcn_readfirstlane(page[g]);
-      int row;
-      if constexpr (KV8) {
-        row = q * 16;
-        if (++q == p.gpp) q = 0;
-      } else {
-        row = g == 0 ? part * 16 : row1;
-      }
+      const int row = g == 0 ? part * 16 : row1;
       int rows = at.rem - 16 * g;
       rows = rows < 0 || id >= (uint32_t)p.pages ? 0 : rows < 16 ? rows : 16;
-      if constexpr (KV8) {
-        const bool in = id < (uint32_t)p.pages;
-        valid[slot] |= (int)in << g;
-        scale8[slot][g] = *(const f32x2 KF_CONST*)(sh + (in ? (uint64_t)id * p.sc_page + (uint32_t)row / 2 : 0));
-      } else {
-        seen[slot][g] = rows;
-      }
-      // One wave loads all groups; of two, each every other; of four, K or V of those.
-      if (NW > 1 && (wave & 1) != (g & 1)) continue;
+      seen[slot][g] = rows;
+      // One wave loads both groups; of two, each a group; of four, K or V of one.
+      if (NW > 1 && (wave & 1) != g) continue;
       // The extent ends with the last visible row.
       if (NW < 4 || wave < 2) {
         const uint64_t ka = kh + (rows ? (uint64_t)id * p.k_page + (uint32_t)row * (uint64_t)p.k_row : 0);

@@ -108,10 +108,16 @@ __device__ inline u32x2 rescale(u32x2 x, float ratio) {
   return out;
 }
 
+// Bytes of new keys and values from which the codes' stores are marked as not
+// read again soon (us, plain and marked: 17 MB of them 6.5 and 6.1, 33 MB 8.9
+// and 7.9, 134 MB 21.3 and 19.9, 268 MB 45.1 and 39.2; marked loads 40.4, both
+// 42.1). A step's rows are read next.
+constexpr int64_t kStreamRows = 16 << 20;
+
 // A wave per request, window of 16 new tokens and head: it stores the runs of
 // tokens of one block that begin in its window (one, in a prompt), so that
 // every block has one wave. `lanes` lanes hold a row, eight elements each.
-template <typename T, int PASSES>
+template <typename T, int PASSES, bool STREAM>
 __global__ __launch_bounds__(256) void fp8_store_kernel(const Fp8StoreParams p) {
   const int lane = threadIdx.x & 63;
   const int w = blockIdx.x * 4 + wave_index();
@@ -224,8 +230,16 @@ __global__ __launch_bounds__(256) void fp8_store_kernel(const Fp8StoreParams p) 
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       if (place[i] < 0) continue;
-      *(u32x2*)(kb + place[i] * p.kp_ss + d) = quantise<T>(kx[i], kinv, klimit, special);
-      *(u32x2*)(vb + place[i] * p.vp_ss + d) = quantise<T>(vx[i], vinv, vlimit, special);
+      const u32x2 k8 = quantise<T>(kx[i], kinv, klimit, special), v8 = quantise<T>(vx[i], vinv, vlimit, special);
+      u32x2* ka = (u32x2*)(kb + place[i] * p.kp_ss + d);
+      u32x2* va = (u32x2*)(vb + place[i] * p.vp_ss + d);
+      if constexpr (STREAM) {
+        __builtin_nontemporal_store(k8, ka);
+        __builtin_nontemporal_store(v8, va);
+      } else {
+        *ka = k8;
+        *va = v8;
+      }
     }
     if (lane == 0) *(f32x2*)sc = f32x2{power(ek), power(ev)};
   }
@@ -248,24 +262,24 @@ struct Fp8ReadParams {
   int64_t ko_sb, ko_sh, ko_ss;
   int64_t vo_sb, vo_sh, vo_ss;
   int64_t cap;            // tokens that a table has columns for
-  int items;              // 16-element pieces of a request and head
+  int items;              // 8-element pieces of a request and head
   Divisor blocks;         // workgroups of a request and head
   Divisor heads, pieces;  // pieces of a row
   Divisor page;
   int pages;
 };
 
+// Eight codes times their block's scale.
 template <typename T>
-__device__ inline void dequantise(u32x4 codes, float scale, u32x4* out) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    out[j / 2][2 * (j % 2)] = dequantise2<T, false>(codes[j], scale);
-    out[j / 2][2 * (j % 2) + 1] = dequantise2<T, true>(codes[j], scale);
-  }
+__device__ inline u32x4 dequantise(u32x2 codes, float scale) {
+  return {dequantise2<T, false>(codes[0], scale), dequantise2<T, true>(codes[0], scale),
+          dequantise2<T, false>(codes[1], scale), dequantise2<T, true>(codes[1], scale)};
 }
 
-// A thread per 16 elements of a row of K and of V.
-template <typename T>
+// A thread per 8 elements of a row of K and of V: a wave's stores are whole
+// kilobytes. HBM-bound: 459 MB written and 229 read 117 us, 5.9 TB/s; 16
+// elements per thread 143, two or four rows per thread 121 and 127.
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void fp8_read_kernel(const Fp8ReadParams p) {
   const int bh = quotient(blockIdx.x, p.blocks);
   const int item = ((int)blockIdx.x - bh * (int)p.blocks.d) * 256 + threadIdx.x;
@@ -273,29 +287,37 @@ __global__ __launch_bounds__(256) void fp8_read_kernel(const Fp8ReadParams p) {
   const int64_t b = quotient(bh, p.heads);
   const int h = bh - (int)b * (int)p.heads.d;
   const int t = quotient(item, p.pieces);
-  const int d = (item - t * (int)p.pieces.d) * 16;
+  const int d = (item - t * (int)p.pieces.d) * 8;
   int64_t first = p.starts ? p.starts[b] : p.start;
   first = first < 0 ? 0 : first;
   const int64_t held = p.lengths[b], at = first + t;
-  u32x4 k[2] = {zero_u4(), zero_u4()}, v[2] = {zero_u4(), zero_u4()};
+  u32x4 k = zero_u4(), v = zero_u4();
   if (at < held && at < p.cap) {
     const int column = quotient((int)at, p.page), row = (int)at - column * (int)p.page.d;
     const int id = p.tables[b * p.t_sb + column];
     if (id >= 0 && id < p.pages) {
-      const u32x4 kk = ldg16(p.kp + id * p.kp_sp + h * p.kp_sh + row * p.kp_ss + d);
-      const u32x4 vv = ldg16(p.vp + id * p.vp_sp + h * p.vp_sh + row * p.vp_ss + d);
+      const u32x2 k8 = *(const u32x2*)(p.kp + id * p.kp_sp + h * p.kp_sh + row * p.kp_ss + d);
+      const u32x2 v8 = *(const u32x2*)(p.vp + id * p.vp_sp + h * p.vp_sh + row * p.vp_ss + d);
       const f32x2 s = *(const f32x2*)(p.scales + id * p.sc_sp + h * p.sc_sh + (row >> 4) * 2);
-      dequantise<T>(kk, s[0], k);
-      dequantise<T>(vv, s[1], v);
+      k = dequantise<T>(k8, s[0]);
+      v = dequantise<T>(v8, s[1]);
     }
   }
-  uint16_t* ko = p.ko + b * p.ko_sb + h * p.ko_sh + t * p.ko_ss + d;
-  uint16_t* vo = p.vo + b * p.vo_sb + h * p.vo_sh + t * p.vo_ss + d;
-  stg16(ko, k[0]);
-  stg16(ko + 8, k[1]);
-  stg16(vo, v[0]);
-  stg16(vo + 8, v[1]);
+  u32x4* ko = (u32x4*)(p.ko + b * p.ko_sb + h * p.ko_sh + t * p.ko_ss + d);
+  u32x4* vo = (u32x4*)(p.vo + b * p.vo_sb + h * p.vo_sh + t * p.vo_ss + d);
+  if constexpr (STREAM) {
+    __builtin_nontemporal_store(k, ko);
+    __builtin_nontemporal_store(v, vo);
+  } else {
+    *ko = k;
+    *vo = v;
+  }
 }
+
+// Bytes of K and V from which the read's stores are marked as not read again
+// soon (us, plain and marked: 67 MB 14.0 and 13.8, 134 MB 24.9 and 24.6, 268 MB 67
+// and 46, beyond what the memory-side cache takes; 459 MB 128 and 117).
+constexpr int64_t kStreamReads = 128 << 20;
 
 int check_fp8_pools(const char* what, const void* k_pages, const void* v_pages, const void* scales, int64_t H,
                     int64_t D, int64_t num_pages, int64_t page_size, const int64_t* k_strides,
@@ -359,17 +381,19 @@ extern "C" int kf_fp8_append(void* k_pages, void* v_pages, float* scales, const 
   p.rows = 64 / p.lanes;
   const dim3 grid((unsigned)((p.waves + 3) / 4)), block(256);
   hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto type) {
+  auto launch = [&](auto type, auto once) {
     using T = decltype(type);
+    constexpr bool S = decltype(once)::value;
     switch (cdiv(16, p.rows)) {
-      case 1: hipLaunchKernelGGL((fp8_store_kernel<T, 1>), grid, block, 0, st, p); break;
-      case 2: hipLaunchKernelGGL((fp8_store_kernel<T, 2>), grid, block, 0, st, p); break;
-      case 3: hipLaunchKernelGGL((fp8_store_kernel<T, 3>), grid, block, 0, st, p); break;
-      default: hipLaunchKernelGGL((fp8_store_kernel<T, 4>), grid, block, 0, st, p); break;
+      case 1: hipLaunchKernelGGL((fp8_store_kernel<T, 1, S>), grid, block, 0, st, p); break;
+      case 2: hipLaunchKernelGGL((fp8_store_kernel<T, 2, S>), grid, block, 0, st, p); break;
+      case 3: hipLaunchKernelGGL((fp8_store_kernel<T, 3, S>), grid, block, 0, st, p); break;
+      default: hipLaunchKernelGGL((fp8_store_kernel<T, 4, S>), grid, block, 0, st, p); break;
     }
   };
-  if (dtype == KF_F16) launch(_Float16{});
-  else launch(__bf16{});
+  const bool once = B * H * Snew * D * 4 >= kStreamRows;
+  if (dtype == KF_F16) once ? launch(_Float16{}, std::true_type{}) : launch(_Float16{}, std::false_type{});
+  else once ? launch(__bf16{}, std::true_type{}) : launch(__bf16{}, std::false_type{});
   return check_launch(what);
 }
 
@@ -393,7 +417,7 @@ extern "C" int kf_fp8_read(const void* k_pages, const void* v_pages, const float
     return set_error(KF_EUNSUPPORTED, "%s: a table of %lld pages of %lld tokens is beyond 32-bit positions", what,
                      (long long)columns, (long long)page_size);
   Fp8ReadParams p{};
-  const int64_t pieces = D / 16, blocks = (width * pieces + 255) / 256;
+    const int64_t pieces = D / 8, blocks = (width * pieces + 255) / 256;
   if (width > 0x3fffffff / pieces || start > 0x3fffffff)
     return set_error(KF_EUNSUPPORTED, "%s: width or start too large", what);
   if (B > 0x7fffffff / H || B * H > ((1ll << 24) - 1) / blocks) return set_error(KF_EUNSUPPORTED, "%s: grid too large", what);
@@ -412,7 +436,14 @@ extern "C" int kf_fp8_read(const void* k_pages, const void* v_pages, const float
   p.cap = columns * page_size;
   p.page = divisor((uint32_t)page_size); p.pages = (int)num_pages;
   const dim3 grid((unsigned)(B * H * blocks));
-  if (dtype == KF_F16) hipLaunchKernelGGL(fp8_read_kernel<_Float16>, grid, dim3(256), 0, (hipStream_t)stream, p);
-  else hipLaunchKernelGGL(fp8_read_kernel<__bf16>, grid, dim3(256), 0, (hipStream_t)stream, p);
+  const bool once = B * H * width * D * 4 >= kStreamReads;
+  hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    if (once) hipLaunchKernelGGL((fp8_read_kernel<T, true>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((fp8_read_kernel<T, false>), grid, dim3(256), 0, st, p);
+  };
+  if (dtype == KF_F16) launch(_Float16{});
+  else launch(__bf16{});
   return check_launch(what);
 }
