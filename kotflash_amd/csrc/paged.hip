@@ -344,7 +344,7 @@ extern "C" int kf_paged_append_decode(const void* q, void* k_pages, void* v_page
 }
 
 // 8-bit pools: head_dim and strides in whole 16-byte pieces.
-static int check_fp8_sizes(const char* what, int64_t Hkv, int64_t D, const int64_t* k_strides, const int64_t* v_strides,
+static int check_fp8_sizes(const char* what, int64_t D, int64_t num_pages, const int64_t* k_strides, const int64_t* v_strides,
                            const int64_t* scale_strides) {
   if (!scale_strides) return set_error(KF_EINVAL, "%s: null strides", what);
   if (D % 16) return set_error(KF_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", what);
@@ -357,8 +357,10 @@ static int check_fp8_sizes(const char* what, int64_t Hkv, int64_t D, const int64
     return set_error(KF_EUNSUPPORTED, "%s: rows of a page overlap, or span more than 2 GiB", what);
   if (scale_strides[0] % 2 || scale_strides[1] % 2)
     return set_error(KF_EINVAL, "%s: scale strides must be multiples of a pair", what);
-  if (scale_strides[0] < 0 || scale_strides[0] >= 1 << 30 || scale_strides[1] < 0 || scale_strides[1] >= 1 << 30)
-    return set_error(KF_EUNSUPPORTED, "%s: scales of a page or head more than 4 GiB apart", what);
+  // The scalar unit adds a page's offset to a head's in 32 bits.
+  if (scale_strides[0] < 0 || scale_strides[1] < 0 || scale_strides[1] >= 1 << 30 ||
+      scale_strides[0] > (1ll << 30) / num_pages - 1)
+    return set_error(KF_EUNSUPPORTED, "%s: scales of a head span more than 4 GiB", what);
   return KF_OK;
 }
 
@@ -366,7 +368,7 @@ extern "C" int kf_fp8_decode_check(int64_t B, int64_t Hq, int64_t Hkv, int64_t S
                                    int64_t page_size, int64_t columns, const int64_t* q_strides,
                                    const int64_t* k_strides, const int64_t* v_strides, const int64_t* scale_strides) {
   const int rc = kf_paged_decode_check(B, Hq, Hkv, Sq, D, num_pages, page_size, columns, q_strides, k_strides, v_strides);
-  return rc ? rc : check_fp8_sizes("kf_fp8_decode", Hkv, D, k_strides, v_strides, scale_strides);
+  return rc ? rc : check_fp8_sizes("kf_fp8_decode", D, num_pages, k_strides, v_strides, scale_strides);
 }
 
 extern "C" int kf_fp8_decode(const void* q, const void* k_pages, const void* v_pages, const float* scales, void* o,
@@ -379,7 +381,7 @@ extern "C" int kf_fp8_decode(const void* q, const void* k_pages, const void* v_p
   const char* what = "kf_fp8_decode";
   if (!scales || !aligned8(scales)) return set_error(KF_EINVAL, "%s: scales must be non-null and 8-byte aligned", what);
   if (!k_strides || !v_strides) return set_error(KF_EINVAL, "%s: null strides", what);
-  const int rc = check_fp8_sizes(what, Hkv, D, k_strides, v_strides, scale_strides);
+  const int rc = check_fp8_sizes(what, D, num_pages, k_strides, v_strides, scale_strides);
   if (rc) return rc;
   return paged_entry(what, q, k_pages, v_pages, Scales{scales, scale_strides}, NewRows{}, o, lse, tables, lengths, B,
                      Hq, Hkv, Sq, D, num_pages, page_size, columns, table_stride, q_strides, k_strides, v_strides,

@@ -9,7 +9,7 @@
 //
 // How the work is cut. The lengths are known on the GPU only (a captured graph
 // replays with others), so the launch cannot be planned on the host. All
-// requests' keys are numbered in steps of 32: unit u = (request, KV head and
+// requests' keys are numbered in steps of 32 (64 in 8 bits): unit u = (request, KV head and
 // row group of up to 64 packed query rows, step). A fixed number of workers, as
 // many as the GPU holds at once, take equal runs of consecutive units, wherever
 // requests begin and end in them: every worker streams the same number of bytes
@@ -41,6 +41,17 @@
 // larger than 4 GiB) and an extent that ends at the last visible row: rows
 // behind it load as zeros, whatever the page holds there (NaN included), and a
 // page number outside the pool reads nothing and its keys are masked.
+//
+// Pools in 8 bits (KV8) hold e4m3 codes, and a scale per 16 rows and head, a power
+// of two. The codes stay codes through the LDS; a conversion that multiplies by
+// the scale makes two 16-bit elements of them in front of the matrix units,
+// exactly, so that the products, and what is rounded, are those of the 16-bit
+// cache. A step has 64 keys, for the same bytes in flight. Half the bytes per
+// key leave the scalar unit, which builds a resource per 16 rows and reads pages
+// and scales, and the vector unit half the time for each key: 64 requests of 512
+// to 8192 tokens (Hq=32 Hkv=8), 16-bit and 8-bit, D=128 185 and 102 us, D=64 100
+// and 59: 6.2, 5.7, 5.8 and 5.0 TB/s. What is left at D=64 is the tail: equal runs
+// end after 40 to 50 us, by where on the chip they are.
 #pragma once
 #include "decode_merge.hpp"
 #include "fp8.hpp"
@@ -511,7 +522,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
         left[g] = in ? at.rem - 16 * g : 0;
         row[g] = q * 16;
         q = q + 1 == p.gpp ? 0 : q + 1;
-        scale8[slot][g] = *(const f32x2 KF_CONST*)(sh + (uint64_t)id[g] * p.sc_page + row[g] / 2);
+        scale8[slot][g] = *(const f32x2 KF_CONST*)(sh + (uint64_t)(id[g] * p.sc_page + row[g] / 2));
       }
       valid[slot] = ok;
       // One wave loads all groups; of two, each every other; of four, K or V of
@@ -815,10 +826,19 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     }
   };
   bool ended = false;
+  // Of two workers on a SIMD the older one goes first, ends first, and leaves the
+  // other alone with half the loads in flight (291 MB, D=64: after 40 and 50 us).
+  // The younger one goes first in three units of four: 60.2 -> 58.6 us; in every
+  // other one 59.7, always 60.1.
+  const bool late = worker >= (int)gridDim.x / 2;
   for (int j0 = -2; j0 < count; j0 += 2) {
     static_for<0, 2>([&](auto sc) {
       constexpr int slot = decltype(sc)::value;
       const int j = j0 + slot;
+      if constexpr (KV8 && NW == 1 && workers_per_cu(DT, NW) > 4) {
+        if (late && j % 4 != 0) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+      }
       if (j >= 0 && j < count) {
         const bool next = j + 1 < count;
         wait(ended, next ? held[1 - slot].begin ? 2 : 1 : 0);
