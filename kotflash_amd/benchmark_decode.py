@@ -17,11 +17,14 @@ The same arguments and report fields as the reference's decode benchmark
   kernel that also writes the new token, then the merge);
 - with ``--page-size N``, ``paged_auto``: ``PagedKVCache``, every sequence's
   pages in no order, its step the table's reserve, the store and the attention
-  (and the trim that takes the token back).
+  (and the trim that takes the token back); with ``--kv-fp8`` too,
+  ``paged_fp8_auto``: the same with ``PagedKVCacheFP8``.
 
 Every candidate's output, attention alone and append + attention, is
 checked against the expanded-SDPA output first (rtol = atol = 8e-3, the
-reference's figure; the reference checks the attention-only output). Per
+reference's figure; the reference checks the attention-only output), that of
+the 8-bit cache against expanded SDPA over the keys and values as it holds
+them. Per
 candidate and metric the report gives GPU-event and synchronized wall-clock medians,
 minima and maxima over ``--repeats`` repeats of ``--iterations`` calls, the
 incremental peak of allocated memory, and speedups against the baseline.
@@ -45,6 +48,7 @@ from .attention import attention
 from .benchmark import _environment, _sync
 from .cache import PreallocatedKVCache, append_kv_cache
 from .paged import PagedKVCache, PageTable
+from .paged_fp8 import PagedKVCacheFP8
 
 APPEND_BACKENDS = ("auto", "torch", "hip", "cuda", "fused")
 
@@ -110,6 +114,8 @@ def run(args: argparse.Namespace) -> dict:
     decode_cache = PreallocatedKVCache(b, hkv, capacity, d, device=device, dtype=dtype)
     decode_cache.append(past_k, past_v, backend="torch")
 
+    references = {}  # of candidates that do not attend to visible_k and visible_v
+
     def expanded(k, v):
         return F.scaled_dot_product_attention(q, k.repeat_interleave(group, 1),
                                               v.repeat_interleave(group, 1))
@@ -135,7 +141,7 @@ def run(args: argparse.Namespace) -> dict:
                                                   attention_backend=attend_backend)
         return attend, decode
 
-    def paged(page):
+    def paged(page, cache_type):
         """Two caches behind tables of their own: one that holds all tokens,
         one that takes the last at every step."""
         pages = -(-sk // page)
@@ -143,7 +149,7 @@ def run(args: argparse.Namespace) -> dict:
         for held, k, v in ((sk, visible_k, visible_v), (sk - 1, past_k, past_v)):
             table = PageTable(b, sk, num_pages=b * pages, page_size=page, device=device)
             table.free_pages.copy_(torch.randperm(b * pages, generator=gen))
-            cache = PagedKVCache(table, hkv, d, dtype=dtype)
+            cache = cache_type(table, hkv, d, dtype=dtype)
             cache.append(k, v, table.reserve(held))
             caches.append(cache)
         whole, growing = caches
@@ -166,7 +172,15 @@ def run(args: argparse.Namespace) -> dict:
         "preallocated_fused_append": preallocated("hip", "fused"),
     }
     if args.page_size:
-        candidates["paged_auto"] = paged(args.page_size)
+        candidates["paged_auto"] = paged(args.page_size, PagedKVCache)
+    if args.kv_fp8:
+        candidates["paged_fp8_auto"] = paged(args.page_size, PagedKVCacheFP8)
+        table = PageTable(b, sk, num_pages=b * -(-sk // 16), device=device)
+        held = PagedKVCacheFP8(table, hkv, d, dtype=dtype)
+        held.append(past_k, past_v, table.reserve(sk - 1))
+        held.append(new_k, new_v, table.reserve(1))
+        references["paged_fp8_auto"] = expanded(*held.read(sk))
+        del table, held
     failures = {}
     correctness = {}
     with torch.inference_mode():
@@ -180,9 +194,10 @@ def run(args: argparse.Namespace) -> dict:
                 except (RuntimeError, ValueError, TypeError) as exc:
                     failures[name] = f"{type(exc).__name__}: {exc}"
                     break
-                err = float((out.float() - reference.float()).abs().max())
+                want = references.get(name, reference).float()
+                err = float((out.float() - want).abs().max())
                 finite = bool(torch.isfinite(out).all())
-                close = bool(torch.allclose(out.float(), reference.float(), rtol=8e-3, atol=8e-3))
+                close = bool(torch.allclose(out.float(), want, rtol=8e-3, atol=8e-3))
                 checks[metric] = {"max_abs_error_vs_expanded_sdpa": err, "finite": finite,
                                   "within_tolerance": close}
                 if not (finite and close):
@@ -249,6 +264,8 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
                     help="append implementation of the preallocated_auto candidate")
     ap.add_argument("--page-size", type=int, default=0,
                     help="also time a paged cache with pages of this many tokens (0: no)")
+    ap.add_argument("--kv-fp8", action="store_true",
+                    help="also time a paged cache in 8 bits (with --page-size, a multiple of 16)")
     ap.add_argument("--seed", type=int, default=1337)
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--output", type=Path, default=None)
@@ -261,6 +278,8 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
         ap.error("the split-KV decode needs --head-dim a multiple of 8 in [8, 128]")
     if args.page_size < 0:
         ap.error("--page-size must not be negative")
+    if args.kv_fp8 and (args.page_size == 0 or args.page_size % 16):
+        ap.error("--kv-fp8 needs --page-size, a multiple of 16")
     if args.kv_seq < 1024:
         ap.error("the split-KV decode benchmark needs --kv-seq >= 1024")
     if args.warmup < 1 or args.iterations < 1 or args.repeats < 3:

@@ -17,6 +17,9 @@ arguments and report fields as the reference's decoder-block benchmark
   finite.
 - Backends are ``sdpa_expanded_kv``, ``sdpa_native_gqa`` and ``hip`` (this
   build's kernels; the reference's ``triton`` slot).
+- With ``--rotary half`` or ``interleaved`` (the reference's block has none)
+  queries and keys are turned by their positions before the attention: by the
+  HIP kernel for ``hip``, in torch operations for the others.
 """
 from __future__ import annotations
 
@@ -31,6 +34,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .attention import attention
+from .rotary import Rotary
 
 BACKENDS = ("sdpa_expanded_kv", "sdpa_native_gqa", "hip")
 
@@ -39,11 +43,12 @@ class DecoderBlock(nn.Module):
     """Pre-norm decoder block with GQA/MQA projections and a gated MLP."""
 
     def __init__(self, q_heads: int, kv_heads: int, head_dim: int, mlp_ratio: int = 4,
-                 attention_dtype: torch.dtype = torch.float16):
+                 attention_dtype: torch.dtype = torch.float16, rotary: Optional[Rotary] = None):
         super().__init__()
         hidden, kv_width = q_heads * head_dim, kv_heads * head_dim
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.attention_dtype = attention_dtype
+        self.rotary = rotary
         self.norm1 = nn.LayerNorm(hidden)
         self.q_proj = nn.Linear(hidden, hidden, bias=False)
         self.k_proj = nn.Linear(hidden, kv_width, bias=False)
@@ -64,6 +69,8 @@ class DecoderBlock(nn.Module):
         q = self._heads(self.q_proj(h), self.q_heads)
         k = self._heads(self.k_proj(h), self.kv_heads)
         v = self._heads(self.v_proj(h), self.kv_heads)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, backend="hip" if backend == "hip" else "torch")
         if backend == "hip":
             a = attention(q, k, v, causal=True, backend="hip")
         elif backend == "sdpa_native_gqa":
@@ -80,6 +87,12 @@ class DecoderBlock(nn.Module):
         return x + self.down_proj(F.silu(self.gate_proj(h)) * self.up_proj(h))
 
 
+def _rotary(args, device) -> Optional[Rotary]:
+    if args.rotary == "none":
+        return None
+    return Rotary(args.head_dim, interleaved=args.rotary == "interleaved", device=device)
+
+
 def _train_step(model, opt, x, target, backend):
     opt.zero_grad(set_to_none=True)
     loss = F.mse_loss(model(x, backend), target)
@@ -89,8 +102,8 @@ def _train_step(model, opt, x, target, backend):
 
 
 def _run_backend(backend, state, x, target, args, attention_dtype) -> dict:
-    model = DecoderBlock(args.q_heads, args.kv_heads, args.head_dim,
-                         attention_dtype=attention_dtype).to(x.device)
+    model = DecoderBlock(args.q_heads, args.kv_heads, args.head_dim, attention_dtype=attention_dtype,
+                         rotary=_rotary(args, x.device)).to(x.device)
     model.load_state_dict(state)
     opt = torch.optim.AdamW(model.parameters(), lr=1e-4)
     for _ in range(args.warmup):
@@ -137,14 +150,15 @@ def run(args: argparse.Namespace) -> dict:
                   "kv_heads": args.kv_heads, "head_dim": args.head_dim, "hidden_size": hidden},
         "model_parameter_dtype": "torch.float32",
         "attention_compute_dtype": str(attention_dtype),
+        "rotary": args.rotary,
         "optimizer": "AdamW with fp32 master parameters",
         "warmup": args.warmup,
         "iterations": args.iterations,
     }
     backends = list(BACKENDS)
     try:
-        ref_model = DecoderBlock(args.q_heads, args.kv_heads, args.head_dim,
-                                 attention_dtype=attention_dtype).to(device)
+        ref_model = DecoderBlock(args.q_heads, args.kv_heads, args.head_dim, attention_dtype=attention_dtype,
+                                 rotary=_rotary(args, device)).to(device)
         ref_model.load_state_dict(state)
         with torch.no_grad():
             ref = ref_model(x, "sdpa_expanded_kv")
@@ -175,7 +189,10 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
     p.add_argument("--warmup", type=int, default=3)
     p.add_argument("--iterations", type=int, default=10)
     p.add_argument("--attention-dtype", choices=("fp16", "bf16"), default="fp16")
+    p.add_argument("--rotary", choices=("none", "half", "interleaved"), default="none")
     args = p.parse_args(argv)
+    if args.rotary != "none" and args.head_dim % 2:
+        p.error("--rotary needs an even --head-dim")
     if min(args.batch, args.seq, args.q_heads, args.kv_heads, args.head_dim) <= 0:
         p.error("batch, sequence length, head counts and head dimension must be positive")
     if args.q_heads % args.kv_heads:

@@ -347,7 +347,7 @@ extern "C" int kf_paged_append_decode(const void* q, void* k_pages, void* v_page
 static int check_fp8_sizes(const char* what, int64_t D, int64_t num_pages, const int64_t* k_strides, const int64_t* v_strides,
                            const int64_t* scale_strides) {
   if (!scale_strides) return set_error(KF_EINVAL, "%s: null strides", what);
-  if (D % 16) return set_error(KF_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", what);
+  if (D % 16 || D > 128) return set_error(KF_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", what);
   for (const int64_t* s : {k_strides, v_strides})
     if (s[0] % 16 || s[1] % 16 || s[2] % 16)
       return set_error(KF_EINVAL, "%s: pool strides must be multiples of 16 bytes", what);
@@ -359,7 +359,7 @@ static int check_fp8_sizes(const char* what, int64_t D, int64_t num_pages, const
     return set_error(KF_EINVAL, "%s: scale strides must be multiples of a pair", what);
   // The scalar unit adds a page's offset to a head's in 32 bits.
   if (scale_strides[0] < 0 || scale_strides[1] < 0 || scale_strides[1] >= 1 << 30 ||
-      scale_strides[0] > (1ll << 30) / num_pages - 1)
+      scale_strides[0] > (1ll << 30) / (num_pages > 0 ? num_pages : 1) - 1)
     return set_error(KF_EUNSUPPORTED, "%s: scales of a head span more than 4 GiB", what);
   return KF_OK;
 }

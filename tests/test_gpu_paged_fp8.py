@@ -496,3 +496,65 @@ def test_step_graph_replays():
         torch.cuda.synchronize()
         want = step(plain)
         assert torch.equal(held, want), i
+
+
+def test_step_under_compile():
+    """A step is one graph of its ops, to the same bits."""
+    caches = [_cache(2, 2, 64, 16, 300) for _ in range(2)]
+    rot = Rotary(64)
+    q, k, v = _randn(2, 8, 1, 64), _randn(2, 2, 1, 64, seed=1), _randn(2, 2, 1, 64, seed=2)
+
+    def step(c, q, k, v):
+        q, k = rot(q, k, positions=c.table.lengths)
+        return c.append_and_attend(q, k, v, c.table.reserve(1))
+
+    compiled = torch.compile(lambda *a: step(caches[0], *a), fullgraph=True, backend="aot_eager")
+    for c in caches:
+        old = _randn(2, 2, 90, 64, seed=7)
+        c.append(old, old, c.table.reserve(90))
+    with torch.no_grad():
+        for _ in range(3):
+            assert torch.equal(compiled(q, k, v), step(caches[1], q, k, v))
+    assert torch.equal(caches[0].scales, caches[1].scales)
+
+
+def test_tables_made_in_inference_mode():
+    with torch.inference_mode():
+        cache = _cache(2, 2, 64, 16, 100)
+        k = _randn(2, 2, 20, 64)
+        cache.append(k, k, cache.table.reserve(20))
+        out = cache.append_and_attend(_randn(2, 4, 1, 64), k[:, :, :1], k[:, :, :1], cache.table.reserve(1))
+    assert out.isfinite().all()
+
+
+def test_calls_on_two_streams():
+    """Caches of their own, on streams of their own, at the same time."""
+    caches = [_cache(4, 2, 128, 16, 3000, BF16, seed=i) for i in range(2)]
+    q = [_randn(4, 8, 1, 128, dtype=BF16, seed=i) for i in range(2)]
+    for i, c in enumerate(caches):
+        k = _randn(4, 2, 2900, 128, dtype=BF16, seed=10 + i)
+        c.append(k, k, c.table.reserve(2900))
+    want = [c.attend(x) for c, x in zip(caches, q)]
+    streams = [torch.cuda.Stream() for _ in caches]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(caches[i].attend(q[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for os, w in zip(got, want) for o in os)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_shapes(seed):
+    import random
+
+    rng = random.Random(seed)
+    dtype = rng.choice([F16, BF16])
+    d, page = 16 * rng.randint(1, 8), 16 * rng.choice([1, 2, 3, 5, 8])
+    hkv = rng.choice([1, 2, 3, 8])
+    hq, sq = hkv * rng.choice([1, 2, 5, 8, 16]), rng.choice([1, 1, 2, 3, 7])
+    lengths = [rng.choice([0, 1, rng.randint(1, 100), rng.randint(1, 2000)]) for _ in range(rng.randint(1, 9))]
+    print(dtype, d, page, hkv, hq, sq, lengths, flush=True)
+    _check(_case(len(lengths), hq, hkv, sq, d, page, lengths, dtype=dtype, seed=seed), causal=rng.random() < 0.5)

@@ -146,6 +146,12 @@ def test_gradients(dtype, interleaved, layout):
     for f in (lambda a, b: _HipRotary.apply(a, b, *args),
               lambda a, b: torch.ops.kotflash_amd.rotary(a, b, rot.turns, n, 0, interleaved, False, 0.75)):
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(f(q, k), (q, k), (gq, gk)), (dq, dk)))
+    both = torch.ops.kotflash_amd.rotary(q, k, rot.turns, n, 0, interleaved, False, 0.75)
+    assert torch.equal(torch.autograd.grad(both[1], k, gk)[0], dk)
+    compiled = torch.compile(lambda a, b: rot(a, b, positions=n), fullgraph=True, backend="aot_eager")
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(compiled(q, k), (q, k), (gq, gk)), (dq, dk)))
+    alone = torch.compile(lambda a: rot(a, positions=n), fullgraph=True, backend="aot_eager")
+    assert torch.equal(torch.autograd.grad(alone(q), q, gq)[0], dq)
     a, b = torch.autograd.grad(_HipRotary.apply(q, k, *args)[1], (q, k), gk, allow_unused=True)
     assert a is None and torch.equal(b, dk)
     # Queries alone, from an int position on.
