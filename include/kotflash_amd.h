@@ -368,7 +368,7 @@ int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const vo
 
 /*
  * The paged cache in 8 bits. Pools of e4m3 codes (OCP), laid out as the 16-bit
- * ones (strides in elements, multiples of 16; D a multiple of 16 up to 128,
+ * ones (strides in elements, multiples of 16; D a multiple of 8 up to 128,
  * page_size of 16), and scales: fp32 [num_pages, Hkv, page_size / 16, 2]
  * (scale_strides {page, head}, the rest contiguous), one for K and one for V of
  * every block of 16 rows of a page and head. A value is code * scale; scales
@@ -409,8 +409,10 @@ int kf_fp8_read(const void* k_pages, const void* v_pages, const float* scales, v
 
 /*
  * Attention of q (16-bit) over pools of codes as they read back in its type:
- * kf_paged_decode otherwise, with the scales and their strides. The workspace
- * has a size of its own.
+ * kf_paged_decode otherwise, with the scales and their strides. K and V pools
+ * have the same strides, and where D is not a multiple of 16, 8 bytes of padding
+ * behind every row, the last included, which are read and may hold anything.
+ * The workspace has a size of its own.
  */
 size_t kf_fp8_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);
 int kf_fp8_decode_check(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D,

@@ -750,6 +750,15 @@ PyObject* py_page_trim(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---------------------------------------------------------------------------
 // Paged cache in 8 bits.
 
+// Whether a row of 8 (2 n + 1) bytes has its last 8 bytes of padding in the
+// tensor's own storage, behind the last row too.
+bool row_padded(const Tensor& t) {
+  if (t.stride(2) < t.size(3) + 8) return false;
+  int64_t end = t.storage_offset() + t.size(3) + 8;
+  for (int i = 0; i < 3; ++i) end += (t.size(i) - 1) * t.stride(i);
+  return end <= (int64_t)t.storage().nbytes();
+}
+
 // Pools [pages, Hkv, page, D] of e4m3 and their scales [pages, Hkv, page / 16,
 // 2], as the kernels address them.
 struct Fp8Pools {
@@ -762,11 +771,13 @@ struct Fp8Pools {
       return false;
     const auto s = k->sizes();
     const int64_t want[4] = {s[0], s[1], s[2] / 16, 2};
-    if (s[2] % 16 || s[3] % 16 || s[3] > 128 || scales->sizes() != at::IntArrayRef(want, 4)) return false;
-    for (const Tensor* t : {k, v})
+    if (s[2] % 16 || s[3] % 8 || s[3] > 128 || scales->sizes() != at::IntArrayRef(want, 4)) return false;
+    for (const Tensor* t : {k, v}) {
       if (t->stride(3) != 1 || t->stride(0) % 16 || t->stride(1) % 16 || t->stride(2) % 16 ||
           reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16)
         return false;
+      if (s[3] % 16 && !row_padded(*t)) return false;
+    }
     return scales->stride(3) == 1 && scales->stride(2) == 2 && scales->stride(1) % 2 == 0 &&
            scales->stride(0) % 2 == 0 && reinterpret_cast<uintptr_t>(scales->const_data_ptr()) % 8 == 0 &&
            is_gfx950(k->device().index());

@@ -117,8 +117,8 @@ static void launch_merge(const PagedParams& p, hipStream_t stream) {
 template <typename T, int DT, int NW>
 static void launch_workers(const PagedParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.workers), block(64 * NW);
-  if (p.nnew > 0) hipLaunchKernelGGL((paged_kernel<T, DT, NW, true, false>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((paged_kernel<T, DT, NW, false, false>), grid, block, 0, stream, p);
+  if (p.nnew > 0) hipLaunchKernelGGL((paged_kernel<T, DT, NW, true, kPool16>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((paged_kernel<T, DT, NW, false, kPool16>), grid, block, 0, stream, p);
 }
 
 template <typename T, int DT>
@@ -267,7 +267,7 @@ static int paged_entry(const char* what, const void* q, const void* k_pages, con
     p.scales = scales.at;
     p.sc_page = (uint32_t)(4 * scales.strides[0]);
     p.sc_head = (uint32_t)(4 * scales.strides[1]);
-    p.row_rest = (int)(k_strides[2] - D);
+    p.row_rest = (int)(k_strides[2] - (D + 15) / 16 * 16);
   }
   p.o_sb = o_strides[0]; p.o_sh = o_strides[1]; p.o_ss = o_strides[2];
   p.B = (int)B; p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.Sq = (int)Sq; p.D = (int)D; p.G = (int)(Hq / Hkv);
@@ -343,17 +343,17 @@ extern "C" int kf_paged_append_decode(const void* q, void* k_pages, void* v_page
                      dtype, workspace, workspace_bytes, stream);
 }
 
-// 8-bit pools: head_dim and strides in whole 16-byte pieces.
+// 8-bit pools: rows of whole 16-byte pieces, the last one perhaps half padding.
 static int check_fp8_sizes(const char* what, int64_t D, int64_t num_pages, const int64_t* k_strides, const int64_t* v_strides,
                            const int64_t* scale_strides) {
   if (!scale_strides) return set_error(KF_EINVAL, "%s: null strides", what);
-  if (D % 16 || D > 128) return set_error(KF_EUNSUPPORTED, "%s: head_dim must be a multiple of 16 up to 128", what);
+  if (D % 8 || D > 128) return set_error(KF_EUNSUPPORTED, "%s: head_dim must be a multiple of 8 up to 128", what);
   for (const int64_t* s : {k_strides, v_strides})
     if (s[0] % 16 || s[1] % 16 || s[2] % 16)
       return set_error(KF_EINVAL, "%s: pool strides must be multiples of 16 bytes", what);
   if (k_strides[0] != v_strides[0] || k_strides[1] != v_strides[1] || k_strides[2] != v_strides[2])
     return set_error(KF_EINVAL, "%s: K and V pools must have the same strides", what);
-  if (k_strides[2] < D || 16 * k_strides[2] > 0x7fffffff)
+  if (k_strides[2] < (D + 15) / 16 * 16 || 16 * k_strides[2] > 0x7fffffff)
     return set_error(KF_EUNSUPPORTED, "%s: rows of a page overlap, or span more than 2 GiB", what);
   if (scale_strides[0] % 2 || scale_strides[1] % 2)
     return set_error(KF_EINVAL, "%s: scale strides must be multiples of a pair", what);

@@ -103,7 +103,7 @@ struct PagedParams {
   // 8-bit pools: the blocks' scales, in pairs (K, V); bytes per page and head.
   const float* scales;
   uint32_t sc_page, sc_head;
-  int row_rest;  // k_row without the row's own bytes
+  int row_rest;  // k_row without the row's own 16-byte pieces
 };
 
 // Direct-to-LDS loads (kf_common.hpp) of whole tiles: N loads of 1 KB, one
@@ -218,9 +218,11 @@ __device__ inline void worker_barrier() {
 // NW waves per worker, 16 packed rows each: they share the ring, every wave
 // loading a part of each step, and read all of it. FUSED: with the store of new
 // rows (in one kernel it costs calls without any up to 0.2 us, for scalars that
-// no longer fit the registers). KV8: pools of e4m3 codes with scales.
-template <typename T, int DT, int NW, bool FUSED, bool KV8>
+// no longer fit the registers).
+enum PoolKind { kPool16, kPool8, kPool8Padded };  // 16 bits; e4m3 codes; rows with padding
+template <typename T, int DT, int NW, bool FUSED, PoolKind POOL>
 __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) void paged_kernel(const PagedParams p) {
+  constexpr bool KV8 = POOL != kPool16;
   constexpr int STEP = kStepOf<KV8>;
   constexpr int GROUPS = STEP / 16;   // 16-row groups of a step
   constexpr int EB = KV8 ? 1 : 2;     // bytes of an element of K and V
@@ -627,6 +629,9 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
       for (int dc = 0; dc < NKA; ++dc) {
         const int key = kb * 16 + (KV8 && kb % 2 ? l16 ^ 8 : l16);
         ka[kb][dc] = lds_read16(Ks + Tile::chunk(key, 4 * dc + g16) * 8);
+        // The second half of a row's last piece: any codes, NaN among them,
+        // which zeros of Q do not silence.
+        if (POOL == kPool8Padded && 4 * dc + g16 == p.D / 16) ka[kb][dc][2] = ka[kb][dc][3] = 0;
       }
     bool masked;
     if constexpr (KV8) masked = valid[slot] != (1 << GROUPS) - 1 || w.rem - most_lag < STEP;

@@ -138,7 +138,7 @@ def attention_fp8(q, k_pages, v_pages, scales, tables, lengths, *, causal: bool,
 
 def pages_in_place(k_pages, v_pages, scales) -> bool:
     """Whether the kernels read and write these pools as they are."""
-    if k_pages.shape[3] % 16 or k_pages.shape[3] > 128:
+    if k_pages.shape[3] % 8 or k_pages.shape[3] > 128:
         return False
     for t, unit, granule in ((k_pages, 1, 16), (v_pages, 1, 16), (scales, 1, 2)):
         st = t.stride()
@@ -147,15 +147,28 @@ def pages_in_place(k_pages, v_pages, scales) -> bool:
         # There is no address under torch.compile; the ops check it.
         if not torch.compiler.is_compiling() and t.data_ptr() % (16 if t is not scales else 8):
             return False
+    if k_pages.shape[3] % 16 and not all(_row_padded(t) for t in (k_pages, v_pages)):
+        return False
     return scales.stride(2) == 2
+
+
+def _row_padded(t) -> bool:
+    """Whether a row of 8 (2 n + 1) bytes has its last 8 bytes of padding in the
+    tensor's own storage, behind the last row too."""
+    if t.stride(2) < t.shape[3] + 8:
+        return False
+    if torch.compiler.is_compiling():
+        return True
+    end = t.storage_offset() + t.shape[3] + 8 + sum((n - 1) * s for n, s in zip(t.shape[:3], t.stride()))
+    return end <= t.untyped_storage().nbytes()
 
 
 def require_in_place(what: str, k_pages, v_pages, scales) -> None:
     if not _hip.is_gfx950(k_pages.device):
         raise RuntimeError(f"{what} requires an AMD gfx950 (MI355X) device")
     if not pages_in_place(k_pages, v_pages, scales):
-        raise ValueError(f"{what} needs head_dim a multiple of 16 in [16, 128], inner-contiguous, 16-byte "
-                         "aligned K/V pages and scales in pairs")
+        raise ValueError(f"{what} needs head_dim a multiple of 8 in [8, 128], inner-contiguous K/V pages, "
+                         "rows and pages 16-byte aligned, and scales in pairs")
 
 
 def append_fp8(k_pages, v_pages, scales, new_k, new_v, slots) -> None:

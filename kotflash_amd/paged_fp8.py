@@ -17,7 +17,8 @@ scale. 16 positions of a page, one head, share a scale for K and one for V: the
 least power of two with which the largest fits. Powers of two make the product
 exact, so that a value is rounded once, by at most 2^-4 of itself. A
 block takes its scale when its first position is stored; a later token that is
-larger makes it grow, and the rows that are there are divided by the ratio (which
+larger makes it grow (for good, though a draft that is trimmed may be the one),
+and the rows that are there are divided by the ratio (which
 rounds only what falls below 2^-6 of the scale). Infinities are stored as NaN.
 Inference only. No counterpart in the reference (kotflash/cache.py:1-10).
 """
@@ -64,7 +65,8 @@ def fp8_append(k_pages, v_pages, scales, new_k, new_v, slots, *, backend: str = 
     and a pool takes one 16-bit type.
 
     ``auto`` takes ``hip`` for fp16 and bf16 on gfx950, for pools with a
-    head_dim that is a multiple of 16 up to 128; ``torch`` takes any."""
+    head_dim that is a multiple of 8 up to 128 and rows that begin at multiples
+    of 16 bytes; ``torch`` takes any."""
     if backend in ("auto", "hip") and not torch.compiler.is_compiling() \
             and _hip.native().fp8_append(k_pages, v_pages, scales, new_k, new_v, slots) is None:
         return
@@ -222,8 +224,8 @@ class PagedKVCacheFP8:
     share (with 16-bit caches too), whose page_size is a multiple of 16.
 
     ``k_pages`` and ``v_pages`` are float8_e4m3fn [num_pages, kv_heads,
-    page_size, head_dim], ``scales`` float32 [num_pages, kv_heads, page_size /
-    16, 2] (K, V). ``dtype`` is that of the tensors it takes and gives.
+    page_size, head_dim] (rows padded to 16 bytes), ``scales`` float32
+    [num_pages, kv_heads, page_size / 16, 2] (K, V). ``dtype`` is that of the tensors it takes and gives.
     """
 
     def __init__(self, table: PageTable, kv_heads: int, head_dim: int, *,
@@ -238,8 +240,10 @@ class PagedKVCacheFP8:
                  _positive("head_dim", head_dim))
         self.table, self.dtype = table, dtype
         device = table.tables.device
-        self.k_pages = torch.empty(shape, device=device, dtype=FP8)
-        self.v_pages = torch.empty_like(self.k_pages)
+        # Rows in whole pieces of 16 bytes, as the kernels load them.
+        wide = (*shape[:3], -(-head_dim // 16) * 16)
+        self.k_pages, self.v_pages = (torch.empty(wide, device=device, dtype=FP8)[..., :head_dim]
+                                      for _ in range(2))
         self.scales = torch.zeros((*shape[:2], table.page_size // BLOCK, 2), device=device)
 
     def append(self, new_k, new_v, slots, *, backend: str = "auto") -> None:

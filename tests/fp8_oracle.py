@@ -128,9 +128,12 @@ def make_cache(batch, hkv, d, page, lengths, *, dtype, seed, device="cpu", spare
             p = order.pop()
             tables[b, c] = p
             mine[p, :min(page, n - c * page)] = True
-    pools = [torch.where(mine[:, None, :, None], c, 127).to(torch.uint8).view(torch.float8_e4m3fn) for c in codes]
+    # Rows padded to 16 bytes, the padding NaN.
+    codes = [torch.cat((torch.where(mine[:, None, :, None], c, 127), torch.full((pages, hkv, page, -d % 16), 127)), 3)
+             for c in codes]
+    pools = [c.to(torch.uint8).to(device).view(torch.float8_e4m3fn)[..., :d] for c in codes]
     lens = torch.tensor(lengths, dtype=torch.int32)
-    return tuple(t.to(device) for t in (*pools, scales, tables, lens))
+    return (*pools, *(t.to(device) for t in (scales, tables, lens)))
 
 
 def assert_attention(got, q, k, v, tables, lengths, *, lse=None, **kw):

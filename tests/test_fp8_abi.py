@@ -22,7 +22,7 @@ POOLS = dict(k=P, v=P, scales=P, H=2, D=64, pages=8, page=16, ks=_arr(2048, 1024
 POOL_REFUSALS = [
     (dict(k=None), "null"), (dict(v=None), "null"), (dict(scales=None), "null"), (dict(ks=None), "strides"),
     (dict(ss=None), "strides"), (dict(H=0), "positive"), (dict(D=0), "positive"), (dict(pages=0), "positive"),
-    (dict(page=-16), "positive"), (dict(D=72), "multiple of 16 up to 128"), (dict(D=144), "multiple of 16 up to 128"),
+    (dict(page=-16), "positive"), (dict(D=76), "multiple of 8 up to 128"), (dict(D=136), "multiple of 8 up to 128"),
     (dict(page=24), "page_size must be a multiple of 16"), (dict(pages=2 ** 31), "too large"),
     (dict(pages=2 ** 30, page=64), "too large"), (dict(k=P + 8), "aligned"), (dict(scales=P + 4), "aligned"),
     (dict(vs=_arr(2048, 1024, 72)), "multiples of 16"), (dict(ss=_arr(4, 1)), "pair"),
@@ -61,7 +61,7 @@ DECODE = dict(q=P, tables=P, lengths=P, B=2, Hq=4, Hkv=2, Sq=1, columns=4, strid
 
 @pytest.mark.parametrize("kw,match", [
     (dict(scales=None), "scales"), (dict(scales=P + 4), "scales"), (dict(ks=None), "strides"), (dict(ss=None), "strides"),
-    (dict(B=0), "positive"), (dict(Hq=3), "divisible"), (dict(D=72), "multiple of 16"), (dict(D=144), "multiple of 16"),
+    (dict(B=0), "positive"), (dict(Hq=3), "divisible"), (dict(D=76), "multiple of 8"), (dict(D=136), "multiple of 8"), (dict(D=72), "overlap"),
     (dict(dtype=7), "dtype"), (dict(q=None), "q is null"), (dict(k=P + 8), "k_pages must be 16-byte"),
     (dict(ks=_arr(2048, 1024, 72)), "multiples of 16"), (dict(vs=_arr(4096, 1024, 64)), "same strides"),
     (dict(ks=_arr(2048, 1024, 48), vs=_arr(2048, 1024, 48)), "overlap"),
@@ -79,7 +79,7 @@ def test_decode(kw, match):
                                      a["ws_bytes"], None), match)
 
 
-@pytest.mark.parametrize("kw,match", [({}, None), (dict(D=72), "multiple of 16"), (dict(B=0), "positive"), (dict(ss=None), "strides"),
+@pytest.mark.parametrize("kw,match", [({}, None), (dict(D=76), "multiple of 8"), (dict(D=56), None), (dict(D=72), "overlap"), (dict(B=0), "positive"), (dict(ss=None), "strides"),
                                       (dict(pages=2 ** 28), "4 GiB"), (dict(Sq=2 ** 24, Hkv=1), "grid")])
 def test_decode_check(kw, match):
     a = {**POOLS, **DECODE, **kw}
@@ -93,7 +93,7 @@ def test_decode_check(kw, match):
 
 def test_workspace_size():
     size = _hip.lib().kf_fp8_decode_workspace_bytes
-    assert size(0, 4, 2, 1, 64) == 0 and size(2, 3, 2, 1, 64) == 0 and size(2, 4, 2, 1, 144) == 0
+    assert size(0, 4, 2, 1, 64) == 0 and size(2, 3, 2, 1, 64) == 0 and size(2, 4, 2, 1, 136) == 0
     for b, hq, hkv, sq, d in ((1, 1, 1, 1, 16), (64, 32, 8, 1, 128), (8, 64, 1, 3, 64)):
         rows = min(64, hq // hkv * sq)
         assert size(b, hq, hkv, sq, d) >= (256 + b * hkv) * rows * (d + 1) * 4

@@ -33,7 +33,7 @@ def _same(a, b):
 # --- store -------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 48, 56, 64, 72, 80, 88, 96, 104, 112, 120, 128])
 def test_append_dims(dtype, d):
     """Prompts, tokens and drafts that make blocks grow."""
     cache = _cache(3, 2, d, 32, 160, dtype, seed=d)
@@ -131,7 +131,7 @@ def test_append_layouts():
 # --- read --------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("d,page", [(16, 16), (48, 48), (64, 16), (80, 32), (128, 16), (128, 256)])
+@pytest.mark.parametrize("d,page", [(8, 16), (16, 16), (40, 48), (48, 48), (64, 16), (72, 16), (80, 32), (128, 16), (128, 256)])
 def test_read(dtype, d, page):
     lengths = [0, 1, 15, 16, 17, 100, 300]
     k8, v8, scales, tables, lens = make_cache(7, 2, d, page, lengths, dtype=dtype, seed=d, device="cuda")
@@ -186,7 +186,8 @@ def test_versions_and_refusals():
     before = [t._version for t in (k8, v8, scales)]
     fp8_append(k8, v8, scales, k, k, slots)
     assert all(t._version > n for t, n in zip((k8, v8, scales), before))
-    with pytest.raises(ValueError, match="head_dim a multiple of 16"):
+    # Rows of 24 bytes without their padding, and at the end of the storage.
+    with pytest.raises(ValueError, match="16-byte aligned"):
         odd = [torch.zeros(2, 1, 16, 24, device="cuda").to(FP8) for _ in range(2)]
         fp8_read(*odd, torch.zeros(2, 1, 1, 2, device="cuda"), tables, lens, 4, dtype=F16, backend="hip")
     with pytest.raises(TypeError, match="float16 and bfloat16"):
@@ -195,6 +196,10 @@ def test_versions_and_refusals():
         fp8_append(k8, v8, scales, k.clone().requires_grad_(), k, slots)
     with pytest.raises(ValueError, match="device"):
         fp8_append(k8, v8, scales, k, k, slots.cpu())
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        short = torch.zeros(2 * 16 * 32 - 8, dtype=torch.uint8, device="cuda").view(FP8)
+        odd = [short.as_strided((2, 1, 16, 24), (512, 512, 32, 1)) for _ in range(2)]
+        fp8_read(*odd, torch.zeros(2, 1, 1, 2, device="cuda"), tables, lens, 4, dtype=F16, backend="hip")
     # What the kernels do not take, auto runs in torch.
     odd = [torch.zeros(2, 1, 16, 24, device="cuda").to(FP8) for _ in range(2)]
     sc = torch.zeros(2, 1, 1, 2, device="cuda")
@@ -273,7 +278,7 @@ def _check(case, causal=False, scale=None, **kw):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 48, 56, 64, 72, 80, 88, 96, 104, 112, 120, 128])
 @pytest.mark.parametrize("wild", [False, True])
 def test_attention_dims(dtype, d, wild):
     _check(_case(4, 8, 2, 1, d, 16, [1, 70, 333, 1000], dtype=dtype, seed=d, wild=wild))
@@ -401,10 +406,18 @@ def test_attention_paths_agree():
     assert (sdpa[0] - want[0]).abs().max() < 4e-3 and (sdpa[1] - want[1]).abs().max() < 2e-3
     # What the kernels do not take, auto runs there.
     odd = make_cache(2, 1, 24, 16, [5, 30], dtype=F16, seed=1, device="cuda")
+    odd = (*(t.view(torch.uint8).contiguous().view(FP8) for t in odd[:2]), *odd[2:])
     out = fp8_attention(_randn(2, 4, 1, 24), *odd)
     assert_attention(out, _randn(2, 4, 1, 24), *Cache(*odd[:3]).held(F16), *odd[3:])
-    with pytest.raises(ValueError, match="head_dim"):
+    with pytest.raises(ValueError, match="16-byte aligned"):
         fp8_attention(_randn(2, 4, 1, 24), *odd, backend="hip")
+    # Pools of different strides: attention needs them alike.
+    q, k8, v8, scales, tables, lens = case
+    other = torch.cat((v8.view(torch.uint8),) * 2, 3).view(FP8)[..., :64]
+    got = fp8_attention(q, k8, other, scales, tables, lens, causal=True, return_lse=True)
+    assert (got[0] - want[0]).abs().max() < 4e-3
+    with pytest.raises(RuntimeError, match="same strides"):
+        fp8_attention(q, k8, other, scales, tables, lens, backend="hip")
 
 
 def test_attention_beyond_32_bits():
@@ -552,7 +565,7 @@ def test_random_shapes(seed):
 
     rng = random.Random(seed)
     dtype = rng.choice([F16, BF16])
-    d, page = 16 * rng.randint(1, 8), 16 * rng.choice([1, 2, 3, 5, 8])
+    d, page = 8 * rng.randint(1, 16), 16 * rng.choice([1, 2, 3, 5, 8])
     hkv = rng.choice([1, 2, 3, 8])
     hq, sq = hkv * rng.choice([1, 2, 5, 8, 16]), rng.choice([1, 1, 2, 3, 7])
     lengths = [rng.choice([0, 1, rng.randint(1, 100), rng.randint(1, 2000)]) for _ in range(rng.randint(1, 9))]
