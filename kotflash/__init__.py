@@ -15,6 +15,8 @@ object: module state, ``isinstance`` checks and monkeypatching are shared.
     kotflash._planning       kotflash_amd._planning
     kotflash._cuda_append    kotflash_amd._hip_append (append_kv_cuda)
     kotflash.paged           kotflash_amd.paged (no reference module)
+    kotflash.paged_fp8       kotflash_amd.paged_fp8 (no reference module)
+    kotflash.rotary          kotflash_amd.rotary (no reference module)
     kotflash.kernels.*       kotflash.kernels (triton_* names -> hip_* modules)
 
 As in the reference, the package attribute ``kotflash.attention`` is the
@@ -30,6 +32,8 @@ _SUBMODULES = {
     "_planning": "kotflash_amd._planning",
     "_cuda_append": "kotflash_amd._hip_append",
     "paged": "kotflash_amd.paged",
+    "paged_fp8": "kotflash_amd.paged_fp8",
+    "rotary": "kotflash_amd.rotary",
 }
 for _name, _target in _SUBMODULES.items():
     _sys.modules[f"{__name__}.{_name}"] = _importlib.import_module(_target)
@@ -38,7 +42,7 @@ from . import kernels  # noqa: E402  (registers kotflash.kernels.triton_*)
 from kotflash_amd import __version__, attention, hip_available  # noqa: E402
 from kotflash_amd.kernels.hip_forward import triton_available, triton_turing_supported  # noqa: E402
 
-for _name in ("cache", "_planning", "_cuda_append", "paged"):
+for _name in ("cache", "_planning", "_cuda_append", "paged", "paged_fp8", "rotary"):
     globals()[_name] = _sys.modules[f"{__name__}.{_name}"]
 del _name, _target
 
