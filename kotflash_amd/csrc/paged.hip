@@ -78,13 +78,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(cons
 
 // Workers: what 256 CUs hold of them at once.
 template <int NW>
-static int workers_of(int DT) {
-  return 256 * (DT == 32 ? workers_per_cu(32, NW) : DT == 64 ? workers_per_cu(64, NW)
-                : DT == 96 ? workers_per_cu(96, NW) : workers_per_cu(128, NW));
+static int workers_of(int DT, bool kv8) {
+  return 256 * (DT == 32 ? workers_per_cu(32, NW, kv8) : DT == 64 ? workers_per_cu(64, NW, kv8)
+                : DT == 96 ? workers_per_cu(96, NW, kv8) : workers_per_cu(128, NW, kv8));
 }
 static int paged_workers(int64_t D, int64_t R, bool kv8) {
   const int DT = paged_tile(D, kv8), NW = paged_waves(R);
-  return NW == 1 ? workers_of<1>(DT) : NW == 2 ? workers_of<2>(DT) : workers_of<4>(DT);
+  return NW == 1 ? workers_of<1>(DT, kv8) : NW == 2 ? workers_of<2>(DT, kv8) : workers_of<4>(DT, kv8);
 }
 
 static int64_t paged_slots(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D, bool kv8) {

@@ -202,9 +202,11 @@ constexpr int worker_lds(int DT, int NW) { return 2 * (2 * 64 * DT + NW * q_load
 // bytes, and by waves (two per SIMD, four of four-wave workers: 16 requests up
 // to 16384 tokens, 8 KV heads, D=64, us with 8, 12 and 16 waves: 32 rows 58.2,
 // 61.6 and 61.4, 64 rows 89.4, 77.1 and 72.6; D=128 is bound by the LDS).
-constexpr int workers_per_cu(int DT, int NW) {
+// In 8 bits the two-wave ones up to three per SIMD (32 rows 52.0 and 48.7; D=128 is
+// bound by the LDS there too).
+constexpr int workers_per_cu(int DT, int NW, bool kv8) {
   const int by_lds = 160 * 1024 / ((worker_lds(DT, NW) + 1279) / 1280 * 1280);
-  const int by_waves = NW == 4 ? 4 : 8 / NW;
+  const int by_waves = NW == 4 ? 4 : NW == 2 && kv8 ? 6 : 8 / NW;
   return by_lds < by_waves ? by_lds : by_waves;
 }
 
@@ -221,7 +223,7 @@ __device__ inline void worker_barrier() {
 // no longer fit the registers).
 enum PoolKind { kPool16, kPool8, kPool8Padded };  // 16 bits; e4m3 codes; rows with padding
 template <typename T, int DT, int NW, bool FUSED, PoolKind POOL>
-__global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) void paged_kernel(const PagedParams p) {
+__global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW, POOL != kPool16) * NW + 3) / 4) void paged_kernel(const PagedParams p) {
   constexpr bool KV8 = POOL != kPool16;
   constexpr int STEP = kStepOf<KV8>;
   constexpr int GROUPS = STEP / 16;   // 16-row groups of a step
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW) * NW + 3) / 4) voi
     static_for<0, 2>([&](auto sc) {
       constexpr int slot = decltype(sc)::value;
       const int j = j0 + slot;
-      if constexpr (KV8 && NW == 1 && workers_per_cu(DT, NW) > 4) {
+      if constexpr (KV8 && NW == 1 && workers_per_cu(DT, NW, true) > 4) {
         if (late && j % 4 != 0) __builtin_amdgcn_s_setprio(1);
         else __builtin_amdgcn_s_setprio(0);
       }
