@@ -458,7 +458,7 @@ extern "C" int kf_fp8_read(const void* k_pages, const void* v_pages, const float
     return set_error(KF_EUNSUPPORTED, "%s: a table of %lld pages of %lld tokens is beyond 32-bit positions", what,
                      (long long)columns, (long long)page_size);
   Fp8ReadParams p{};
-    const int64_t pieces = D / 8, blocks = (width * pieces + 255) / 256;
+  const int64_t pieces = D / 8, blocks = (width * pieces + 255) / 256;
   if (width > 0x3fffffff / pieces || start > 0x3fffffff)
     return set_error(KF_EUNSUPPORTED, "%s: width or start too large", what);
   if (B > 0x7fffffff / H || B * H > ((1ll << 24) - 1) / blocks) return set_error(KF_EUNSUPPORTED, "%s: grid too large", what);
