@@ -538,9 +538,13 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW, POOL != kPool16) *
         for (int j = 0; j < (NW > 1 ? GROUPS / 2 : GROUPS); ++j) {
           const int g = NW > 1 ? 2 * j : j, mine = NW > 1 ? g + odd : g;
           const uint32_t i = NW > 1 && odd ? id[g + 1] : id[g], r = NW > 1 && odd ? row[g + 1] : row[g];
-          const uint64_t off = (uint64_t)i * p.k_page + r * p.k_row;
+          // A page's rows may be more than 4 GiB apart, where pages lie inside
+          // a position's; 16 of them are less than 2.
+          const uint64_t off = (uint64_t)i * p.k_page + (uint64_t)r * p.k_row;
+          // (Not a clamp to 0 as well: that is a vector instruction, and a
+          // resource is in scalar registers.)
           const int rows = min(NW > 1 && odd ? left[g + 1] : left[g], 16);
-          const int extent = max(rows * (int)p.k_row - p.row_rest, 0);
+          const uint32_t extent = rows > 0 ? (uint32_t)rows * p.k_row - (uint32_t)p.row_rest : 0u;
           const uint32_t m0 = kv0 + mine * 16 * DT;
           if (NW < 4) {
             dma_tile<NGI, decltype(nt)::value>(make_rsrc((const void*)(uintptr_t)(kh + off), extent), m0, koff);
