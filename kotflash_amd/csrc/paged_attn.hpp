@@ -665,6 +665,13 @@ __global__ __launch_bounds__(64 * NW, (workers_per_cu(DT, NW, POOL != kPool16) *
     }
     // Masked after the scale, so that a scale of zero leaves -inf.
     if (masked) {
+      // A group without visible rows has codes of zero; its block's scale may be
+      // anything (never written, or that of another request's page): 0 V.
+      if constexpr (KV8) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          if (seen_of(w, slot, g) == 0) scale8[slot][g][1] = 1.f;
+      }
 #pragma unroll
       for (int kb = 0; kb < GROUPS; ++kb)
 #pragma unroll
