@@ -7,9 +7,10 @@
 // as they are. `inverse` turns by -a: with the same amplitude that is the
 // transpose, so the gradient's kernel too.
 //
-// Angles. f_i / 2 pi comes as a 64-bit fraction of a turn, F_i / 2^64. n F_i mod
-// 2^64 is then the angle's fraction of a turn with an error of n / 2^65, for
-// any 64-bit n, negative ones too; its top 32 bits are kept (2^-32 of a turn).
+// Angles. f_i / 2 pi comes as a 64-bit fraction of a turn, F_i / 2^64, rounded
+// to the nearest. n F_i mod 2^64 is then the angle's fraction of a turn with an
+// error of n / 2^65, negative n too; its top 32 bits are kept (2^-32 of a turn;
+// the table's error reaches that at n = 2^33, and 2^-22 rad at 2^40).
 // In fp32 the product n f_i alone would be off by 0.03 rad at n = 10^6. The
 // nearest quarter turn leaves |x| <= pi / 4 for Taylor polynomials in fp32:
 // sin to x^9 (next term 2e-9), cos to x^8 (3e-8).

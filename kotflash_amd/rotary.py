@@ -16,6 +16,7 @@ takes what it is given (kotflash/attention.py:223-312).
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 from typing import Optional, Sequence, Union
 
 import torch
@@ -27,6 +28,9 @@ ROTARY_BACKENDS = ("auto", "hip", "torch")
 SCALINGS = ("none", "linear", "base", "ramp")
 
 _HALF = (torch.float16, torch.bfloat16)
+
+# To 50 digits: a double's 2 pi would leave 53 of the table's 64 bits.
+_TWO_PI = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
 
 
 def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str = "none",
@@ -128,8 +132,9 @@ class Rotary:
     ``amplitude``.
 
     ``turns`` (int64 [rotary_dim / 2], on the device) holds f_i / 2 pi in units
-    of 2^-64 turns: products with positions wrap at whole turns, so angles are
-    right for positions of any size.
+    of 2^-64 turns, rounded once from the frequencies as doubles
+    (``frequencies``): products with positions wrap at whole turns, and the angle
+    at position n is off by at most n / 2^65 of a turn (2^-22 of a radian at 2^40).
     """
 
     def __init__(self, head_dim: int, *, rotary_dim: Optional[int] = None, base: float = 10000.0,
@@ -158,7 +163,7 @@ class Rotary:
         self.interleaved = interleaved
         self.amplitude = float(amplitude)
         self.frequencies = tuple(computed)
-        self.turns = torch.tensor([round(x / (2 * math.pi) * 2.0 ** 64) for x in computed],
+        self.turns = torch.tensor([round(Fraction(x) * 2 ** 64 / _TWO_PI) for x in computed],
                                   dtype=torch.int64, device=device)
 
     def __call__(self, q, k=None, *, positions: Union[int, torch.Tensor] = 0, backend: str = "auto"):
