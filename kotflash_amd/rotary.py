@@ -20,6 +20,7 @@ from fractions import Fraction
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 from .kernels import hip_rotary
@@ -101,6 +102,14 @@ class _HipRotary(torch.autograd.Function):
         return (*grads, None, None, None, None, None)
 
 
+def _transformed(*tensors) -> bool:
+    """Whether a torch.func transform or a forward-mode gradient is under way:
+    the kernel's autograd node has reverse mode alone."""
+    return not torch.compiler.is_compiling() and (
+        torch._C._are_functorch_transforms_active()
+        or any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t is not None))
+
+
 def _torch_rotate(x, turns, positions, interleaved: bool, amplitude: float):
     """The same in torch operations, in fp32 (fp64 for fp64)."""
     b, _, s, _ = x.shape
@@ -172,8 +181,10 @@ class Rotary:
         int), ``positions[b] + t`` (int32 or int64 [B], on the device) or
         ``positions[b, t]`` ([B, S], or [1, S] for all).
 
-        ``auto`` takes ``hip`` for fp16 and bf16 on gfx950; ``torch`` takes any
-        floating-point type, and computes in 32 bits (64 for fp64)."""
+        ``auto`` takes ``hip`` for fp16 and bf16 on gfx950, but not under
+        torch.func's transforms and forward-mode gradients, which ``hip``
+        refuses; ``torch`` takes any floating-point type, and computes in 32 bits
+        (64 for fp64)."""
         if backend in ("auto", "hip") and not torch.compiler.is_compiling():
             out = _hip.native().rotary(q, k, self.turns, positions, self.head_dim, self.interleaved,
                                        self.amplitude)
@@ -187,7 +198,13 @@ class Rotary:
             raise RuntimeError("HIP backend requires an AMD MI355X (gfx950) GPU")
         if backend == "hip" and q.dtype not in _HALF:
             raise TypeError(f"HIP rotary supports float16 and bfloat16, got {q.dtype}")
-        if backend == "torch" or not on_gfx950 or q.dtype not in _HALF:
+        on_hip = backend != "torch" and on_gfx950 and q.dtype in _HALF
+        if on_hip and _transformed(q, k):
+            if backend == "hip":
+                raise RuntimeError("HIP rotary has no torch.func transforms and forward-mode gradients; "
+                                   "backend='torch' has")
+            on_hip = False
+        if not on_hip:
             out = tuple(None if x is None else
                         _torch_rotate(x, self.turns, positions, self.interleaved, self.amplitude)
                         for x in (q, k))
