@@ -15,11 +15,14 @@ reads, of ``PagedKVCache`` behind the same ``PageTable``.
 Keys and values are codes of e4m3 (4 significant bits, largest 448) times a
 scale. 16 positions of a page, one head, share a scale for K and one for V: the
 least power of two with which the largest fits. Powers of two make the product
-exact, so that a value is rounded once, by at most 2^-4 of itself. A
+exact, so that a value is rounded once, by at most 2^-4 of itself, or 2^-10 of
+the scale if that is more: codes below 2^-6 have a step of 2^-9, and values
+below 2^-10 of the scale (4.4e-6 of the largest it was made for) become zero. A
 block takes its scale when its first position is stored; a later token that is
 larger makes it grow (for good, though a draft that is trimmed may be the one),
-and the rows that are there are divided by the ratio (which
-rounds only what falls below 2^-6 of the scale). Infinities are stored as NaN.
+and the rows that are there are divided by the ratio, which rounds what falls
+below 2^-6 of the new scale again, by up to 2^-10 of it. Infinities are stored
+as NaN.
 Inference only. No counterpart in the reference (kotflash/cache.py:1-10).
 """
 from __future__ import annotations
