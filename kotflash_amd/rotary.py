@@ -172,8 +172,10 @@ class Rotary:
         self.interleaved = interleaved
         self.amplitude = float(amplitude)
         self.frequencies = tuple(computed)
-        self.turns = torch.tensor([round(Fraction(x) * 2 ** 64 / _TWO_PI) for x in computed],
-                                  dtype=torch.int64, device=device)
+        # An inference tensor could not be saved for a backward pass later.
+        with torch.inference_mode(False):
+            self.turns = torch.tensor([round(Fraction(x) * 2 ** 64 / _TWO_PI) for x in computed],
+                                      dtype=torch.int64, device=device)
 
     def __call__(self, q, k=None, *, positions: Union[int, torch.Tensor] = 0, backend: str = "auto"):
         """q [B, Hq, S, D] and k [B, Hk, S, D] turned, as new tensors; q alone

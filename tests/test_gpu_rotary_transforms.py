@@ -59,3 +59,11 @@ def test_hip_refuses(rot):
         torch.func.jvp(lambda x: rot(x, backend="hip"), (q,), (t,))
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="backend='torch'"):
         rot(forward_ad.make_dual(q, t), backend="hip")
+
+
+def test_made_in_inference_mode():
+    with torch.inference_mode():
+        made = Rotary(64, device="cuda")
+    q, g = _randn(2, 4, 5, 64).requires_grad_(), _randn(2, 4, 5, 64, seed=1)
+    dq, = torch.autograd.grad(made(q, positions=9), q, g)
+    assert torch.equal(dq, torch.autograd.grad(Rotary(64, device="cuda")(q, positions=9), q, g)[0])

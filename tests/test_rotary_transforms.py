@@ -15,3 +15,11 @@ def test_transforms():
     leaf = q[0].clone().requires_grad_()
     want, = torch.autograd.grad(rot(leaf, positions=9), leaf, t[0])
     assert torch.equal(back, want)
+
+
+def test_made_in_inference_mode():
+    with torch.inference_mode():
+        rot = Rotary(16, device="cpu")
+    assert not rot.turns.is_inference()
+    q = torch.randn(1, 2, 3, 16).requires_grad_()
+    assert torch.autograd.grad(rot(q).sum(), q)[0].shape == q.shape
