@@ -382,7 +382,8 @@ int kf_paged_append_decode(const void* q, void* k_pages, void* v_pages, const vo
  * that grows, the block's other rows are divided by the ratio and rounded. Codes
  * are rounded to even; infinities become NaN; a code that would stand for 2^16
  * (fp16) or 2^128 (bf16) is the one below. Slots that are not skipped must differ,
- * and those of one block be of one request and follow one another. new_k/new_v
+ * and those of one block be of one request and follow one another, with none
+ * skipped between them. new_k/new_v
  * have a unit head_dim stride, 16-byte aligned bases and strides that are
  * multiples of 8 elements (int64_t[3]).
  */
@@ -412,6 +413,7 @@ int kf_fp8_read(const void* k_pages, const void* v_pages, const float* scales, v
  * kf_paged_decode otherwise, with the scales and their strides. K and V pools
  * have the same strides, and where D is not a multiple of 16, 8 bytes of padding
  * behind every row, the last included, which are read and may hold anything.
+ * So may scales of blocks that hold none of a request's first lengths[b] rows.
  * The workspace has a size of its own.
  */
 size_t kf_fp8_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t D);

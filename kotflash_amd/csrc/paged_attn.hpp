@@ -49,8 +49,8 @@
 // cache. A step has 64 keys, for the same bytes in flight. Half the bytes per
 // key leave the scalar unit, which builds a resource per 16 rows and reads pages
 // and scales, and the vector unit half the time for each key: 64 requests of 512
-// to 8192 tokens (Hq=32 Hkv=8), 16-bit and 8-bit, D=128 185 and 102 us, D=64 100
-// and 59: 6.2, 5.7, 5.8 and 5.0 TB/s. What is left at D=64 is the tail: equal runs
+// to 8192 tokens (Hq=32 Hkv=8), 16-bit and 8-bit, D=128 185 and 103 us, D=64 99
+// and 59: 6.2, 5.6, 5.8 and 5.0 TB/s. What is left at D=64 is the tail: equal runs
 // end after 40 to 50 us, by where on the chip they are.
 #pragma once
 #include "decode_merge.hpp"

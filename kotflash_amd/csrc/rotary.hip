@@ -152,7 +152,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   }
 }
 
-// Any strides and any even R: a thread per pair, or element that passes.
+// Any strides and any even R: a thread per pair, or element that passes. Bound
+// by instructions (64-bit divisions, an angle per head) and 2-byte accesses, at a
+// quarter to a seventh of a copy's rate: 40 heads, 32768 tokens, D = R = 72 285
+// us (a copy 71), 40 166 (40), R = 56 of D = 112 665 (109).
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_plain_kernel(const RotaryParams p, int interleaved) {
   const int half = p.R / 2, items = half + p.D - p.R;

@@ -64,8 +64,8 @@ def fp8_append(k_pages, v_pages, scales, new_k, new_v, slots, *, backend: str = 
     row), with ``scales`` (float32 [pages, Hkv, page_size / 16, 2]; zeros before
     the first call). Slots outside the pool (-1 in the padding of ``reserve``)
     are skipped. Two tokens of a call must not share a slot, tokens of one
-    block must follow one another in one request (``reserve`` gives them so),
-    and a pool takes one 16-bit type.
+    block must follow one another in one request, with no skipped slot between
+    (``reserve`` gives them so), and a pool takes one 16-bit type.
 
     ``auto`` takes ``hip`` for fp16 and bf16 on gfx950, for pools with a
     head_dim that is a multiple of 8 up to 128 and rows that begin at multiples
